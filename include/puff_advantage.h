@@ -36,6 +36,8 @@ extern "C" {
 #define PUFF_ERR_WORKSPACE     -9   /* scratch / workspace too small or missing   */
 #define PUFF_ERR_SIZE         -10   /* size beyond what the entry point supports  */
 #define PUFF_ERR_DEVICE_BOUNDS -11  /* debug builds (PUFF_DEBUG_BOUNDS): a kernel formed an out-of-range index (see _device_status) */
+#define PUFF_ERR_DTYPE        -12   /* unknown element type                       */
+#define PUFF_ERR_VALUE        -13   /* a scalar argument is outside its range     */
 
 /* ---- kernel variants ----------------------------------------------------- */
 #define PUFF_VARIANT_AUTO       0   /* pick from (num_segments, horizon, alignment): a bit-exact serial kernel,
@@ -308,6 +310,140 @@ int puff_rollout_sm100_write(float* rewards, float* terminals, float* values,
 int puff_priorities_sm100_weights_noalloc(const float* seg_abs_sum, float* weights,
                                           double* total_w, float alpha,
                                           long long num_segments, void* cuda_stream);
+
+/*
+ * ---- the policy update -----------------------------------------------------
+ *
+ * What a trainer computes from the advantages on: the log-probability and
+ * entropy of the chosen actions from the policy's logits (the reference's
+ * sample_logits, pufferlib/pytorch.py), the clipped policy loss
+ * (pufferl.py:390-411, 422), and the gated linear recurrence of a policy
+ * that is read along the horizon.  All on DEVICE buffers, asynchronous on
+ * `cuda_stream`; nothing is allocated.  dtype names the element type of the
+ * `void*` arrays; sums, softmax statistics and states are fp32 or fp64 whatever
+ * it is.  Outputs may not overlap inputs or one another (PUFF_ERR_ALIAS).
+ */
+#define PUFF_DTYPE_F32   0
+#define PUFF_DTYPE_F16   1
+#define PUFF_DTYPE_BF16  2
+
+/*
+ * Log-probability and entropy of one action per row of logits.  With
+ * z = logits / temperature and p = softmax(z):
+ *     logprobs[r] = log p[actions[r]]       entropy[r] = -sum_j p_j log p_j
+ * Rows are addressed as [outer, inner] with a stride each, in elements, so that
+ * a slice of [sequences, steps, vocab] needs no copy; the elements of a row are
+ * adjacent.  entropy (nullable), logprobs: fp32 [outer * inner], contiguous.
+ * row_stats (nullable): 2 fp32 per row for the backward pass, 8-byte aligned.
+ * A logit of -inf is an action that cannot be taken.  A row with nothing but
+ * -inf has log-probability -inf, entropy 0 and no gradient.  actions[r] < 0
+ * marks padding: log-probability and entropy 0, no gradient, its logits are not
+ * read.  actions[r] >= vocab does the same and raises the flag that
+ * puff_policy_sm100_bad_action() returns (and clears) after synchronising.
+ *
+ * _backward: dlogits (contiguous [outer * inner, vocab], every row written) =
+ *     (dlogprobs (onehot - p) - dentropy p (log p + entropy)) / temperature
+ * dentropy nullable (then entropy may be too).
+ */
+int puff_policy_sm100_logprobs(const void* logits, int dtype, const long long* actions,
+                               long long outer, long long inner, long long vocab,
+                               long long logits_outer_stride, long long logits_inner_stride,
+                               long long actions_outer_stride, long long actions_inner_stride,
+                               float temperature, float* logprobs, float* entropy,
+                               float* row_stats, void* cuda_stream);
+int puff_policy_sm100_logprobs_backward(const void* logits, int dtype, const long long* actions,
+                                        long long outer, long long inner, long long vocab,
+                                        long long logits_outer_stride, long long logits_inner_stride,
+                                        long long actions_outer_stride, long long actions_inner_stride,
+                                        float temperature, const float* row_stats,
+                                        const float* entropy, const float* dlogprobs,
+                                        const float* dentropy, void* dlogits, void* cuda_stream);
+int puff_policy_sm100_bad_action(void);
+
+/*
+ * Clipped policy loss over [rows, steps] tokens (all arrays contiguous fp32,
+ * mask one byte per token, 0 = not part of the loss).  Per token, with
+ * d = logprobs - old_logprobs, r = e^d, A = advantages, q = ref_logprobs - logprobs:
+ *     policy = max(-A r, -A clip(r, 1 - clip_low, 1 + clip_high))
+ *     kl     = e^q - 1 - q                        (0 without ref_logprobs)
+ *     loss   = mean(policy) + kl_coef mean(kl) - ent_coef mean(entropy)
+ * reduction PUFF_MEAN_TOKENS: means over all unmasked tokens.
+ * PUFF_MEAN_SEQUENCES: means over the rows that have an unmasked token of the
+ * row's mean over its unmasked tokens.  denominator > 0 takes the place of the
+ * number of tokens (or of rows) in those means: the count over all micro-batches
+ * or ranks that one update sums over; 0 counts this call's own.  Where nothing
+ * is unmasked the loss is 0.  What is masked is not read into any result,
+ * whatever its value.
+ * Outputs: loss [1]; ratio [rows, steps] (1 where masked; the `importance` of
+ * the advantage op); stats [6] = mean policy, mean kl, mean entropy as they
+ * enter the loss, then over the unmasked tokens the means of -d, of e^d - 1 - d
+ * and of "r outside the clip range" (old_approx_kl, approx_kl and clipfrac of
+ * pufferl.py:396-398).
+ * advantage_per_row != 0: advantages is [rows], one for all tokens of a row.
+ * For the backward pass, all nullable together: slope [rows, steps], weight [1],
+ * row_scale [rows] (PUFF_MEAN_SEQUENCES only).  scratch: at least
+ * puff_policy_sm100_loss_scratch_bytes bytes, 8-byte aligned, owned by the caller
+ * and by this call alone until the stream has passed it.
+ *
+ * _backward: dlogprobs and dentropy (nullable each) from the saved arrays and
+ * dloss [1] on the device.
+ */
+#define PUFF_MEAN_TOKENS     0
+#define PUFF_MEAN_SEQUENCES  1
+size_t puff_policy_sm100_loss_scratch_bytes(long long rows, long long steps);
+int puff_policy_sm100_loss(const float* logprobs, const float* old_logprobs, const float* advantages,
+                           int advantage_per_row, const float* ref_logprobs, const float* entropy,
+                           const unsigned char* mask, double clip_low, double clip_high,
+                           float kl_coef, float ent_coef, int reduction, double denominator,
+                           long long rows, long long steps, float* loss, float* ratio, float* stats,
+                           float* slope, float* row_scale, float* weight,
+                           void* scratch, size_t scratch_bytes, void* cuda_stream);
+int puff_policy_sm100_loss_backward(const float* slope, const float* row_scale, const float* weight,
+                                    const float* dloss, const unsigned char* mask, float ent_coef,
+                                    long long rows, long long steps, float* dlogprobs,
+                                    float* dentropy, void* cuda_stream);
+
+/*
+ * Gated linear recurrence over [batch, steps, channels], per channel:
+ *     f_t = sigmoid(gates_t)
+ *     h_t = f_t h_{t-1} + (1 - f_t) inputs_t,  h_{t-1} taken as 0 where resets_t != 0
+ * gates and inputs: `dtype`, a stride for batch and steps each, in elements,
+ * channels adjacent (two halves of one projection need no copy).  resets
+ * (nullable): [batch, steps] contiguous, fp32 (reset_bytes 4, the `terminals` of
+ * the experience buffers) or one byte each (reset_bytes 1); a reset cuts off
+ * whatever came before it, NaN and infinities too.  state (nullable, zeros):
+ * fp32 [batch, channels] before the first step.  outputs: contiguous, `dtype`;
+ * final_state: fp32 [batch, channels], the state after the last step (`state`
+ * itself when steps == 0).  The state between steps is fp32.
+ * saved (nullable): fp32 states along the way for the backward pass,
+ * puff_policy_sm100_recurrence_saved_floats of them.
+ *
+ * _backward: gradients of gates, inputs (contiguous, `dtype`) and state (nullable)
+ * from those of outputs (nullable: zeros) and final_state (nullable: zeros).  The
+ * states between the saved ones are computed again, in fp32.
+ *
+ * _step: one step of every row ([batch, channels], a row stride for gates and
+ * inputs; resets [batch]) from state to new_state, which may be state itself.
+ */
+long long puff_policy_sm100_recurrence_saved_floats(long long batch, long long steps, long long channels);
+int puff_policy_sm100_recurrence(const void* gates, const void* inputs, int dtype, const void* resets,
+                                 int reset_bytes, const float* state, long long batch, long long steps,
+                                 long long channels, long long gates_batch_stride,
+                                 long long gates_step_stride, long long inputs_batch_stride,
+                                 long long inputs_step_stride, void* outputs, float* final_state,
+                                 float* saved, void* cuda_stream);
+int puff_policy_sm100_recurrence_backward(const void* gates, const void* inputs, int dtype,
+                                          const void* resets, int reset_bytes, const float* saved,
+                                          long long batch, long long steps, long long channels,
+                                          long long gates_batch_stride, long long gates_step_stride,
+                                          long long inputs_batch_stride, long long inputs_step_stride,
+                                          const void* doutputs, const float* dfinal, void* dgates,
+                                          void* dinputs, float* dstate, void* cuda_stream);
+int puff_policy_sm100_recurrence_step(const void* gates, const void* inputs, int dtype,
+                                      const void* resets, int reset_bytes, const float* state,
+                                      long long batch, long long channels, long long gates_stride,
+                                      long long inputs_stride, void* outputs, float* new_state,
+                                      void* cuda_stream);
 
 /* ---- introspection ------------------------------------------------------- */
 /* Human-readable text for a return code of any entry point above. */

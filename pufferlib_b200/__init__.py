@@ -19,3 +19,10 @@ from .advantage import (  # noqa: F401
     rollout_write,
     set_variant,
 )
+from .policy import (  # noqa: F401
+    action_logprobs,
+    bad_action,
+    gated_recurrence,
+    gated_recurrence_step,
+    policy_loss,
+)

@@ -28,9 +28,12 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CABI_LIB = os.path.join(HERE, "libpuff_advantage_sm100.so")
 TORCH_EXT = os.path.join(HERE, "_C.so")
+OBJ_DIR = os.path.join(HERE, "build")   # object files, kept between builds
 
 CU_SOURCES = ["puff_advantage_sm100.cu", "puff_priorities_sm100.cu", "puff_minibatch_sm100.cu",
-              "puff_rollout_sm100.cu", "puff_host_pipeline.cu"]
+              "puff_rollout_sm100.cu", "puff_host_pipeline.cu", "puff_logprobs_sm100.cu",
+              "puff_policy_loss_sm100.cu", "puff_recurrence_sm100.cu"]
+TORCH_SOURCES = ["torch_binding.cpp", "torch_policy_binding.cpp"]
 
 # --fmad=true leaves nvcc free to contract a*b+c into an FMA.  One such contraction in the
 # recurrence changes the last bit of about half of the outputs, so every kernel that must be
@@ -82,36 +85,59 @@ def build_debug_cabi(out_path, verbose=False):
     return out_path
 
 
+def _objects(sources, deps_of_all, command, force, verbose):
+    """Compile each source to build/<name>.o unless the object is newer than the
+    source and every file of `deps_of_all`; stale ones are compiled side by side."""
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    objects, running = [], []
+    for name in sources:
+        src, obj = os.path.join(CSRC, name), os.path.join(OBJ_DIR, name + ".o")
+        objects.append(obj)
+        if force or _stale(obj, [src] + deps_of_all):
+            cmd = command + ["-c", "-o", obj, src]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            running.append((cmd, obj, subprocess.Popen(cmd)))
+    failed = [(cmd, obj) for cmd, obj, proc in running if proc.wait() != 0]
+    for _, obj in failed:
+        if os.path.exists(obj):
+            os.remove(obj)
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0][0])
+    return objects
+
+
 def build_cabi(force=False, verbose=False, ptxas_info=False):
-    sources = [os.path.join(CSRC, s) for s in CU_SOURCES]
     headers = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cuh")]
-    deps = sources + headers + [os.path.join(INCLUDE, "puff_advantage.h")]
-    if force or _stale(CABI_LIB, deps):
-        flags = list(NVCC_FLAGS)
+    headers.append(os.path.join(INCLUDE, "puff_advantage.h"))
+    sources = [os.path.join(CSRC, s) for s in CU_SOURCES]
+    if force or _stale(CABI_LIB, sources + headers):
+        flags = [f for f in NVCC_FLAGS if f != "-shared"]
         if ptxas_info:
             flags += ["-Xptxas", "-v"]
-        _run([NVCC] + flags + ["-o", CABI_LIB] + sources, verbose)
+        objects = _objects(CU_SOURCES, headers, [NVCC] + flags, force, verbose)
+        _run([NVCC] + NVCC_FLAGS + ["-o", CABI_LIB] + objects, verbose)
     return CABI_LIB
 
 
 def build_torch_ext(force=False, verbose=False):
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
-    src = os.path.join(CSRC, "torch_binding.cpp")
-    deps = [src, os.path.join(INCLUDE, "puff_advantage.h"), CABI_LIB]
+    header = os.path.join(INCLUDE, "puff_advantage.h")
+    deps = [os.path.join(CSRC, s) for s in TORCH_SOURCES] + [header, CABI_LIB]
     if force or _stale(TORCH_EXT, deps):
         cxx = _host_cxx()
         inc = [f"-I{p}" for p in include_paths()]
         inc += [f"-I{os.path.join(CUDA_HOME, 'include')}", f"-I{sysconfig.get_paths()['include']}"]
         libdir = library_paths()[0]
-        cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-               "-DTORCH_EXTENSION_NAME=_C"] + inc + [
-               "-o", TORCH_EXT, src,
-               f"-L{HERE}", "-lpuff_advantage_sm100", "-Wl,-rpath,$ORIGIN",
-               f"-L{libdir}", f"-Wl,-rpath,{libdir}",
-               "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"]
-        _run(cmd, verbose)
+        flags = [cxx, "-O2", "-std=c++17", "-fPIC",
+                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                 "-DTORCH_EXTENSION_NAME=_C"] + inc
+        objects = _objects(TORCH_SOURCES, [header], flags, force, verbose)
+        _run([cxx, "-shared", "-o", TORCH_EXT] + objects + [
+              f"-L{HERE}", "-lpuff_advantage_sm100", "-Wl,-rpath,$ORIGIN",
+              f"-L{libdir}", f"-Wl,-rpath,{libdir}",
+              "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"], verbose)
     return TORCH_EXT
 
 

@@ -18,6 +18,9 @@ LIB_PATH = os.environ.get("PUFF_ADV_LIB") or os.path.join(_HERE, "libpuff_advant
 OK = 0
 ERR_NULL, ERR_SHAPE, ERR_VARIANT, ERR_ALIGN, ERR_ALIAS = -1, -2, -3, -4, -5
 ERR_ARCH, ERR_DRIVER, ERR_DEVICE_WAIT, ERR_WORKSPACE, ERR_SIZE, ERR_DEVICE_BOUNDS = -6, -7, -8, -9, -10, -11
+ERR_DTYPE, ERR_VALUE = -12, -13
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+MEAN_TOKENS, MEAN_SEQUENCES = 0, 1
 NOALLOC_MAX_SEGMENTS = 524288
 EXCHANGE_HANDLE_BYTES = 64
 FLAG_ZERO_LAST_COLUMN = 1
@@ -30,6 +33,7 @@ KERNEL_NAMES = {KERNEL_NONE: "none", KERNEL_TMA2D: "tma2d", KERNEL_BULK1D: "bulk
 # every symbol the header declares, with its ctypes signature
 _P = ctypes.c_void_p
 _F = ctypes.c_float
+_D = ctypes.c_double
 _LL = ctypes.c_longlong
 _I = ctypes.c_int
 SIGNATURES = {
@@ -55,6 +59,17 @@ SIGNATURES = {
     "puff_minibatch_sm100_bad_index": (_I, []),
     "puff_rollout_sm100_write": (_I, [_P] * 6 + [_LL] * 5 + [_F, _P]),
     "puff_priorities_sm100_weights_noalloc": (_I, [_P, _P, _P, _F, _LL, _P]),
+    "puff_policy_sm100_logprobs": (_I, [_P, _I, _P] + [_LL] * 7 + [_F] + [_P] * 4),
+    "puff_policy_sm100_logprobs_backward": (_I, [_P, _I, _P] + [_LL] * 7 + [_F] + [_P] * 6),
+    "puff_policy_sm100_bad_action": (_I, []),
+    "puff_policy_sm100_loss_scratch_bytes": (ctypes.c_size_t, [_LL, _LL]),
+    "puff_policy_sm100_loss": (_I, [_P] * 3 + [_I] + [_P] * 3 + [_D, _D, _F, _F, _I, _D, _LL, _LL] + [_P] * 7
+                               + [ctypes.c_size_t, _P]),
+    "puff_policy_sm100_loss_backward": (_I, [_P] * 5 + [_F, _LL, _LL] + [_P] * 3),
+    "puff_policy_sm100_recurrence_saved_floats": (_LL, [_LL] * 3),
+    "puff_policy_sm100_recurrence": (_I, [_P, _P, _I, _P, _I, _P] + [_LL] * 7 + [_P] * 4),
+    "puff_policy_sm100_recurrence_backward": (_I, [_P, _P, _I, _P, _I, _P] + [_LL] * 7 + [_P] * 6),
+    "puff_policy_sm100_recurrence_step": (_I, [_P, _P, _I, _P, _I, _P] + [_LL] * 4 + [_P] * 3),
     "puff_advantage_sm100_strerror": (ctypes.c_char_p, [_I]),
     "puff_advantage_sm100_last_kernel": (_I, []),
     "puff_advantage_sm100_launch_count": (_LL, []),

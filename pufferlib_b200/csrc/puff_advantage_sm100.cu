@@ -612,6 +612,8 @@ extern "C" const char* puff_advantage_sm100_strerror(int code)
         case PUFF_ERR_WORKSPACE: return "scratch or workspace missing, misaligned or too small";
         case PUFF_ERR_SIZE: return "size beyond what this entry point supports";
         case PUFF_ERR_DEVICE_BOUNDS: return "a kernel formed an out-of-range index (debug build)";
+        case PUFF_ERR_DTYPE: return "unknown element type";
+        case PUFF_ERR_VALUE: return "a scalar argument is outside its range";
         default: break;
     }
     if (code > 0) return cudaGetErrorString(static_cast<cudaError_t>(code));
@@ -628,6 +630,13 @@ extern "C" long long puff_advantage_sm100_launch_count(void)
 namespace puff {
 void count_launch() { g_launch_count.fetch_add(1, std::memory_order_relaxed); }
 int tune_value(int knob, int fallback) { return tune(knob, fallback); }
+int require_sm100(int* sm_count)
+{
+    int code = PUFF_OK;
+    const DeviceInfo* dev = device_info(&code);
+    if (dev != nullptr) *sm_count = dev->sm_count;
+    return code;
+}
 }
 
 namespace puff {

@@ -1,0 +1,640 @@
+// PyTorch operators of the policy update, with their gradients.
+//
+// Adds to the `pufferlib` operator library of torch_binding.cpp what follows the advantages in the trainer: the
+// log-probability and entropy of chosen actions (sample_logits of pufferlib/pytorch.py), the clipped policy loss
+// (pufferl.py:390-411, 422) and the gated linear recurrence along the horizon.  No arithmetic here: tensors are
+// checked, buffers allocated, and the C ABI of include/puff_advantage.h is called on the current stream of the
+// tensors' device.
+//
+// Each differentiable operator has an autograd kernel whose node keeps what the backward operator needs and calls it.
+// The *_forward and *_backward operators can be called without autograd (for a program that captures a whole update
+// into a CUDA graph); their results are not differentiable, and a second derivative raises.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/all.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <optional>
+#include <string>
+#include <tuple>
+
+#include "../../include/puff_advantage.h"
+
+namespace pufferlib_b200 {
+namespace {
+
+using torch::Tensor;
+using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void check_rc(int rc, const char* what)
+{
+    TORCH_CHECK(rc == PUFF_OK, what, ": ", puff_advantage_sm100_strerror(rc), " (code ", rc, ")");
+}
+
+int dtype_code(const Tensor& t, const char* name)
+{
+    switch (t.scalar_type()) {
+        case torch::kFloat32: return PUFF_DTYPE_F32;
+        case torch::kFloat16: return PUFF_DTYPE_F16;
+        case torch::kBFloat16: return PUFF_DTYPE_BF16;
+        default: TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+    }
+}
+
+void check_f32(const Tensor& t, const Tensor& like, at::IntArrayRef sizes, const char* name)
+{
+    TORCH_CHECK(t.device() == like.device(), "All tensors must be on same device");
+    TORCH_CHECK(t.scalar_type() == torch::kFloat32, name, " must be float32");
+    TORCH_CHECK(t.sizes() == sizes, name, " must have shape ", sizes, ", got ", t.sizes());
+    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+template <typename T> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+template <typename T> const T* ptr(const OptTensor& t) { return t.has_value() && t->defined() ? static_cast<const T*>(t->data_ptr()) : nullptr; }
+bool present(const OptTensor& t) { return t.has_value() && t->defined(); }
+OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+cudaStream_t current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+// ---- log-probabilities ------------------------------------------------------------------------------------------
+
+// The leading sizes of a tensor as rows [outer, inner] with one stride each
+struct Rows {
+    int64_t outer = 1, inner = 1, outer_stride = 0, inner_stride = 0;
+};
+Rows rows_of(const Tensor& t, int64_t lead, const char* name)
+{
+    Rows r;
+    bool second = false;
+    // from the innermost leading dimension outwards: one that continues the run so far is folded into it
+    for (int64_t d = lead - 1; d >= 0; --d) {
+        const int64_t n = t.size(d), s = t.stride(d);
+        if (n == 1) continue;
+        if (!second && (r.inner == 1 || s == r.inner * r.inner_stride)) {
+            if (r.inner == 1) r.inner_stride = s;
+            r.inner *= n;
+        } else if (r.outer == 1 || s == r.outer * r.outer_stride) {
+            if (r.outer == 1) r.outer_stride = s;
+            r.outer *= n;
+            second = true;
+        } else {
+            TORCH_CHECK(false, name, " has more than two runs of rows that a stride separates; make it contiguous");
+        }
+    }
+    return r;
+}
+// logits and actions must be cut into [outer, inner] alike
+void rows_alike(Rows& a, Rows& b, const char* what)
+{
+    if (a.inner == b.inner) return;
+    Rows& coarse = a.inner > b.inner ? a : b;
+    const Rows& fine = a.inner > b.inner ? b : a;
+    TORCH_CHECK(coarse.outer == 1 && fine.inner > 0 && coarse.inner % fine.inner == 0, what,
+                " must be cut into rows alike; make one of them contiguous");
+    coarse.outer = coarse.inner / fine.inner;
+    coarse.outer_stride = coarse.inner_stride * fine.inner;
+    coarse.inner = fine.inner;
+}
+
+struct LogprobArgs {
+    int dtype;
+    int64_t vocab, rows;
+    Rows l, a;
+};
+LogprobArgs logprob_args(const Tensor& logits, const Tensor& actions)
+{
+    LogprobArgs g;
+    g.dtype = dtype_code(logits, "logits");
+    TORCH_CHECK(logits.dim() >= 1, "logits must have at least one dimension");
+    TORCH_CHECK(actions.scalar_type() == torch::kInt64, "actions must be int64");
+    TORCH_CHECK(actions.device() == logits.device(), "All tensors must be on same device");
+    const int64_t lead = logits.dim() - 1;
+    TORCH_CHECK(actions.sizes() == logits.sizes().slice(0, lead), "actions must have the shape of logits without its last dimension");
+    g.vocab = logits.size(-1);
+    g.rows = actions.numel();
+    TORCH_CHECK(g.vocab > 0 || g.rows == 0, "logits must have at least one entry per row");
+    TORCH_CHECK(g.vocab <= 1 || logits.stride(-1) == 1, "the last dimension of logits must be contiguous");
+    if (g.rows > 0) {
+        g.l = rows_of(logits, lead, "logits");
+        g.a = rows_of(actions, lead, "actions");
+        rows_alike(g.l, g.a, "logits and actions");
+    }
+    return g;
+}
+
+// (logprobs, entropy or an empty tensor, row_stats or an empty tensor)
+std::tuple<Tensor, Tensor, Tensor> logprobs_forward_meta(const Tensor& logits, const Tensor& actions, double temperature,
+                                                         bool want_entropy, bool save)
+{
+    logprob_args(logits, actions);
+    TORCH_CHECK(temperature > 0, "temperature must be positive");
+    const auto opts = logits.options().dtype(torch::kFloat32);
+    Tensor logprobs = torch::empty(actions.sizes(), opts);
+    Tensor entropy = torch::empty(want_entropy ? actions.sizes() : at::IntArrayRef({0}), opts);
+    Tensor stats = torch::empty({save ? actions.numel() : 0, 2}, opts);
+    return {logprobs, entropy, stats};
+}
+std::tuple<Tensor, Tensor, Tensor> logprobs_forward_cuda(const Tensor& logits, const Tensor& actions, double temperature,
+                                                         bool want_entropy, bool save)
+{
+    const LogprobArgs g = logprob_args(logits, actions);
+    const c10::cuda::CUDAGuard guard(logits.device());
+    auto out = logprobs_forward_meta(logits, actions, temperature, want_entropy, save);
+    if (g.rows == 0) return out;
+    check_rc(puff_policy_sm100_logprobs(logits.data_ptr(), g.dtype, ptr<const long long>(actions), g.l.outer, g.l.inner,
+                                        g.vocab, g.l.outer_stride, g.l.inner_stride, g.a.outer_stride, g.a.inner_stride,
+                                        static_cast<float>(temperature), ptr<float>(std::get<0>(out)),
+                                        want_entropy ? ptr<float>(std::get<1>(out)) : nullptr,
+                                        save ? ptr<float>(std::get<2>(out)) : nullptr, current_stream()),
+             "puff_action_logprobs");
+    return out;
+}
+std::tuple<Tensor, Tensor, Tensor> logprobs_forward(const Tensor& logits, const Tensor& actions, double temperature,
+                                                    bool want_entropy, bool save)
+{
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_action_logprobs_forward", "")
+                         .typed<decltype(logprobs_forward_meta)>();
+    return op.call(logits, actions, temperature, want_entropy, save);
+}
+std::tuple<Tensor, Tensor> action_logprobs(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
+{
+    auto out = logprobs_forward(logits, actions, temperature, want_entropy, false);
+    return {std::get<0>(out), std::get<1>(out)};
+}
+
+Tensor logprobs_backward_meta(const Tensor& logits, const Tensor& actions, double, const Tensor&, const OptTensor&,
+                              const Tensor&, const OptTensor&)
+{
+    logprob_args(logits, actions);
+    return torch::empty(logits.sizes(), logits.options());
+}
+Tensor logprobs_backward_cuda(const Tensor& logits, const Tensor& actions, double temperature, const Tensor& row_stats,
+                              const OptTensor& entropy, const Tensor& dlogprobs, const OptTensor& dentropy)
+{
+    const LogprobArgs g = logprob_args(logits, actions);
+    check_f32(row_stats, logits, {g.rows, 2}, "row_stats");
+    check_f32(dlogprobs, logits, actions.sizes(), "dlogprobs");
+    if (present(dentropy)) {
+        TORCH_CHECK(present(entropy), "dentropy needs the entropy of the forward pass");
+        check_f32(*dentropy, logits, actions.sizes(), "dentropy");
+        check_f32(*entropy, logits, actions.sizes(), "entropy");
+    }
+    const c10::cuda::CUDAGuard guard(logits.device());
+    Tensor dlogits = torch::empty(logits.sizes(), logits.options());
+    if (g.rows == 0) return dlogits;
+    check_rc(puff_policy_sm100_logprobs_backward(
+                 logits.data_ptr(), g.dtype, ptr<const long long>(actions), g.l.outer, g.l.inner, g.vocab,
+                 g.l.outer_stride, g.l.inner_stride, g.a.outer_stride, g.a.inner_stride, static_cast<float>(temperature),
+                 ptr<const float>(row_stats), present(dentropy) ? ptr<float>(entropy) : nullptr,
+                 ptr<const float>(dlogprobs), ptr<float>(dentropy), dlogits.data_ptr(), current_stream()),
+             "puff_action_logprobs_backward");
+    return dlogits;
+}
+Tensor logprobs_backward(const Tensor& logits, const Tensor& actions, double temperature, const Tensor& row_stats,
+                         const OptTensor& entropy, const Tensor& dlogprobs, const OptTensor& dentropy)
+{
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_action_logprobs_backward", "")
+                         .typed<decltype(logprobs_backward_meta)>();
+    return op.call(logits, actions, temperature, row_stats, entropy, dlogprobs, dentropy);
+}
+
+struct LogprobsNode : public torch::autograd::Function<LogprobsNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& actions, double temperature,
+                                 bool want_entropy)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [logprobs, entropy, stats] = logprobs_forward(logits, actions, temperature, want_entropy, true);
+        ctx->set_materialize_grads(false);
+        if (!want_entropy) ctx->mark_non_differentiable({entropy});
+        ctx->save_for_backward({logits, actions, stats, entropy});
+        ctx->saved_data["temperature"] = temperature;
+        return {logprobs, entropy};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto saved = ctx->get_saved_variables();
+        Tensor dlogits;
+        if (grads[0].defined() || grads[1].defined()) {
+            const Tensor dlp = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(grads[1], at::MemoryFormat::Contiguous);
+            const OptTensor dh = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
+            dlogits = logprobs_backward(saved[0], saved[1], ctx->saved_data["temperature"].toDouble(), saved[2], saved[3], dlp, dh);
+        }
+        return {dlogits, Tensor(), Tensor(), Tensor()};
+    }
+};
+std::tuple<Tensor, Tensor> action_logprobs_autograd(const Tensor& logits, const Tensor& actions, double temperature,
+                                                    bool want_entropy)
+{
+    if (!(at::GradMode::is_enabled() && logits.requires_grad())) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return action_logprobs(logits, actions, temperature, want_entropy);
+    }
+    auto out = LogprobsNode::apply(logits, actions, temperature, want_entropy);
+    return {out[0], out[1]};
+}
+
+// ---- policy loss -------------------------------------------------------------------------------------------------
+
+int reduction_code(c10::string_view reduction)
+{
+    TORCH_CHECK(reduction == "token" || reduction == "sequence", "reduction must be \"token\" or \"sequence\"");
+    return reduction == "token" ? PUFF_MEAN_TOKENS : PUFF_MEAN_SEQUENCES;
+}
+// one advantage per row?
+bool loss_args(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, const OptTensor& ref_logprobs,
+               const OptTensor& entropy, const OptTensor& mask, double clip_low, double clip_high, double denominator)
+{
+    TORCH_CHECK(logprobs.dim() == 2, "logprobs must be 2D [rows, steps]");
+    check_f32(logprobs, logprobs, logprobs.sizes(), "logprobs");
+    check_f32(old_logprobs, logprobs, logprobs.sizes(), "old_logprobs");
+    const int64_t rows = logprobs.size(0), steps = logprobs.size(1);
+    const bool per_row = advantages.dim() == 1 || (advantages.dim() == 2 && advantages.size(1) == 1 && steps != 1);
+    if (per_row && advantages.dim() == 2) check_f32(advantages, logprobs, {rows, 1}, "advantages");
+    else if (per_row) check_f32(advantages, logprobs, {rows}, "advantages");
+    else check_f32(advantages, logprobs, logprobs.sizes(), "advantages");
+    if (present(ref_logprobs)) check_f32(*ref_logprobs, logprobs, logprobs.sizes(), "ref_logprobs");
+    if (present(entropy)) check_f32(*entropy, logprobs, logprobs.sizes(), "entropy");
+    if (present(mask)) {
+        TORCH_CHECK(mask->device() == logprobs.device(), "All tensors must be on same device");
+        TORCH_CHECK(mask->scalar_type() == torch::kBool, "mask must be bool");
+        TORCH_CHECK(mask->sizes() == logprobs.sizes(), "mask must have the shape of logprobs");
+        TORCH_CHECK(mask->is_contiguous(), "mask must be contiguous");
+    }
+    TORCH_CHECK(clip_low >= 0 && clip_high >= 0, "clip_low and clip_high must not be negative");
+    TORCH_CHECK(denominator >= 0, "denominator must be positive");
+    return per_row;
+}
+
+using LossOut = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+// (loss, ratio, stats, slope, row_scale, weight); the last three hold nothing unless `save`
+LossOut loss_forward_meta(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
+                          double clip_high, const OptTensor& ref_logprobs, double, const OptTensor& entropy, double,
+                          const OptTensor& mask, c10::string_view reduction, double denominator, bool save)
+{
+    loss_args(logprobs, old_logprobs, advantages, ref_logprobs, entropy, mask, clip_low, clip_high, denominator);
+    const bool sequence = reduction_code(reduction) == PUFF_MEAN_SEQUENCES;
+    const auto opts = logprobs.options();
+    return {torch::empty({}, opts), torch::empty(logprobs.sizes(), opts), torch::empty({6}, opts),
+            torch::empty(save ? logprobs.sizes() : at::IntArrayRef({0}), opts),
+            torch::empty({save && sequence ? logprobs.size(0) : 0}, opts), torch::empty({save ? 1 : 0}, opts)};
+}
+LossOut loss_forward_cuda(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
+                          double clip_high, const OptTensor& ref_logprobs, double kl_coef, const OptTensor& entropy,
+                          double ent_coef, const OptTensor& mask, c10::string_view reduction, double denominator, bool save)
+{
+    const bool per_row = loss_args(logprobs, old_logprobs, advantages, ref_logprobs, entropy, mask, clip_low, clip_high, denominator);
+    const c10::cuda::CUDAGuard guard(logprobs.device());
+    LossOut out = loss_forward_meta(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
+                                    ent_coef, mask, reduction, denominator, save);
+    auto& [loss, ratio, stats, slope, row_scale, weight] = out;
+    const int64_t rows = logprobs.size(0), steps = logprobs.size(1);
+    const bool sequence = reduction_code(reduction) == PUFF_MEAN_SEQUENCES;
+    const size_t sbytes = puff_policy_sm100_loss_scratch_bytes(rows, steps);
+    Tensor scratch = torch::empty({static_cast<int64_t>((sbytes + 7) / 8)}, logprobs.options().dtype(torch::kFloat64));
+    check_rc(puff_policy_sm100_loss(ptr<const float>(logprobs), ptr<const float>(old_logprobs), ptr<const float>(advantages),
+                                    per_row, ptr<float>(ref_logprobs), ptr<float>(entropy), ptr<unsigned char>(mask),
+                                    clip_low, clip_high, static_cast<float>(kl_coef), static_cast<float>(ent_coef),
+                                    sequence ? PUFF_MEAN_SEQUENCES : PUFF_MEAN_TOKENS, denominator, rows, steps,
+                                    ptr<float>(loss), ptr<float>(ratio), ptr<float>(stats),
+                                    save ? ptr<float>(slope) : nullptr, save && sequence ? ptr<float>(row_scale) : nullptr,
+                                    save ? ptr<float>(weight) : nullptr, scratch.data_ptr(), sbytes, current_stream()),
+             "puff_policy_loss");
+    return out;
+}
+LossOut loss_forward(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
+                     double clip_high, const OptTensor& ref_logprobs, double kl_coef, const OptTensor& entropy,
+                     double ent_coef, const OptTensor& mask, c10::string_view reduction, double denominator, bool save)
+{
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_policy_loss_forward", "")
+                         .typed<decltype(loss_forward_meta)>();
+    return op.call(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy, ent_coef, mask,
+                   reduction, denominator, save);
+}
+std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages,
+                                               double clip_low, double clip_high, const OptTensor& ref_logprobs,
+                                               double kl_coef, const OptTensor& entropy, double ent_coef,
+                                               const OptTensor& mask, c10::string_view reduction, double denominator)
+{
+    LossOut out = loss_forward(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
+                               ent_coef, mask, reduction, denominator, false);
+    return {std::get<0>(out), std::get<1>(out), std::get<2>(out)};
+}
+
+// (dlogprobs, dentropy or an empty tensor)
+std::tuple<Tensor, Tensor> loss_backward_meta(const Tensor& slope, const Tensor&, const Tensor&, const Tensor&,
+                                              const OptTensor&, double, bool want_dentropy)
+{
+    return {torch::empty_like(slope), torch::empty(want_dentropy ? slope.sizes() : at::IntArrayRef({0}), slope.options())};
+}
+std::tuple<Tensor, Tensor> loss_backward_cuda(const Tensor& slope, const Tensor& row_scale, const Tensor& weight,
+                                              const Tensor& dloss, const OptTensor& mask, double ent_coef,
+                                              bool want_dentropy)
+{
+    TORCH_CHECK(slope.dim() == 2, "slope must be 2D [rows, steps]");
+    check_f32(slope, slope, slope.sizes(), "slope");
+    check_f32(weight, slope, {1}, "weight");
+    check_f32(dloss, slope, {}, "dloss");
+    TORCH_CHECK(row_scale.numel() == 0 || row_scale.numel() == slope.size(0), "row_scale must be [rows] or empty");
+    check_f32(row_scale, slope, row_scale.sizes(), "row_scale");
+    if (present(mask))
+        TORCH_CHECK(mask->scalar_type() == torch::kBool && mask->sizes() == slope.sizes() && mask->is_contiguous() &&
+                        mask->device() == slope.device(),
+                    "mask must be a contiguous bool tensor of the shape of slope on the same device");
+    const c10::cuda::CUDAGuard guard(slope.device());
+    auto out = loss_backward_meta(slope, row_scale, weight, dloss, mask, ent_coef, want_dentropy);
+    check_rc(puff_policy_sm100_loss_backward(ptr<const float>(slope), row_scale.numel() > 0 ? ptr<const float>(row_scale) : nullptr,
+                                             ptr<const float>(weight), ptr<const float>(dloss), ptr<unsigned char>(mask),
+                                             static_cast<float>(ent_coef), slope.size(0), slope.size(1),
+                                             ptr<float>(std::get<0>(out)),
+                                             want_dentropy ? ptr<float>(std::get<1>(out)) : nullptr, current_stream()),
+             "puff_policy_loss_backward");
+    return out;
+}
+std::tuple<Tensor, Tensor> loss_backward(const Tensor& slope, const Tensor& row_scale, const Tensor& weight,
+                                         const Tensor& dloss, const OptTensor& mask, double ent_coef, bool want_dentropy)
+{
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_policy_loss_backward", "")
+                         .typed<decltype(loss_backward_meta)>();
+    return op.call(slope, row_scale, weight, dloss, mask, ent_coef, want_dentropy);
+}
+
+struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logprobs, const Tensor& old_logprobs,
+                                 const Tensor& advantages, double clip_low, double clip_high,
+                                 const OptTensor& ref_logprobs, double kl_coef, const OptTensor& entropy, double ent_coef,
+                                 const OptTensor& mask, const std::string& reduction, double denominator)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [loss, ratio, stats, slope, row_scale, weight] =
+            loss_forward(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy, ent_coef,
+                         mask, reduction, denominator, true);
+        ctx->mark_non_differentiable({ratio, stats});
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({slope, row_scale, weight, mask.value_or(Tensor())});
+        ctx->saved_data["ent_coef"] = ent_coef;
+        ctx->saved_data["dentropy"] = present(entropy) && entropy->requires_grad();
+        return {loss, ratio, stats};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        variable_list out(12);
+        if (!grads[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const bool want_dentropy = ctx->saved_data["dentropy"].toBool();
+        auto [dlp, dent] = loss_backward(saved[0], saved[1], saved[2], grads[0], optional(saved[3]),
+                                         ctx->saved_data["ent_coef"].toDouble(), want_dentropy);
+        out[0] = dlp;
+        if (want_dentropy) out[7] = dent;
+        return out;
+    }
+};
+bool wants_grad(const OptTensor& t) { return present(t) && t->requires_grad(); }
+std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor& logprobs, const Tensor& old_logprobs,
+                                                        const Tensor& advantages, double clip_low, double clip_high,
+                                                        const OptTensor& ref_logprobs, double kl_coef,
+                                                        const OptTensor& entropy, double ent_coef, const OptTensor& mask,
+                                                        c10::string_view reduction, double denominator)
+{
+    if (at::GradMode::is_enabled())
+        TORCH_CHECK(!old_logprobs.requires_grad() && !advantages.requires_grad() && !wants_grad(ref_logprobs),
+                    "old_logprobs, advantages and ref_logprobs are constants of the loss; detach them");
+    if (!(at::GradMode::is_enabled() && (logprobs.requires_grad() || wants_grad(entropy)))) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return policy_loss(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
+                           ent_coef, mask, reduction, denominator);
+    }
+    auto out = PolicyLossNode::apply(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
+                                     ent_coef, mask, std::string(reduction), denominator);
+    return {out[0], out[1], out[2]};
+}
+
+// ---- gated recurrence --------------------------------------------------------------------------------------------
+
+int check_resets(const OptTensor& resets, const Tensor& like, at::IntArrayRef sizes)
+{
+    if (!present(resets)) return 0;
+    const auto t = resets->scalar_type();
+    TORCH_CHECK(resets->device() == like.device(), "All tensors must be on same device");
+    TORCH_CHECK(t == torch::kFloat32 || t == torch::kBool || t == torch::kUInt8, "resets must be float32 or bool");
+    TORCH_CHECK(resets->sizes() == sizes, "resets must have shape ", sizes, ", got ", resets->sizes());
+    TORCH_CHECK(resets->is_contiguous(), "resets must be contiguous");
+    return t == torch::kFloat32 ? 4 : 1;
+}
+void recurrence_args(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, int64_t dims)
+{
+    dtype_code(gates, "gates");
+    TORCH_CHECK(gates.dim() == dims, "gates must be ", dims == 3 ? "3D [batch, steps, channels]" : "2D [batch, channels]");
+    TORCH_CHECK(inputs.sizes() == gates.sizes() && inputs.scalar_type() == gates.scalar_type(),
+                "gates and inputs must have one shape and one type");
+    TORCH_CHECK(inputs.device() == gates.device(), "All tensors must be on same device");
+    if (gates.numel() > 0 && gates.size(-1) > 1)
+        TORCH_CHECK(gates.stride(-1) == 1 && inputs.stride(-1) == 1, "the last dimension of gates and inputs must be contiguous");
+    check_resets(resets, gates, gates.sizes().slice(0, dims - 1));
+}
+
+using RecOut = std::tuple<Tensor, Tensor, Tensor>;
+// (outputs, final state, saved states or an empty tensor)
+RecOut recurrence_forward_meta(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const OptTensor& state,
+                               bool save)
+{
+    recurrence_args(gates, inputs, resets, 3);
+    const int64_t B = gates.size(0), T = gates.size(1), C = gates.size(2);
+    if (present(state)) check_f32(*state, gates, {B, C}, "state");
+    const auto f32 = gates.options().dtype(torch::kFloat32);
+    return {torch::empty({B, T, C}, gates.options()), torch::empty({B, C}, f32),
+            torch::empty({save ? puff_policy_sm100_recurrence_saved_floats(B, T, C) : 0}, f32)};
+}
+RecOut recurrence_forward_cuda(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const OptTensor& state,
+                               bool save)
+{
+    const c10::cuda::CUDAGuard guard(gates.device());
+    RecOut out = recurrence_forward_meta(gates, inputs, resets, state, save);
+    auto& [outputs, final_state, saved] = out;
+    check_rc(puff_policy_sm100_recurrence(gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets),
+                                          check_resets(resets, gates, gates.sizes().slice(0, 2)), ptr<float>(state),
+                                          gates.size(0), gates.size(1), gates.size(2), gates.stride(0), gates.stride(1),
+                                          inputs.stride(0), inputs.stride(1), outputs.data_ptr(), ptr<float>(final_state),
+                                          save && saved.numel() > 0 ? ptr<float>(saved) : nullptr, current_stream()),
+             "puff_gated_recurrence");
+    return out;
+}
+RecOut recurrence_forward(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const OptTensor& state, bool save)
+{
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_gated_recurrence_forward", "")
+                         .typed<decltype(recurrence_forward_meta)>();
+    return op.call(gates, inputs, resets, state, save);
+}
+std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const OptTensor& state)
+{
+    RecOut out = recurrence_forward(gates, inputs, resets, state, false);
+    return {std::get<0>(out), std::get<1>(out)};
+}
+
+// (dgates, dinputs, dstate)
+RecOut recurrence_backward_meta(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const Tensor&,
+                                const OptTensor&, const OptTensor&)
+{
+    recurrence_args(gates, inputs, resets, 3);
+    return {torch::empty(gates.sizes(), gates.options()), torch::empty(gates.sizes(), gates.options()),
+            torch::empty({gates.size(0), gates.size(2)}, gates.options().dtype(torch::kFloat32))};
+}
+RecOut recurrence_backward_cuda(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const Tensor& saved,
+                                const OptTensor& doutputs, const OptTensor& dfinal)
+{
+    const c10::cuda::CUDAGuard guard(gates.device());
+    RecOut out = recurrence_backward_meta(gates, inputs, resets, saved, doutputs, dfinal);
+    const int64_t B = gates.size(0), T = gates.size(1), C = gates.size(2);
+    check_f32(saved, gates, {puff_policy_sm100_recurrence_saved_floats(B, T, C)}, "saved");
+    if (present(doutputs))
+        TORCH_CHECK(doutputs->sizes() == gates.sizes() && doutputs->scalar_type() == gates.scalar_type() &&
+                        doutputs->is_contiguous() && doutputs->device() == gates.device(),
+                    "doutputs must be contiguous, of the shape and type of gates, on the same device");
+    if (present(dfinal)) check_f32(*dfinal, gates, {B, C}, "dfinal");
+    auto& [dgates, dinputs, dstate] = out;
+    check_rc(puff_policy_sm100_recurrence_backward(
+                 gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets),
+                 check_resets(resets, gates, gates.sizes().slice(0, 2)), ptr<const float>(saved), B, T, C, gates.stride(0),
+                 gates.stride(1), inputs.stride(0), inputs.stride(1), ptr<void>(doutputs), ptr<float>(dfinal),
+                 dgates.data_ptr(), dinputs.data_ptr(), ptr<float>(dstate), current_stream()),
+             "puff_gated_recurrence_backward");
+    return out;
+}
+RecOut recurrence_backward(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const Tensor& saved,
+                           const OptTensor& doutputs, const OptTensor& dfinal)
+{
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_gated_recurrence_backward", "")
+                         .typed<decltype(recurrence_backward_meta)>();
+    return op.call(gates, inputs, resets, saved, doutputs, dfinal);
+}
+
+struct RecurrenceNode : public torch::autograd::Function<RecurrenceNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& gates, const Tensor& inputs, const OptTensor& resets,
+                                 const OptTensor& state)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [outputs, final_state, saved] = recurrence_forward(gates, inputs, resets, state, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({gates, inputs, resets.value_or(Tensor()), saved});
+        ctx->saved_data["dstate"] = present(state) && state->requires_grad();
+        return {outputs, final_state};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        variable_list out(4);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const OptTensor dout = grads[0].defined() ? OptTensor(grads[0].contiguous()) : std::nullopt;
+        const OptTensor dfinal = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
+        auto [dgates, dinputs, dstate] = recurrence_backward(saved[0], saved[1], optional(saved[2]), saved[3], dout, dfinal);
+        out[0] = dgates;
+        out[1] = dinputs;
+        if (ctx->saved_data["dstate"].toBool()) out[3] = dstate;
+        return out;
+    }
+};
+std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor& gates, const Tensor& inputs, const OptTensor& resets,
+                                                     const OptTensor& state)
+{
+    if (!(at::GradMode::is_enabled() && (gates.requires_grad() || inputs.requires_grad() || wants_grad(state)))) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return gated_recurrence(gates, inputs, resets, state);
+    }
+    auto out = RecurrenceNode::apply(gates, inputs, resets, state);
+    return {out[0], out[1]};
+}
+
+void step_args(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, const Tensor& new_state)
+{
+    recurrence_args(gates, inputs, resets, 2);
+    check_f32(state, gates, gates.sizes(), "state");
+    check_f32(new_state, gates, gates.sizes(), "new_state");
+}
+Tensor recurrence_step_meta(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, Tensor new_state)
+{
+    step_args(gates, inputs, state, resets, new_state);
+    return torch::empty(gates.sizes(), gates.options());
+}
+Tensor recurrence_step_cuda(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, Tensor new_state)
+{
+    step_args(gates, inputs, state, resets, new_state);
+    const c10::cuda::CUDAGuard guard(gates.device());
+    Tensor outputs = torch::empty(gates.sizes(), gates.options());
+    check_rc(puff_policy_sm100_recurrence_step(gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets),
+                                               check_resets(resets, gates, gates.sizes().slice(0, 1)), ptr<const float>(state),
+                                               gates.size(0), gates.size(1), gates.stride(0), inputs.stride(0),
+                                               outputs.data_ptr(), ptr<float>(new_state), current_stream()),
+             "puff_gated_recurrence_step");
+    return outputs;
+}
+// the single step is for acting, not for training
+Tensor recurrence_step_autograd(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, Tensor new_state)
+{
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (gates.requires_grad() || inputs.requires_grad() || state.requires_grad() ||
+                                                 new_state.requires_grad())),
+                "the single step has no gradient; call it under torch.no_grad() or use puff_gated_recurrence");
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_gated_recurrence_step", "")
+                         .typed<decltype(recurrence_step_meta)>();
+    Tensor outputs = op.call(gates, inputs, state, resets, new_state);
+    new_state.unsafeGetTensorImpl()->bump_version();
+    return outputs;
+}
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(pufferlib, m)
+{
+    m.def("puff_action_logprobs(Tensor logits, Tensor actions, float temperature=1.0, bool entropy=True) -> (Tensor, Tensor)");
+    m.def("puff_action_logprobs_forward(Tensor logits, Tensor actions, float temperature, bool entropy, bool save) -> (Tensor, Tensor, Tensor)");
+    m.def("puff_action_logprobs_backward(Tensor logits, Tensor actions, float temperature, Tensor row_stats, Tensor? entropy, Tensor dlogprobs, Tensor? dentropy) -> Tensor");
+    m.def("puff_policy_loss(Tensor logprobs, Tensor old_logprobs, Tensor advantages, float clip_low, float clip_high, Tensor? ref_logprobs, float kl_coef, Tensor? entropy, float ent_coef, Tensor? mask, str reduction, float denominator) -> (Tensor, Tensor, Tensor)");
+    m.def("puff_policy_loss_forward(Tensor logprobs, Tensor old_logprobs, Tensor advantages, float clip_low, float clip_high, Tensor? ref_logprobs, float kl_coef, Tensor? entropy, float ent_coef, Tensor? mask, str reduction, float denominator, bool save) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("puff_policy_loss_backward(Tensor slope, Tensor row_scale, Tensor weight, Tensor dloss, Tensor? mask, float ent_coef, bool want_dentropy) -> (Tensor, Tensor)");
+    m.def("puff_gated_recurrence(Tensor gates, Tensor inputs, Tensor? resets, Tensor? state) -> (Tensor, Tensor)");
+    m.def("puff_gated_recurrence_forward(Tensor gates, Tensor inputs, Tensor? resets, Tensor? state, bool save) -> (Tensor, Tensor, Tensor)");
+    m.def("puff_gated_recurrence_backward(Tensor gates, Tensor inputs, Tensor? resets, Tensor saved, Tensor? doutputs, Tensor? dfinal) -> (Tensor, Tensor, Tensor)");
+    m.def("puff_gated_recurrence_step(Tensor gates, Tensor inputs, Tensor state, Tensor? resets, Tensor(a!) new_state) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(pufferlib, CUDA, m)
+{
+    m.impl("puff_action_logprobs", &action_logprobs);
+    m.impl("puff_action_logprobs_forward", &logprobs_forward_cuda);
+    m.impl("puff_action_logprobs_backward", &logprobs_backward_cuda);
+    m.impl("puff_policy_loss", &policy_loss);
+    m.impl("puff_policy_loss_forward", &loss_forward_cuda);
+    m.impl("puff_policy_loss_backward", &loss_backward_cuda);
+    m.impl("puff_gated_recurrence", &gated_recurrence);
+    m.impl("puff_gated_recurrence_forward", &recurrence_forward_cuda);
+    m.impl("puff_gated_recurrence_backward", &recurrence_backward_cuda);
+    m.impl("puff_gated_recurrence_step", &recurrence_step_cuda);
+}
+
+TORCH_LIBRARY_IMPL(pufferlib, Meta, m)
+{
+    m.impl("puff_action_logprobs", &action_logprobs);
+    m.impl("puff_action_logprobs_forward", &logprobs_forward_meta);
+    m.impl("puff_action_logprobs_backward", &logprobs_backward_meta);
+    m.impl("puff_policy_loss", &policy_loss);
+    m.impl("puff_policy_loss_forward", &loss_forward_meta);
+    m.impl("puff_policy_loss_backward", &loss_backward_meta);
+    m.impl("puff_gated_recurrence", &gated_recurrence);
+    m.impl("puff_gated_recurrence_forward", &recurrence_forward_meta);
+    m.impl("puff_gated_recurrence_backward", &recurrence_backward_meta);
+    m.impl("puff_gated_recurrence_step", &recurrence_step_meta);
+}
+
+TORCH_LIBRARY_IMPL(pufferlib, Autograd, m)
+{
+    m.impl("puff_action_logprobs", &action_logprobs_autograd);
+    m.impl("puff_policy_loss", &policy_loss_autograd);
+    m.impl("puff_gated_recurrence", &gated_recurrence_autograd);
+    m.impl("puff_gated_recurrence_step", &recurrence_step_autograd);
+    for (const char* name : {"puff_action_logprobs_forward", "puff_action_logprobs_backward", "puff_policy_loss_forward",
+                             "puff_policy_loss_backward", "puff_gated_recurrence_forward", "puff_gated_recurrence_backward"})
+        m.impl(name, torch::autograd::autogradNotImplementedFallback());
+}
+
+}  // namespace pufferlib_b200
