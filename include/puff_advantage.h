@@ -416,7 +416,9 @@ int puff_policy_sm100_loss_backward(const float* slope, const float* row_scale, 
  * final_state: fp32 [batch, channels], the state after the last step (`state`
  * itself when steps == 0).  The state between steps is fp32.
  * saved (nullable): fp32 states along the way for the backward pass,
- * puff_policy_sm100_recurrence_saved_floats of them.
+ * puff_policy_sm100_recurrence_saved_floats of them.  scratch: at least
+ * puff_policy_sm100_recurrence_scratch_bytes bytes (0 for most shapes: then it may
+ * be NULL), 8-byte aligned, for this call alone until the stream has passed it.
  *
  * _backward: gradients of gates, inputs (contiguous, `dtype`) and state (nullable)
  * from those of outputs (nullable: zeros) and final_state (nullable: zeros).  The
@@ -426,19 +428,21 @@ int puff_policy_sm100_loss_backward(const float* slope, const float* row_scale, 
  * inputs; resets [batch]) from state to new_state, which may be state itself.
  */
 long long puff_policy_sm100_recurrence_saved_floats(long long batch, long long steps, long long channels);
+size_t puff_policy_sm100_recurrence_scratch_bytes(long long batch, long long steps, long long channels);
 int puff_policy_sm100_recurrence(const void* gates, const void* inputs, int dtype, const void* resets,
                                  int reset_bytes, const float* state, long long batch, long long steps,
                                  long long channels, long long gates_batch_stride,
                                  long long gates_step_stride, long long inputs_batch_stride,
                                  long long inputs_step_stride, void* outputs, float* final_state,
-                                 float* saved, void* cuda_stream);
+                                 float* saved, void* scratch, size_t scratch_bytes, void* cuda_stream);
 int puff_policy_sm100_recurrence_backward(const void* gates, const void* inputs, int dtype,
                                           const void* resets, int reset_bytes, const float* saved,
                                           long long batch, long long steps, long long channels,
                                           long long gates_batch_stride, long long gates_step_stride,
                                           long long inputs_batch_stride, long long inputs_step_stride,
                                           const void* doutputs, const float* dfinal, void* dgates,
-                                          void* dinputs, float* dstate, void* cuda_stream);
+                                          void* dinputs, float* dstate, void* scratch,
+                                          size_t scratch_bytes, void* cuda_stream);
 int puff_policy_sm100_recurrence_step(const void* gates, const void* inputs, int dtype,
                                       const void* resets, int reset_bytes, const float* state,
                                       long long batch, long long channels, long long gates_stride,

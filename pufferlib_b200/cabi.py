@@ -67,8 +67,11 @@ SIGNATURES = {
                                + [ctypes.c_size_t, _P]),
     "puff_policy_sm100_loss_backward": (_I, [_P] * 5 + [_F, _LL, _LL] + [_P] * 3),
     "puff_policy_sm100_recurrence_saved_floats": (_LL, [_LL] * 3),
-    "puff_policy_sm100_recurrence": (_I, [_P, _P, _I, _P, _I, _P] + [_LL] * 7 + [_P] * 4),
-    "puff_policy_sm100_recurrence_backward": (_I, [_P, _P, _I, _P, _I, _P] + [_LL] * 7 + [_P] * 6),
+    "puff_policy_sm100_recurrence": (_I, [_P, _P, _I, _P, _I, _P] + [_LL] * 7 + [_P] * 4
+                                     + [ctypes.c_size_t, _P]),
+    "puff_policy_sm100_recurrence_backward": (_I, [_P, _P, _I, _P, _I, _P] + [_LL] * 7 + [_P] * 6
+                                              + [ctypes.c_size_t, _P]),
+    "puff_policy_sm100_recurrence_scratch_bytes": (ctypes.c_size_t, [_LL] * 3),
     "puff_policy_sm100_recurrence_step": (_I, [_P, _P, _I, _P, _I, _P] + [_LL] * 4 + [_P] * 3),
     "puff_advantage_sm100_strerror": (ctypes.c_char_p, [_I]),
     "puff_advantage_sm100_last_kernel": (_I, []),

@@ -435,6 +435,13 @@ void recurrence_args(const Tensor& gates, const Tensor& inputs, const OptTensor&
     check_resets(resets, gates, gates.sizes().slice(0, dims - 1));
 }
 
+// the workspace of one call, or an undefined tensor where it needs none
+Tensor recurrence_scratch(const Tensor& gates, size_t* bytes)
+{
+    *bytes = puff_policy_sm100_recurrence_scratch_bytes(gates.size(0), gates.size(1), gates.size(2));
+    return *bytes == 0 ? Tensor() : torch::empty({static_cast<int64_t>((*bytes + 7) / 8)}, gates.options().dtype(torch::kFloat64));
+}
+
 using RecOut = std::tuple<Tensor, Tensor, Tensor>;
 // (outputs, final state, saved states or an empty tensor)
 RecOut recurrence_forward_meta(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const OptTensor& state,
@@ -453,11 +460,14 @@ RecOut recurrence_forward_cuda(const Tensor& gates, const Tensor& inputs, const 
     const c10::cuda::CUDAGuard guard(gates.device());
     RecOut out = recurrence_forward_meta(gates, inputs, resets, state, save);
     auto& [outputs, final_state, saved] = out;
+    size_t sbytes;
+    const Tensor scratch = recurrence_scratch(gates, &sbytes);
     check_rc(puff_policy_sm100_recurrence(gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets),
                                           check_resets(resets, gates, gates.sizes().slice(0, 2)), ptr<float>(state),
                                           gates.size(0), gates.size(1), gates.size(2), gates.stride(0), gates.stride(1),
                                           inputs.stride(0), inputs.stride(1), outputs.data_ptr(), ptr<float>(final_state),
-                                          save && saved.numel() > 0 ? ptr<float>(saved) : nullptr, current_stream()),
+                                          save && saved.numel() > 0 ? ptr<float>(saved) : nullptr, ptr<void>(scratch), sbytes,
+                                          current_stream()),
              "puff_gated_recurrence");
     return out;
 }
@@ -494,11 +504,13 @@ RecOut recurrence_backward_cuda(const Tensor& gates, const Tensor& inputs, const
                     "doutputs must be contiguous, of the shape and type of gates, on the same device");
     if (present(dfinal)) check_f32(*dfinal, gates, {B, C}, "dfinal");
     auto& [dgates, dinputs, dstate] = out;
+    size_t sbytes;
+    const Tensor scratch = recurrence_scratch(gates, &sbytes);
     check_rc(puff_policy_sm100_recurrence_backward(
                  gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets),
                  check_resets(resets, gates, gates.sizes().slice(0, 2)), ptr<const float>(saved), B, T, C, gates.stride(0),
                  gates.stride(1), inputs.stride(0), inputs.stride(1), ptr<void>(doutputs), ptr<float>(dfinal),
-                 dgates.data_ptr(), dinputs.data_ptr(), ptr<float>(dstate), current_stream()),
+                 dgates.data_ptr(), dinputs.data_ptr(), ptr<float>(dstate), ptr<void>(scratch), sbytes, current_stream()),
              "puff_gated_recurrence_backward");
     return out;
 }

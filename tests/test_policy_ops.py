@@ -165,10 +165,10 @@ def test_loss_entry_point_checks():
 
 def test_recurrence_entry_point_checks():
     from pufferlib_b200 import cabi
-    lib, h = cabi.load(), Host(1 << 16)
+    lib, h = cabi.load(), Host(1 << 21)
     assert lib.puff_policy_sm100_recurrence_saved_floats(2, 3, 0) == 0 and lib.puff_policy_sm100_recurrence_saved_floats(2, 3, 4) >= 8
     ok = dict(gates=h[0], inputs=h[512], dtype=0, resets=h[1024], rb=4, state=h[1280], B=2, T=5, C=4, gb=20, gs=4, ib=20, is_=4,
-              out=h[2048], final=h[3072], saved=h[4096])
+              out=h[2048], final=h[3072], saved=h[4096], scratch=None, size=0)
     run = lambda **kw: lib.puff_policy_sm100_recurrence(*(ok | kw).values(), None)  # noqa: E731
     assert run(dtype=3) == run(rb=2) == cabi.ERR_DTYPE
     assert run(B=-1) == run(gs=-4) == cabi.ERR_SHAPE and run(B=1 << 30, C=1 << 30) == run(T=1 << 40) == cabi.ERR_SIZE
@@ -176,8 +176,14 @@ def test_recurrence_entry_point_checks():
     assert run(gates=h[2]) == run(state=h[1281]) == run(final=h[3073]) == cabi.ERR_ALIGN
     assert run(out=h[0]) == run(out=h[600]) == run(final=h[1280]) == run(saved=h[2048]) == run(final=h[1024]) == cabi.ERR_ALIAS
     assert run(B=0) == run(C=0) == cabi.OK
+    # one long row is cut into ranges whose joins need a workspace
+    big = dict(T=4000, gb=0, gs=0, ib=0, is_=0, resets=None, saved=None, out=h[1 << 20], final=h[4096])
+    need = lib.puff_policy_sm100_recurrence_scratch_bytes(2, 4000, 4)
+    assert need >= 16 and lib.puff_policy_sm100_recurrence_scratch_bytes(1 << 14, 64, 512) == 0
+    assert run(**big) == run(**big, scratch=h[8192], size=need - 1) == run(**big, scratch=h[8196], size=need) == cabi.ERR_WORKSPACE
+    assert run(**big, scratch=h[4096], size=need) == run(**big, scratch=h[1 << 20], size=need) == cabi.ERR_ALIAS
     b = dict(gates=h[0], inputs=h[512], dtype=0, resets=h[1024], rb=4, saved=h[1280], B=2, T=5, C=4, gb=20, gs=4, ib=20, is_=4,
-             dout=h[4096], dfinal=h[5120], dg=h[6144], dx=h[7168], ds=h[8192])
+             dout=h[4096], dfinal=h[5120], dg=h[6144], dx=h[7168], ds=h[8192], scratch=None, size=0)
     back = lambda **kw: lib.puff_policy_sm100_recurrence_backward(*(b | kw).values(), None)  # noqa: E731
     assert back(saved=None) == back(dg=None) == cabi.ERR_NULL and back(dg=h[4096]) == back(dx=h[6144]) == back(ds=h[1280]) == cabi.ERR_ALIAS
     s = dict(gates=h[0], inputs=h[512], dtype=0, resets=h[1024], rb=4, state=h[1280], B=2, C=4, gs=4, is_=4, out=h[2048], new=h[3072])
