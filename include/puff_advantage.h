@@ -337,8 +337,8 @@ int puff_priorities_sm100_weights_noalloc(const float* seg_abs_sum, float* weigh
  * row_stats (nullable): 2 fp32 per row for the backward pass, 8-byte aligned.
  * A logit of -inf is an action that cannot be taken.  A row with nothing but
  * -inf has log-probability -inf, entropy 0 and no gradient.  actions[r] < 0
- * marks padding: log-probability and entropy 0, no gradient, its logits are not
- * read.  actions[r] >= vocab does the same and raises the flag that
+ * marks padding: log-probability and entropy 0, no gradient, whatever its logits
+ * hold.  actions[r] >= vocab does the same and raises the flag that
  * puff_policy_sm100_bad_action() returns (and clears) after synchronising.
  *
  * _backward: dlogits (contiguous [outer * inner, vocab], every row written) =

@@ -6,6 +6,7 @@
 //
 // The step between the policy's logits and the ratio of pufferl.py:390-394 (the log-probability and entropy of
 // pufferlib/pytorch.py sample_logits), for action heads of a few entries up to vocabularies of 10^5 and more.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -15,6 +16,32 @@
 namespace puff {
 
 __device__ int g_bad_action = 0;
+
+constexpr int kLpMaxCluster = 8;
+
+// 16 bytes from global to shared memory without a register in between
+__device__ __forceinline__ void copy16_async(uint4* shared, const uint4* global)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared))),
+                 "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// bytes [shift, shift + 16) of the 32 in a, b; shift is even
+__device__ __forceinline__ uint4 cut_vector(uint4 a, uint4 b, unsigned shift)
+{
+    uint32_t w[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
+    const uint32_t last = b.w;
+    if (shift & 8u) {
+        w[0] = w[2], w[1] = w[3], w[2] = w[4], w[3] = w[5], w[4] = w[6], w[5] = last;
+    }
+    if (shift & 4u) {
+        w[0] = w[1], w[1] = w[2], w[2] = w[3], w[3] = w[4], w[4] = w[5];
+    }
+    const unsigned bits = (shift & 2u) * 8u;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                      __funnelshift_r(w[3], w[4], bits));
+}
 
 // where row r of a tensor with rows [outer, inner] starts, in elements
 struct RowMap {
@@ -65,23 +92,19 @@ __device__ __forceinline__ void soft_add_all(SoftSums& a, const float* x, float 
 #pragma unroll
     for (int i = 0; i < N; ++i) soft_add<ENT>(a, x[i], shift, c);
 }
+// sums of a team's threads over their warp: the common maximum first, then one rescaling each
 template <bool ENT>
-__device__ __forceinline__ void soft_join(SoftSums& a, SoftSums b, float c)
+__device__ __forceinline__ void soft_warp_join(SoftSums& a, float c)
 {
-    const float m = fmaxf(a.m, b.m);
+    float m = a.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     soft_rescale<ENT>(a, m, c);
-    soft_rescale<ENT>(b, m, c);
-    a.s += b.s;
-    if (ENT) a.u += b.u;
-}
-template <bool ENT>
-__device__ __forceinline__ SoftSums soft_shuffle(const SoftSums& a, int mask)
-{
-    SoftSums b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, mask);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, mask);
-    b.u = ENT ? __shfl_xor_sync(0xffffffffu, a.u, mask) : 0.0f;
-    return b;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        if (ENT) a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+    }
 }
 
 // One row read by `lanes` threads (this one is number `lane`): 16-byte loads between the row's first and last 16-byte
@@ -95,6 +118,10 @@ __device__ __forceinline__ SoftSums row_sums(const T* row, long long vocab, int 
     if (head > vocab) head = vocab;
     const long long nvec = (vocab - head) / N;
     const uint4* body = reinterpret_cast<const uint4*>(row + head);
+    // the ends: fewer than 2 N <= 32 elements, at most one each for the first warp's lanes; requested first
+    const long long tail = head + nvec * N;
+    const bool end = lane < head + (vocab - tail);
+    const float x_end = end ? to_f32(row[lane < head ? lane : tail + (lane - head)]) : 0.0f;
     constexpr int kBatch = 4;
     long long i = lane;
     for (; i + (kBatch - 1) * lanes < nvec; i += kBatch * lanes) {
@@ -111,117 +138,388 @@ __device__ __forceinline__ SoftSums row_sums(const T* row, long long vocab, int 
         Vec16<T>::unpack(__ldg(body + i), f);
         soft_add_all<ENT, N>(a, f, c);
     }
-    // the ends: fewer than 2 N elements
-    const long long tail = head + nvec * N;
-    for (long long j = lane; j < head + (vocab - tail); j += lanes) {
-        const float x = to_f32(row[j < head ? j : tail + (j - head)]);
-        soft_add_all<ENT, 1>(a, &x, c);
-    }
+    if (end) soft_add_all<ENT, 1>(a, &x_end, c);
     return a;
 }
 
-// One row per CTA of THREADS (32: one warp).
-template <typename T, bool ENT, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-puff_logprobs_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
-                     long long rows, long long vocab, float inv_temperature, float* __restrict__ logprobs,
-                     float* __restrict__ entropy, float2* __restrict__ row_stats)
+struct LogprobOut {
+    float* logprobs;
+    float* entropy;
+    float2* row_stats;
+};
+// what one thread writes for row r once its sums are known
+template <bool ENT>
+__device__ __forceinline__ void write_row(const LogprobOut& o, long long r, const SoftSums& a, float chosen, float inv_temperature)
 {
-    __shared__ SoftSums s_part[THREADS / 32];
+    // every logit -inf: no distribution; log-probability -inf, entropy 0, no gradient
+    const bool empty = a.m == -CUDART_INF_F && a.s == 0.0f;
+    const float log_s = empty ? 0.0f : logf(a.s);
+    o.logprobs[r] = empty ? -CUDART_INF_F : (chosen - a.m) * inv_temperature - log_s;
+    if (ENT) o.entropy[r] = empty ? 0.0f : log_s - kLn2 * (a.u / a.s);
+    if (o.row_stats != nullptr) o.row_stats[r] = make_float2(a.m, log_s);
+}
+template <bool ENT>
+__device__ __forceinline__ void write_padding(const LogprobOut& o, long long r, bool beyond)
+{
+    if (beyond) atomicExch(&g_bad_action, 1);
+    o.logprobs[r] = 0.0f;
+    if (ENT) o.entropy[r] = 0.0f;
+    if (o.row_stats != nullptr) o.row_stats[r] = make_float2(0.0f, 0.0f);
+}
+
+constexpr int kLpThreads = 256;
+constexpr int kLpWarps = kLpThreads / 32;
+
+// Forward, one row per warp: rows of a few KB, where a CTA would spend its time on joining.
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kLpThreads)
+puff_logprobs_warp_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
+                          long long rows, long long vocab, float inv_temperature, LogprobOut out)
+{
     const float c = inv_temperature * kLog2e;
-    for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int lane = threadIdx.x & 31;
+    const long long stride = static_cast<long long>(gridDim.x) * kLpWarps;
+    for (long long r = blockIdx.x * static_cast<long long>(kLpWarps) + (threadIdx.x >> 5); r < rows; r += stride) {
         const long long action = actions[amap.at(r)];
         if (action < 0 || action >= vocab) {
-            if (threadIdx.x == 0) {
-                if (action >= vocab) atomicExch(&g_bad_action, 1);
-                logprobs[r] = 0.0f;
-                if (ENT) entropy[r] = 0.0f;
-                if (row_stats != nullptr) row_stats[r] = make_float2(0.0f, 0.0f);
-            }
+            if (lane == 0) write_padding<ENT>(out, r, action >= vocab);
             continue;
         }
         const T* row = logits + lmap.at(r);
-        SoftSums a = row_sums<T, ENT>(row, vocab, threadIdx.x, THREADS, c);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) soft_join<ENT>(a, soft_shuffle<ENT>(a, o), c);
-        if (THREADS > 32) {
-            if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = a;
-            __syncthreads();
-            if (threadIdx.x == 0)
-                for (int w = 1; w < THREADS / 32; ++w) soft_join<ENT>(a, s_part[w], c);
-        }
-        if (threadIdx.x == 0) {
-            // every logit -inf: no distribution; log-probability -inf, entropy 0, no gradient
-            const bool empty = a.m == -CUDART_INF_F && a.s == 0.0f;
-            const float log_s = empty ? 0.0f : logf(a.s);
-            logprobs[r] = empty ? -CUDART_INF_F : (to_f32(row[action]) - a.m) * inv_temperature - log_s;
-            if (ENT) entropy[r] = empty ? 0.0f : log_s - kLn2 * (a.u / a.s);
-            if (row_stats != nullptr) row_stats[r] = make_float2(a.m, log_s);
-        }
-        if (THREADS > 32) __syncthreads();
+        const float chosen = to_f32(row[action]);
+        SoftSums a = row_sums<T, ENT>(row, vocab, lane, 32, c);
+        soft_warp_join<ENT>(a, c);
+        if (lane == 0) write_row<ENT>(out, r, a, chosen, inv_temperature);
     }
 }
 
-// One row per CTA; dlogits is contiguous.
-template <typename T, bool ENT, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+// Forward, one row per CTA, or per cluster of CTAs where rows are few: each takes a share of the row's vectors and the
+// first adds up what the others leave in its shared memory.
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kLpThreads)
+puff_logprobs_cta_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
+                         long long rows, long long vocab, float inv_temperature, LogprobOut out)
+{
+    __shared__ SoftSums s_part[kLpWarps];
+    __shared__ SoftSums s_cta[kLpMaxCluster];
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int share = static_cast<int>(cluster.block_rank()), shares = static_cast<int>(cluster.num_blocks());
+    const float c = inv_temperature * kLog2e;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (long long r = blockIdx.x / shares; r < rows; r += gridDim.x / shares) {
+        const long long action = actions[amap.at(r)];
+        const bool none = action < 0 || action >= vocab;
+        if (none) {
+            if (share == 0 && threadIdx.x == 0) write_padding<ENT>(out, r, action >= vocab);
+            continue;       // the same for every CTA of the cluster
+        }
+        const T* row = logits + lmap.at(r);
+        const float chosen = to_f32(row[action]);
+        SoftSums a = row_sums<T, ENT>(row, vocab, share * kLpThreads + threadIdx.x, shares * kLpThreads, c);
+        soft_warp_join<ENT>(a, c);
+        if (lane == 0) s_part[warp] = a;
+        __syncthreads();
+        if (warp == 0) {
+            a = lane < kLpWarps ? s_part[lane] : SoftSums{-CUDART_INF_F, 0.0f, 0.0f};
+            soft_warp_join<ENT>(a, c);
+            if (shares == 1) {
+                if (lane == 0) write_row<ENT>(out, r, a, chosen, inv_temperature);
+            } else if (lane == 0) {
+                *cluster.map_shared_rank(&s_cta[share], 0) = a;
+            }
+        }
+        if (shares > 1) {
+            cluster.sync();
+            if (share == 0 && warp == 0) {
+                a = lane < shares ? s_cta[lane] : SoftSums{-CUDART_INF_F, 0.0f, 0.0f};
+                soft_warp_join<ENT>(a, c);
+                if (lane == 0) write_row<ENT>(out, r, a, chosen, inv_temperature);
+            }
+            if (r + gridDim.x / shares < rows) cluster.sync();   // before s_cta is written again
+        } else {
+            __syncthreads();
+        }
+    }
+}
+
+// gradient of one logit
+template <bool ENT>
+__device__ __forceinline__ float logit_gradient(float x, float m, float log_s, float h, float dlp, float dh, float inv_temperature)
+{
+    const float logp = (x - m) * inv_temperature - log_s;
+    const float p = exp2_approx(logp * kLog2e);
+    float g = -dlp * p;
+    if (ENT) g = fmaf(-dh * p, fmaxf(logp, -1e4f) + h, g);
+    return g * inv_temperature;
+}
+
+// Backward of rows beyond the small kernel's: a warp takes 128 16-byte vectors of a row of dlogits (contiguous).  The
+// vectors are those of the output; where the row of logits lies at another offset from a 16-byte boundary, a vector is
+// cut out of the two aligned ones that hold it.  The first warp of a row also does the elements at its ends.
+constexpr int kLpUnitVecs = 4;      // vectors a lane
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kLpThreads)
 puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions,
-                              RowMap amap, long long rows, long long vocab, float inv_temperature,
+                              RowMap amap, long long rows, long long vocab, long long units_per_row, float inv_temperature,
                               const float2* __restrict__ row_stats, const float* __restrict__ entropy,
                               const float* __restrict__ dlogprobs, const float* __restrict__ dentropy,
                               T* __restrict__ dlogits)
 {
-    for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-        const long long action = actions[amap.at(r)];
-        const float2 st = row_stats[r];
-        T* out = dlogits + r * vocab;
-        const bool none = action < 0 || action >= vocab || (st.x == -CUDART_INF_F && st.y == 0.0f);
-        const T* row = logits + (none ? 0 : lmap.at(r));
-        const float dlp = none ? 0.0f : dlogprobs[r];
-        const float dh = none || !ENT ? 0.0f : dentropy[r], h = none || !ENT ? 0.0f : entropy[r];
-        for (long long j = threadIdx.x; j < vocab; j += THREADS) {
+    constexpr int N = Vec16<T>::N;
+    const int lane = threadIdx.x & 31;
+    const long long unit = blockIdx.x * static_cast<long long>(kLpWarps) + (threadIdx.x >> 5);
+    const long long r = unit / units_per_row;
+    if (r >= rows) return;
+    const long long chunk = unit - r * units_per_row;
+    const long long action = actions[amap.at(r)];
+    const float2 st = row_stats[r];
+    const float dlp = dlogprobs[r], dh = ENT ? dentropy[r] : 0.0f, h = ENT ? entropy[r] : 0.0f;
+    const T* row = logits + lmap.at(r);
+    T* out = dlogits + r * vocab;
+    const bool none = action < 0 || action >= vocab || (st.x == -CUDART_INF_F && st.y == 0.0f);
+    // vectors [0, nvec) start at element `head` of the row; shift: how far behind a boundary the logits' bytes lie
+    long long head = static_cast<long long>(((16u - (reinterpret_cast<uintptr_t>(out) & 15u)) & 15u) / sizeof(T));
+    const unsigned shift = static_cast<unsigned>(reinterpret_cast<uintptr_t>(row + head) & 15u);
+    if (shift != 0 && head * static_cast<long long>(sizeof(T)) < shift) head += N;   // the aligned vector would start before the row
+    long long nvec = shift == 0 ? (vocab - head) / N : ((vocab - head) * static_cast<long long>(sizeof(T)) + shift) / 16 - 1;
+    if (nvec < 0) nvec = 0;
+    const uint4* in = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row + head) & ~static_cast<uintptr_t>(15));
+    uint4* to = reinterpret_cast<uint4*>(out + head);
+    const long long first = chunk * (32 * kLpUnitVecs) + lane;
+    uint4 q[kLpUnitVecs];
+    if (!none) {
+#pragma unroll
+        for (int k = 0; k < kLpUnitVecs; ++k)
+            if (first + 32 * k < nvec) q[k] = __ldg(in + first + 32 * k);
+        if (shift != 0) {
+            uint4 next[kLpUnitVecs];
+#pragma unroll
+            for (int k = 0; k < kLpUnitVecs; ++k)
+                if (first + 32 * k < nvec) next[k] = __ldg(in + first + 32 * k + 1);
+#pragma unroll
+            for (int k = 0; k < kLpUnitVecs; ++k) q[k] = cut_vector(q[k], next[k], shift);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kLpUnitVecs; ++k) {
+        const long long i = first + 32 * k;
+        if (i >= nvec) break;
+        float f[N];
+        if (none) {
+#pragma unroll
+            for (int v = 0; v < N; ++v) f[v] = 0.0f;
+        } else {
+            Vec16<T>::unpack(q[k], f);
+            const long long at = action - (head + i * N);    // the chosen one among these?
+#pragma unroll
+            for (int v = 0; v < N; ++v) {
+                f[v] = logit_gradient<ENT>(f[v], st.x, st.y, h, dlp, dh, inv_temperature);
+                if (at == v) f[v] = fmaf(dlp, inv_temperature, f[v]);
+            }
+        }
+        to[i] = Vec16<T>::pack(f);
+    }
+    if (chunk == 0) {
+        const long long tail = head + nvec * N;
+        for (long long j = lane; j < head + (vocab - tail); j += 32) {
+            const long long e = j < head ? j : tail + (j - head);
+            if (e >= vocab) break;
             float g = 0.0f;
             if (!none) {
-                const float logp = (to_f32(row[j]) - st.x) * inv_temperature - st.y;
-                const float p = exp2_approx(logp * kLog2e);
-                g = -dlp * p;
-                if (ENT) g = fmaf(-dh * p, fmaxf(logp, -1e4f) + h, g);
-                if (j == action) g += dlp;
-                g *= inv_temperature;
+                g = logit_gradient<ENT>(to_f32(row[e]), st.x, st.y, h, dlp, dh, inv_temperature);
+                if (e == action) g = fmaf(dlp, inv_temperature, g);
             }
-            out[j] = from_f32<T>(g);
+            out[e] = from_f32<T>(g);
         }
     }
 }
 
-template <typename T, bool ENT>
-static void launch_logprobs(const void* logits, RowMap lmap, const long long* actions, RowMap amap, long long rows,
-                            long long vocab, float inv_t, float* logprobs, float* entropy, float* row_stats,
-                            cudaStream_t st)
+// Rows of up to kLpSmall entries, both directions.  A CTA brings 256 / G rows into shared memory by 16-byte copies of
+// their common span, wherever rows begin; G threads then work on a row from there (fewer than 33 elements each), and
+// the backward pass writes gradients over the logits and copies the span out.  The maximum and the sums are computed
+// again in the backward pass: reading them back would cost more than the arithmetic.  Rows start at different banks:
+// row i of the tile begins its walk i * skew elements in.
+constexpr int kLpSmall = 1024;
+template <typename T, bool ENT, int G, bool BACKWARD>
+__global__ void __launch_bounds__(kLpThreads)
+puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
+                           long long rows, int vocab, float inv_temperature, LogprobOut out,
+                           const float* __restrict__ dlogprobs, const float* __restrict__ dentropy, T* __restrict__ dlogits)
 {
-    const int grid = static_cast<int>(rows < (1 << 30) ? rows : (1 << 30));
-    if (vocab <= 2048)
-        puff_logprobs_kernel<T, ENT, 32><<<grid, 32, 0, st>>>(static_cast<const T*>(logits), lmap, actions, amap, rows,
-            vocab, inv_t, logprobs, entropy, reinterpret_cast<float2*>(row_stats));
-    else
-        puff_logprobs_kernel<T, ENT, 256><<<grid, 256, 0, st>>>(static_cast<const T*>(logits), lmap, actions, amap, rows,
-            vocab, inv_t, logprobs, entropy, reinterpret_cast<float2*>(row_stats));
+    extern __shared__ uint4 s_raw[];
+    constexpr int R = kLpThreads / G;
+    const long long r0 = static_cast<long long>(blockIdx.x) * R;
+    const int n_rows = static_cast<int>(rows - r0 < R ? rows - r0 : R);
+    const int local = threadIdx.x / G, g = threadIdx.x % G;
+    const bool has = local < n_rows;
+    const long long action = has ? actions[amap.at(r0 + local)] : -1;
+    const bool live = action >= 0 && action < vocab;
+    float dlp = 0.0f, dh = 0.0f;
+    if (BACKWARD && has) {
+        dlp = dlogprobs[r0 + local];
+        if (ENT) dh = dentropy[r0 + local];
+    }
+    // ---- in
+    const bool one_run = lmap.inner_stride == vocab && r0 / lmap.inner == (r0 + n_rows - 1) / lmap.inner;
+    const T* src = logits + lmap.at(r0);
+    const int count = n_rows * vocab;
+    const unsigned out_phase = BACKWARD ? static_cast<unsigned>(reinterpret_cast<uintptr_t>(dlogits + r0 * vocab) & 15u) : 0u;
+    const unsigned phase = one_run ? static_cast<unsigned>(reinterpret_cast<uintptr_t>(src) & 15u) : out_phase;
+    T* tile = reinterpret_cast<T*>(reinterpret_cast<char*>(s_raw) + phase);
+    constexpr int N = Vec16<T>::N;
+    const int head_all = static_cast<int>(((16u - phase) & 15u) / sizeof(T));
+    const int head = head_all < count ? head_all : count, body = (count - head) / N, tail = head + body * N;
+    if (one_run) {
+        for (int i = threadIdx.x; i < body; i += kLpThreads)
+            copy16_async(reinterpret_cast<uint4*>(tile + head) + i, reinterpret_cast<const uint4*>(src + head) + i);
+        if (static_cast<int>(threadIdx.x) < head + (count - tail)) {
+            const int e = static_cast<int>(threadIdx.x) < head ? threadIdx.x : tail + (threadIdx.x - head);
+            tile[e] = src[e];
+        }
+        copy_async_wait();
+    } else {
+        for (int i = threadIdx.x >> 5; i < n_rows; i += kLpWarps) {
+            const T* row = logits + lmap.at(r0 + i);
+            for (int j = threadIdx.x & 31; j < vocab; j += 32) tile[i * vocab + j] = row[j];
+        }
+    }
+    __syncthreads();
+    // ---- the sums of this thread's row
+    constexpr int kBankElems = 128 / sizeof(T);
+    const int skew = G == 1 ? (sizeof(T) == 4 ? 1 - (vocab & 1) : (2 - vocab) & 3)
+                            : ((G * (kBankElems / 32) - vocab) & (kBankElems - 1));
+    const int start = (local * skew) % vocab;
+    T* row = tile + local * vocab;
+    const float c = inv_temperature * kLog2e;
+    SoftSums a = {-CUDART_INF_F, 0.0f, 0.0f};
+    if (live) {
+        int j = start + g;
+        for (int k = g; k < vocab; k += G, j += G) a.m = fmaxf(a.m, to_f32(row[j < vocab ? j : j - vocab]));
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(0xffffffffu, a.m, o));
+    const float shift = a.m == -CUDART_INF_F ? 0.0f : a.m;
+    if (live) {
+        int j = start + g;
+        for (int k = g; k < vocab; k += G, j += G) soft_add<ENT>(a, to_f32(row[j < vocab ? j : j - vocab]), shift, c);
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        if (ENT) a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+    }
+    if (!BACKWARD) {
+        if (has && g == 0) {
+            if (live) write_row<ENT>(out, r0 + local, a, to_f32(row[action]), inv_temperature);
+            else write_padding<ENT>(out, r0 + local, action >= vocab);
+        }
+        return;
+    }
+    // ---- gradients over the logits
+    if (has) {
+        const bool none = !live || (a.m == -CUDART_INF_F && a.s == 0.0f);
+        const float log_s = none ? 0.0f : logf(a.s);
+        const float h = ENT && !none ? log_s - kLn2 * (a.u / a.s) : 0.0f;
+        int j = start + g;
+        for (int k = g; k < vocab; k += G, j += G) {
+            const int e = j < vocab ? j : j - vocab;
+            float d = 0.0f;
+            if (!none) {
+                d = logit_gradient<ENT>(to_f32(row[e]), a.m, log_s, h, dlp, dh, inv_temperature);
+                if (e == action) d = fmaf(dlp, inv_temperature, d);
+            }
+            row[e] = from_f32<T>(d);
+        }
+    }
+    __syncthreads();
+    // ---- out
+    T* dst = dlogits + r0 * vocab;
+    if (phase == out_phase) {
+        for (int i = threadIdx.x; i < body; i += kLpThreads)
+            reinterpret_cast<uint4*>(dst + head)[i] = reinterpret_cast<const uint4*>(tile + head)[i];
+        if (static_cast<int>(threadIdx.x) < head + (count - tail)) {
+            const int e = static_cast<int>(threadIdx.x) < head ? threadIdx.x : tail + (threadIdx.x - head);
+            dst[e] = tile[e];
+        }
+    } else {
+        for (int i = threadIdx.x; i < count; i += kLpThreads) dst[i] = tile[i];
+    }
+}
+
+template <typename T, bool ENT, bool BACKWARD>
+static cudaError_t launch_small(const void* logits, RowMap lmap, const long long* actions, RowMap amap, long long rows,
+                                long long vocab, float inv_t, LogprobOut out, const float* dlogprobs, const float* dentropy,
+                                void* dlogits, cudaStream_t st)
+{
+    int g = 1;
+    while (g < 32 && vocab > 32 * g) g *= 2;
+    const long long tile = kLpThreads / g;
+    const size_t smem = static_cast<size_t>(tile) * vocab * sizeof(T) + 32;
+    const int grid = static_cast<int>((rows + tile - 1) / tile);
+#define PUFF_SMALL(G)                                                                                                       \
+    puff_logprobs_small_kernel<T, ENT, G, BACKWARD><<<grid, kLpThreads, smem, st>>>(                                        \
+        static_cast<const T*>(logits), lmap, actions, amap, rows, static_cast<int>(vocab), inv_t, out, dlogprobs, dentropy, \
+        static_cast<T*>(dlogits))
+    if (g == 1) PUFF_SMALL(1);
+    else if (g == 2) PUFF_SMALL(2);
+    else if (g == 4) PUFF_SMALL(4);
+    else if (g == 8) PUFF_SMALL(8);
+    else if (g == 16) PUFF_SMALL(16);
+    else PUFF_SMALL(32);
+#undef PUFF_SMALL
+    return cudaGetLastError();
+}
+
+template <typename T, bool ENT>
+static cudaError_t launch_logprobs(const void* logits, RowMap lmap, const long long* actions, RowMap amap, long long rows,
+                                   long long vocab, float inv_t, float* logprobs, float* entropy, float* row_stats,
+                                   cudaStream_t st)
+{
+    const LogprobOut out = {logprobs, entropy, reinterpret_cast<float2*>(row_stats)};
+    if (vocab <= kLpSmall)
+        return launch_small<T, ENT, false>(logits, lmap, actions, amap, rows, vocab, inv_t, out, nullptr, nullptr, nullptr, st);
+    const T* z = static_cast<const T*>(logits);
+    const long long bytes = vocab * static_cast<long long>(sizeof(T));
+    // a warp a row while rows are short and many enough to give every SM sixteen warps
+    if (bytes <= 16384 && rows >= 148 * 16) {
+        const long long grid = (rows + kLpWarps - 1) / kLpWarps;
+        puff_logprobs_warp_kernel<T, ENT><<<static_cast<int>(grid < (1 << 30) ? grid : (1 << 30)), kLpThreads, 0, st>>>(
+            z, lmap, actions, amap, rows, vocab, inv_t, out);
+        return cudaGetLastError();
+    }
+    // otherwise a CTA, or two, four, eight while that leaves SMs idle and each thread has two vectors to read
+    int shares = 1;
+    while (shares < kLpMaxCluster && rows * shares < 148 * 2 && bytes >= 2LL * shares * kLpThreads * 32) shares *= 2;
+    const long long grid = rows < (1 << 26) ? rows : (1 << 26);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid * shares));
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(shares);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, puff_logprobs_cta_kernel<T, ENT>, z, lmap, actions, amap, rows, vocab, inv_t, out);
 }
 template <typename T, bool ENT>
-static void launch_logprobs_backward(const void* logits, RowMap lmap, const long long* actions, RowMap amap,
-                                     long long rows, long long vocab, float inv_t, const float* row_stats,
-                                     const float* entropy, const float* dlogprobs, const float* dentropy, void* dlogits,
-                                     cudaStream_t st)
+static cudaError_t launch_logprobs_backward(const void* logits, RowMap lmap, const long long* actions, RowMap amap,
+                                            long long rows, long long vocab, float inv_t, const float* row_stats,
+                                            const float* entropy, const float* dlogprobs, const float* dentropy,
+                                            void* dlogits, cudaStream_t st)
 {
-    const int grid = static_cast<int>(rows < (1 << 30) ? rows : (1 << 30));
-    if (vocab <= 2048)
-        puff_logprobs_backward_kernel<T, ENT, 32><<<grid, 32, 0, st>>>(static_cast<const T*>(logits), lmap, actions, amap,
-            rows, vocab, inv_t, reinterpret_cast<const float2*>(row_stats), entropy, dlogprobs, dentropy,
-            static_cast<T*>(dlogits));
-    else
-        puff_logprobs_backward_kernel<T, ENT, 256><<<grid, 256, 0, st>>>(static_cast<const T*>(logits), lmap, actions,
-            amap, rows, vocab, inv_t, reinterpret_cast<const float2*>(row_stats), entropy, dlogprobs, dentropy,
-            static_cast<T*>(dlogits));
+    if (vocab <= kLpSmall)
+        return launch_small<T, ENT, true>(logits, lmap, actions, amap, rows, vocab, inv_t, LogprobOut{}, dlogprobs, dentropy,
+                                          dlogits, st);
+    constexpr long long per_unit = 32LL * kLpUnitVecs * Vec16<T>::N;
+    const long long units = (vocab + per_unit - 1) / per_unit;
+    const long long grid = (rows * units + kLpWarps - 1) / kLpWarps;
+    puff_logprobs_backward_kernel<T, ENT><<<static_cast<unsigned>(grid), kLpThreads, 0, st>>>(
+        static_cast<const T*>(logits), lmap, actions, amap, rows, vocab, units, inv_t,
+        reinterpret_cast<const float2*>(row_stats), entropy, dlogprobs, dentropy, static_cast<T*>(dlogits));
+    return cudaGetLastError();
 }
 
 // bytes from the first to one past the last element of rows [outer, inner] of `width` elements
@@ -239,7 +537,7 @@ static int check_logprobs(const void* logits, int dtype, const long long* action
     const int size = dtype_bytes(dtype);
     if (size == 0) return PUFF_ERR_DTYPE;
     if (outer < 0 || inner < 0 || vocab < 0 || los < 0 || lis < 0 || aos < 0 || ais < 0) return PUFF_ERR_SHAPE;
-    if (!(temperature > 0.0f) || temperature > 3.0e38f || 1.0f / temperature > 3.0e38f) return PUFF_ERR_VALUE;
+    if (!(temperature > 0.0f) || temperature > 3.0e38f || 1.5f / temperature > 3.0e38f) return PUFF_ERR_VALUE;
     if (outer == 0 || inner == 0) return PUFF_OK;
     if (vocab == 0) return PUFF_ERR_SHAPE;
     if (inner > (1LL << 40) / outer) return PUFF_ERR_SIZE;
@@ -287,12 +585,10 @@ extern "C" int puff_policy_sm100_logprobs(const void* logits, int dtype, const l
                                                    row_stats, st)                                                          \
                         : launch_logprobs<T, false>(logits, lmap, actions, amap, rows, vocab, inv_t, logprobs, entropy,    \
                                                     row_stats, st))
-    if (dtype == PUFF_DTYPE_F32) PUFF_RUN(float);
-    else if (dtype == PUFF_DTYPE_F16) PUFF_RUN(__half);
-    else PUFF_RUN(__nv_bfloat16);
+    const cudaError_t e = dtype == PUFF_DTYPE_F32 ? PUFF_RUN(float) : dtype == PUFF_DTYPE_F16 ? PUFF_RUN(__half) : PUFF_RUN(__nv_bfloat16);
 #undef PUFF_RUN
     count_launch();
-    return static_cast<int>(cudaGetLastError());
+    return static_cast<int>(e);
 }
 
 extern "C" int puff_policy_sm100_logprobs_backward(const void* logits, int dtype, const long long* actions,
@@ -331,12 +627,10 @@ extern "C" int puff_policy_sm100_logprobs_backward(const void* logits, int dtype
                                                              entropy, dlogprobs, dentropy, dlogits, st)                   \
                          : launch_logprobs_backward<T, false>(logits, lmap, actions, amap, rows, vocab, inv_t, row_stats, \
                                                               entropy, dlogprobs, dentropy, dlogits, st))
-    if (dtype == PUFF_DTYPE_F32) PUFF_RUN(float);
-    else if (dtype == PUFF_DTYPE_F16) PUFF_RUN(__half);
-    else PUFF_RUN(__nv_bfloat16);
+    const cudaError_t e = dtype == PUFF_DTYPE_F32 ? PUFF_RUN(float) : dtype == PUFF_DTYPE_F16 ? PUFF_RUN(__half) : PUFF_RUN(__nv_bfloat16);
 #undef PUFF_RUN
     count_launch();
-    return static_cast<int>(cudaGetLastError());
+    return static_cast<int>(e);
 }
 
 extern "C" int puff_policy_sm100_bad_action(void)
