@@ -46,18 +46,82 @@ __device__ __forceinline__ uint4 cut_vector(uint4 a, uint4 b, unsigned shift)
 // where row r of a tensor with rows [outer, inner] starts, in elements
 struct RowMap {
     long long inner, outer_stride, inner_stride;
+    bool one_run;      // a single run of rows: nothing to divide
     __device__ __forceinline__ long long at(long long r) const
     {
-        const long long o = r / inner;
+        if (one_run) return r * inner_stride;
+        const long long o = ((r | inner) >> 32) == 0 ? static_cast<unsigned>(r) / static_cast<unsigned>(inner) : r / inner;
         return o * outer_stride + (r - o * inner) * inner_stride;
     }
 };
+
+// -inf (an illegal action) would make 0 x inf of the entropy's terms: it is raised to a value whose exponential is 0
+// all the same, two packed elements at once, as long as the row's maximum is far enough above it.
+template <typename T> __device__ __forceinline__ float raised_inf() { return sizeof(T) == 2 ? -60000.0f : -1e30f; }
+template <> __device__ __forceinline__ float raised_inf<__nv_bfloat16>() { return -9.969209968386869e29f; }   // a bf16 value
+__device__ __forceinline__ uint32_t raise2(uint32_t w, __half)
+{
+    const __half2 p = __hmax2_nan(*reinterpret_cast<const __half2*>(&w), __float2half2_rn(raised_inf<__half>()));
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t raise2(uint32_t w, __nv_bfloat16)
+{
+    const __nv_bfloat162 p = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w), __float2bfloat162_rn(raised_inf<__nv_bfloat16>()));
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t raise2(uint32_t w, float)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(__uint_as_float(w)), "f"(raised_inf<float>()));
+    return __float_as_uint(y);
+}
+template <typename T> __device__ __forceinline__ uint4 raise_vector(const uint4& q)
+{
+    return make_uint4(raise2(q.x, T()), raise2(q.y, T()), raise2(q.z, T()), raise2(q.w, T()));
+}
+// the largest element of 16 bytes (NaN aside)
+__device__ __forceinline__ float vector_max(const uint4& q, float)
+{
+    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+}
+__device__ __forceinline__ float vector_max(const uint4& q, __half)
+{
+    const __half2* w = reinterpret_cast<const __half2*>(&q);
+    const __half2 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float vector_max(const uint4& q, __nv_bfloat16)
+{
+    const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&q);
+    const __nv_bfloat162 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
 
 // Running softmax sums of a set of logits x, in units of log2: with t = (x - m) c, c = log2(e) / temperature,
 // s = sum 2^t and u = sum t 2^t.  m is the largest x so far (-inf: none, or only -inf, which leave s and u alone).
 struct SoftSums {
     float m, s, u;
 };
+// How t is computed.  One fused multiply-add x c - sc does it, sc being m c rounded, off by the known d = m c - sc for
+// every element alike: the sums are corrected by k = 2^-d afterwards.  Where m is so large that d matters, or so low
+// that the raised -inf would count, `direct`: (x - m) c, element by element.
+struct SoftScale {
+    float sc, d, k;
+    bool direct;
+};
+template <typename T>
+__device__ __forceinline__ SoftScale soft_scale(float m, float c)
+{
+    SoftScale z = {0.0f, 0.0f, 1.0f, false};
+    const float top = m == -CUDART_INF_F ? 0.0f : m;
+    z.sc = __fmul_rn(top, c);
+    z.direct = !(fabsf(z.sc) <= 1e6f && (raised_inf<T>() - top) * c < -200.0f);
+    if (!z.direct) {
+        z.d = fmaf(top, c, -z.sc);
+        z.k = exp2_approx(-z.d);
+    }
+    return z;
+}
 
 template <bool ENT>
 __device__ __forceinline__ void soft_rescale(SoftSums& a, float m_new, float c)
@@ -73,24 +137,68 @@ __device__ __forceinline__ void soft_rescale(SoftSums& a, float m_new, float c)
     }
 }
 template <bool ENT>
-__device__ __forceinline__ void soft_add(SoftSums& a, float x, float shift, float c)
+__device__ __forceinline__ void soft_add(SoftSums& a, float x, float c)
 {
-    const float t = (x - shift) * c;
+    const float t = (x - (a.m == -CUDART_INF_F ? 0.0f : a.m)) * c;
     const float e = exp2_approx(t);
     a.s += e;
-    if (ENT) a.u = fmaf(e, fmaxf(t, -1e4f), a.u);   // -inf (an illegal action) adds 0; NaN comes in through e
+    if (ENT) a.u = fmaf(e, fmaxf(t, -1e4f), a.u);   // NaN comes in through e
 }
-// n values at once: their maximum first, then one rescaling for all of them
-template <bool ENT, int N>
-__device__ __forceinline__ void soft_add_all(SoftSums& a, const float* x, float c)
+// What 16-byte vectors q[k], of which `valid` has a bit each, add to s and u under the scale z
+template <typename T, bool ENT, int K>
+__device__ __forceinline__ float2 soft_terms(const SoftScale& z, const uint4 (&q)[K], unsigned valid, float c)
 {
-    float top = x[0];
+    constexpr int N = Vec16<T>::N;
+    float2 s = make_float2(0.0f, 0.0f), u = make_float2(0.0f, 0.0f);
+    const float2 c2 = make_float2(c, c), sc2 = make_float2(-z.sc, -z.sc);
 #pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-    soft_rescale<ENT>(a, top, c);
-    const float shift = a.m == -CUDART_INF_F ? 0.0f : a.m;
+    for (int k = 0; k < K; ++k) {
+        if (!(valid >> k & 1u)) continue;
+        float f[N];
+        Vec16<T>::unpack(ENT ? raise_vector<T>(q[k]) : q[k], f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) soft_add<ENT>(a, x[i], shift, c);
+        for (int i = 0; i < N; i += 2) {
+            const float2 t = __ffma2_rn(make_float2(f[i], f[i + 1]), c2, sc2);
+            const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+            s = __fadd2_rn(s, e);
+            if (ENT) u = __ffma2_rn(e, t, u);
+        }
+    }
+    return make_float2(s.x + s.y, u.x + u.y);
+}
+// The reference m need not be the maximum: it is kept while the new terms stay below 2^12, which costs no more than
+// 12 ln 2 |log-probability| in rounding steps and spares looking for the maximum (half an instruction an element, and
+// everything waiting for it).  Otherwise: the vectors' maximum, one rescaling, and their terms again.
+template <typename T, bool ENT, int K>
+__device__ __forceinline__ void soft_add_vectors(SoftSums& a, SoftScale& z, const uint4 (&q)[K], unsigned valid, float c)
+{
+    constexpr int N = Vec16<T>::N;
+    float2 su = make_float2(CUDART_INF_F, 0.0f);
+    if (a.m != -CUDART_INF_F && !z.direct) su = soft_terms<T, ENT, K>(z, q, valid, c);
+    if (!(su.x <= 4096.0f)) {
+        float top = -CUDART_INF_F;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (valid >> k & 1u) top = fmaxf(top, vector_max(q[k], T()));
+        if (top > a.m) {
+            soft_rescale<ENT>(a, top, c);
+            z = soft_scale<T>(a.m, c);
+        }
+        if (z.direct) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!(valid >> k & 1u)) continue;
+                float f[N];
+                Vec16<T>::unpack(q[k], f);
+#pragma unroll
+                for (int i = 0; i < N; ++i) soft_add<ENT>(a, f[i], c);
+            }
+            return;
+        }
+        su = soft_terms<T, ENT, K>(z, q, valid, c);
+    }
+    a.s = fmaf(su.x, z.k, a.s);
+    if (ENT) a.u = fmaf(fmaf(-z.d, su.x, su.y), z.k, a.u);
 }
 // sums of a team's threads over their warp: the common maximum first, then one rescaling each
 template <bool ENT>
@@ -107,13 +215,32 @@ __device__ __forceinline__ void soft_warp_join(SoftSums& a, float c)
     }
 }
 
-// One row read by `lanes` threads (this one is number `lane`): 16-byte loads between the row's first and last 16-byte
+// A thread's own ring of 16-byte slots in shared memory, filled by asynchronous copies and read by nobody else, so that
+// no thread waits for another: kRing - 1 groups of kGroup vectors are on their way while one is used, for no registers.
+constexpr int kLpThreads = 256;
+constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kGroup = 2, kRing = 5;
+struct VectorRing {
+    uint4* slots;      // [kRing][kGroup] for this thread, kLpThreads apart
+    __device__ __forceinline__ uint4* at(int stage, int k) const { return slots + (stage * kGroup + k) * kLpThreads; }
+    // vectors i, i + lanes, ... of a row of nvec into a stage
+    __device__ __forceinline__ void request(int stage, const uint4* body, long long i, int lanes, long long nvec) const
+    {
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k)
+            if (i + k * lanes < nvec) copy16_async(at(stage, k), body + i + k * lanes);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+};
+
+// One row read by `lanes` threads (this one is number `lane`): 16-byte vectors between the row's first and last 16-byte
 // boundary, single elements outside.
 template <typename T, bool ENT>
-__device__ __forceinline__ SoftSums row_sums(const T* row, long long vocab, int lane, int lanes, float c)
+__device__ __forceinline__ SoftSums row_sums(const T* row, long long vocab, int lane, int lanes, float c, const VectorRing& ring)
 {
     constexpr int N = Vec16<T>::N;
     SoftSums a = {-CUDART_INF_F, 0.0f, 0.0f};
+    SoftScale z = soft_scale<T>(a.m, c);
     long long head = static_cast<long long>(((16u - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / sizeof(T));
     if (head > vocab) head = vocab;
     const long long nvec = (vocab - head) / N;
@@ -122,23 +249,31 @@ __device__ __forceinline__ SoftSums row_sums(const T* row, long long vocab, int 
     const long long tail = head + nvec * N;
     const bool end = lane < head + (vocab - tail);
     const float x_end = end ? to_f32(row[lane < head ? lane : tail + (lane - head)]) : 0.0f;
-    constexpr int kBatch = 4;
-    long long i = lane;
-    for (; i + (kBatch - 1) * lanes < nvec; i += kBatch * lanes) {
-        uint4 q[kBatch];
+    const int step = kGroup * lanes;
+    long long ahead = lane;
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) q[k] = __ldg(body + i + k * lanes);
-        float f[kBatch * N];
+    for (int st = 0; st < kRing - 1; ++st, ahead += step) ring.request(st, body, ahead, lanes, nvec);
+    int stage = 0;
+    for (long long i = lane; i < nvec; i += step, ahead += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+        uint4 q[kGroup];
+        unsigned valid = 0;
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) Vec16<T>::unpack(q[k], f + k * N);
-        soft_add_all<ENT, kBatch * N>(a, f, c);
+        for (int k = 0; k < kGroup; ++k)
+            if (i + k * lanes < nvec) {
+                q[k] = *ring.at(stage, k);
+                valid |= 1u << k;
+            }
+        // the stage before this one is free: its vectors were in registers a round ago
+        ring.request(stage == 0 ? kRing - 1 : stage - 1, body, ahead, lanes, nvec);
+        soft_add_vectors<T, ENT, kGroup>(a, z, q, valid, c);
+        stage = stage == kRing - 1 ? 0 : stage + 1;
     }
-    for (; i < nvec; i += lanes) {
-        float f[N];
-        Vec16<T>::unpack(__ldg(body + i), f);
-        soft_add_all<ENT, N>(a, f, c);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (end) {
+        soft_rescale<ENT>(a, x_end, c);
+        soft_add<ENT>(a, x_end, c);
     }
-    if (end) soft_add_all<ENT, 1>(a, &x_end, c);
     return a;
 }
 
@@ -167,15 +302,14 @@ __device__ __forceinline__ void write_padding(const LogprobOut& o, long long r, 
     if (o.row_stats != nullptr) o.row_stats[r] = make_float2(0.0f, 0.0f);
 }
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
-
 // Forward, one row per warp: rows of a few KB, where a CTA would spend its time on joining.
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kLpThreads)
+__global__ void __launch_bounds__(kLpThreads, 4)
 puff_logprobs_warp_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
                           long long rows, long long vocab, float inv_temperature, LogprobOut out)
 {
+    __shared__ uint4 s_ring[kRing * kGroup * kLpThreads];
+    const VectorRing ring = {s_ring + threadIdx.x};
     const float c = inv_temperature * kLog2e;
     const int lane = threadIdx.x & 31;
     const long long stride = static_cast<long long>(gridDim.x) * kLpWarps;
@@ -187,7 +321,7 @@ puff_logprobs_warp_kernel(const T* __restrict__ logits, RowMap lmap, const long 
         }
         const T* row = logits + lmap.at(r);
         const float chosen = to_f32(row[action]);
-        SoftSums a = row_sums<T, ENT>(row, vocab, lane, 32, c);
+        SoftSums a = row_sums<T, ENT>(row, vocab, lane, 32, c, ring);
         soft_warp_join<ENT>(a, c);
         if (lane == 0) write_row<ENT>(out, r, a, chosen, inv_temperature);
     }
@@ -196,15 +330,17 @@ puff_logprobs_warp_kernel(const T* __restrict__ logits, RowMap lmap, const long 
 // Forward, one row per CTA, or per cluster of CTAs where rows are few: each takes a share of the row's vectors and the
 // first adds up what the others leave in its shared memory.
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kLpThreads)
+__global__ void __launch_bounds__(kLpThreads, 4)
 puff_logprobs_cta_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
                          long long rows, long long vocab, float inv_temperature, LogprobOut out)
 {
+    __shared__ uint4 s_ring[kRing * kGroup * kLpThreads];
     __shared__ SoftSums s_part[kLpWarps];
     __shared__ SoftSums s_cta[kLpMaxCluster];
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
     const int share = static_cast<int>(cluster.block_rank()), shares = static_cast<int>(cluster.num_blocks());
+    const VectorRing ring = {s_ring + threadIdx.x};
     const float c = inv_temperature * kLog2e;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (long long r = blockIdx.x / shares; r < rows; r += gridDim.x / shares) {
@@ -216,7 +352,7 @@ puff_logprobs_cta_kernel(const T* __restrict__ logits, RowMap lmap, const long l
         }
         const T* row = logits + lmap.at(r);
         const float chosen = to_f32(row[action]);
-        SoftSums a = row_sums<T, ENT>(row, vocab, share * kLpThreads + threadIdx.x, shares * kLpThreads, c);
+        SoftSums a = row_sums<T, ENT>(row, vocab, share * kLpThreads + threadIdx.x, shares * kLpThreads, c, ring);
         soft_warp_join<ENT>(a, c);
         if (lane == 0) s_part[warp] = a;
         __syncthreads();
@@ -243,15 +379,40 @@ puff_logprobs_cta_kernel(const T* __restrict__ logits, RowMap lmap, const long l
     }
 }
 
-// gradient of one logit
-template <bool ENT>
-__device__ __forceinline__ float logit_gradient(float x, float m, float log_s, float h, float dlp, float dh, float inv_temperature)
+// The gradient of a row's logits as p (A + B t) with t = log2 p: A = -(dlp + dh H) / temperature, B = -dh ln 2 /
+// temperature.  t is one multiply-add again, x c - l with l = m c + log2 s rounded and its error d carried into A and the
+// factor 2^-d of both; `direct` as in SoftScale.
+struct RowGradient {
+    float c, l, a, b, m, log2_s, dlp;
+    bool direct;
+};
+template <typename T, bool ENT>
+__device__ __forceinline__ RowGradient row_gradient(float m, float log_s, float h, float dlp, float dh, float inv_temperature)
 {
-    const float logp = (x - m) * inv_temperature - log_s;
-    const float p = exp2_approx(logp * kLog2e);
-    float g = -dlp * p;
-    if (ENT) g = fmaf(-dh * p, fmaxf(logp, -1e4f) + h, g);
-    return g * inv_temperature;
+    RowGradient g;
+    g.c = inv_temperature * kLog2e;
+    g.m = m;
+    g.log2_s = __fmul_rn(log_s, kLog2e);
+    g.dlp = dlp * inv_temperature;
+    const float mc = __fmul_rn(m, g.c);      // rounded here: the errors below are of these very values
+    g.l = __fadd_rn(mc, g.log2_s);
+    g.direct = !(fabsf(g.l) <= 1e6f && fabsf(mc) <= 1e6f && (raised_inf<T>() - m) * g.c < -200.0f);
+    float d = 0.0f;
+    if (!g.direct) {
+        const float back = __fsub_rn(g.l, mc);
+        d = fmaf(m, g.c, -mc) + __fadd_rn(__fsub_rn(mc, __fsub_rn(g.l, back)), __fsub_rn(g.log2_s, back));
+    }
+    const float k = exp2_approx(-d) * inv_temperature;
+    g.b = ENT ? -dh * kLn2 * k : 0.0f;
+    g.a = ENT ? -fmaf(dh, fmaf(-kLn2, d, h), dlp) * k : -dlp * k;
+    return g;
+}
+template <bool ENT>
+__device__ __forceinline__ float logit_gradient(float x, const RowGradient& g)
+{
+    const float t = g.direct ? fmaf(x - g.m, g.c, -g.log2_s) : fmaf(x, g.c, -g.l);
+    const float p = exp2_approx(t);
+    return p * (ENT ? fmaf(g.b, fmaxf(t, -1e4f), g.a) : g.a);
 }
 
 // Backward of rows beyond the small kernel's: a warp takes 128 16-byte vectors of a row of dlogits (contiguous).  The
@@ -259,25 +420,30 @@ __device__ __forceinline__ float logit_gradient(float x, float m, float log_s, f
 // cut out of the two aligned ones that hold it.  The first warp of a row also does the elements at its ends.
 constexpr int kLpUnitVecs = 4;      // vectors a lane
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kLpThreads)
+__global__ void __launch_bounds__(kLpThreads, 4)
 puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions,
-                              RowMap amap, long long rows, long long vocab, long long units_per_row, float inv_temperature,
-                              const float2* __restrict__ row_stats, const float* __restrict__ entropy,
+                              RowMap amap, long long rows, long long vocab, int warps_per_row, unsigned ctas_per_row,
+                              float inv_temperature, const float2* __restrict__ row_stats, const float* __restrict__ entropy,
                               const float* __restrict__ dlogprobs, const float* __restrict__ dentropy,
                               T* __restrict__ dlogits)
 {
     constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 31;
-    const long long unit = blockIdx.x * static_cast<long long>(kLpWarps) + (threadIdx.x >> 5);
-    const long long r = unit / units_per_row;
+    // 8 / warps_per_row rows a CTA, or ctas_per_row CTAs a row
+    const unsigned block_row = blockIdx.x / ctas_per_row;
+    const int warp = threadIdx.x >> 5;
+    const long long r = static_cast<long long>(block_row) * (kLpWarps / warps_per_row) + warp / warps_per_row;
     if (r >= rows) return;
-    const long long chunk = unit - r * units_per_row;
+    const long long chunk = (blockIdx.x - block_row * ctas_per_row) * kLpWarps + warp % warps_per_row;
     const long long action = actions[amap.at(r)];
     const float2 st = row_stats[r];
     const float dlp = dlogprobs[r], dh = ENT ? dentropy[r] : 0.0f, h = ENT ? entropy[r] : 0.0f;
     const T* row = logits + lmap.at(r);
     T* out = dlogits + r * vocab;
     const bool none = action < 0 || action >= vocab || (st.x == -CUDART_INF_F && st.y == 0.0f);
+    const RowGradient grad = row_gradient<T, ENT>(st.x, st.y, h, dlp, dh, inv_temperature);
+    const float2 a2 = make_float2(grad.a, grad.a), b2 = make_float2(grad.b, grad.b);
+    const float2 c2 = make_float2(grad.c, grad.c), l2 = make_float2(-grad.l, -grad.l);
     // vectors [0, nvec) start at element `head` of the row; shift: how far behind a boundary the logits' bytes lie
     long long head = static_cast<long long>(((16u - (reinterpret_cast<uintptr_t>(out) & 15u)) & 15u) / sizeof(T));
     const unsigned shift = static_cast<unsigned>(reinterpret_cast<uintptr_t>(row + head) & 15u);
@@ -310,12 +476,25 @@ puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const l
 #pragma unroll
             for (int v = 0; v < N; ++v) f[v] = 0.0f;
         } else {
-            Vec16<T>::unpack(q[k], f);
-            const long long at = action - (head + i * N);    // the chosen one among these?
+            if (grad.direct) {
+                Vec16<T>::unpack(q[k], f);
 #pragma unroll
-            for (int v = 0; v < N; ++v) {
-                f[v] = logit_gradient<ENT>(f[v], st.x, st.y, h, dlp, dh, inv_temperature);
-                if (at == v) f[v] = fmaf(dlp, inv_temperature, f[v]);
+                for (int v = 0; v < N; ++v) f[v] = logit_gradient<ENT>(f[v], grad);
+            } else {
+                Vec16<T>::unpack(ENT ? raise_vector<T>(q[k]) : q[k], f);
+#pragma unroll
+                for (int v = 0; v < N; v += 2) {
+                    const float2 t = __ffma2_rn(make_float2(f[v], f[v + 1]), c2, l2);
+                    const float2 p = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+                    const float2 d = __fmul2_rn(p, ENT ? __ffma2_rn(b2, t, a2) : a2);
+                    f[v] = d.x;
+                    f[v + 1] = d.y;
+                }
+            }
+            const long long at = action - (head + i * N);
+            if (at >= 0 && at < N) {                         // the chosen one is among these
+#pragma unroll
+                for (int v = 0; v < N; ++v) f[v] += at == v ? grad.dlp : 0.0f;
             }
         }
         to[i] = Vec16<T>::pack(f);
@@ -327,8 +506,8 @@ puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const l
             if (e >= vocab) break;
             float g = 0.0f;
             if (!none) {
-                g = logit_gradient<ENT>(to_f32(row[e]), st.x, st.y, h, dlp, dh, inv_temperature);
-                if (e == action) g = fmaf(dlp, inv_temperature, g);
+                g = logit_gradient<ENT>(to_f32(row[e]), grad);
+                if (e == action) g += grad.dlp;
             }
             out[e] = from_f32<T>(g);
         }
@@ -340,7 +519,7 @@ puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const l
 // the backward pass writes gradients over the logits and copies the span out.  The maximum and the sums are computed
 // again in the backward pass: reading them back would cost more than the arithmetic.  Rows start at different banks:
 // row i of the tile begins its walk i * skew elements in.
-constexpr int kLpSmall = 1024;
+constexpr int kLpSmall = 128;
 template <typename T, bool ENT, int G, bool BACKWARD>
 __global__ void __launch_bounds__(kLpThreads)
 puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
@@ -361,7 +540,7 @@ puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long
         if (ENT) dh = dentropy[r0 + local];
     }
     // ---- in
-    const bool one_run = lmap.inner_stride == vocab && r0 / lmap.inner == (r0 + n_rows - 1) / lmap.inner;
+    const bool one_run = lmap.inner_stride == vocab && (lmap.one_run || r0 / lmap.inner == (r0 + n_rows - 1) / lmap.inner);
     const T* src = logits + lmap.at(r0);
     const int count = n_rows * vocab;
     const unsigned out_phase = BACKWARD ? static_cast<unsigned>(reinterpret_cast<uintptr_t>(dlogits + r0 * vocab) & 15u) : 0u;
@@ -399,10 +578,9 @@ puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long
     }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(0xffffffffu, a.m, o));
-    const float shift = a.m == -CUDART_INF_F ? 0.0f : a.m;
     if (live) {
         int j = start + g;
-        for (int k = g; k < vocab; k += G, j += G) soft_add<ENT>(a, to_f32(row[j < vocab ? j : j - vocab]), shift, c);
+        for (int k = g; k < vocab; k += G, j += G) soft_add<ENT>(a, to_f32(row[j < vocab ? j : j - vocab]), c);
     }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) {
@@ -421,13 +599,14 @@ puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long
         const bool none = !live || (a.m == -CUDART_INF_F && a.s == 0.0f);
         const float log_s = none ? 0.0f : logf(a.s);
         const float h = ENT && !none ? log_s - kLn2 * (a.u / a.s) : 0.0f;
+        const RowGradient grad = row_gradient<T, ENT>(a.m, log_s, h, dlp, dh, inv_temperature);
         int j = start + g;
         for (int k = g; k < vocab; k += G, j += G) {
             const int e = j < vocab ? j : j - vocab;
             float d = 0.0f;
             if (!none) {
-                d = logit_gradient<ENT>(to_f32(row[e]), a.m, log_s, h, dlp, dh, inv_temperature);
-                if (e == action) d = fmaf(dlp, inv_temperature, d);
+                d = logit_gradient<ENT>(to_f32(row[e]), grad);
+                if (e == action) d += grad.dlp;
             }
             row[e] = from_f32<T>(d);
         }
@@ -453,7 +632,7 @@ static cudaError_t launch_small(const void* logits, RowMap lmap, const long long
                                 void* dlogits, cudaStream_t st)
 {
     int g = 1;
-    while (g < 32 && vocab > 32 * g) g *= 2;
+    while (vocab > 32 * g) g *= 2;
     const long long tile = kLpThreads / g;
     const size_t smem = static_cast<size_t>(tile) * vocab * sizeof(T) + 32;
     const int grid = static_cast<int>((rows + tile - 1) / tile);
@@ -463,10 +642,7 @@ static cudaError_t launch_small(const void* logits, RowMap lmap, const long long
         static_cast<T*>(dlogits))
     if (g == 1) PUFF_SMALL(1);
     else if (g == 2) PUFF_SMALL(2);
-    else if (g == 4) PUFF_SMALL(4);
-    else if (g == 8) PUFF_SMALL(8);
-    else if (g == 16) PUFF_SMALL(16);
-    else PUFF_SMALL(32);
+    else PUFF_SMALL(4);
 #undef PUFF_SMALL
     return cudaGetLastError();
 }
@@ -515,9 +691,12 @@ static cudaError_t launch_logprobs_backward(const void* logits, RowMap lmap, con
                                           dlogits, st);
     constexpr long long per_unit = 32LL * kLpUnitVecs * Vec16<T>::N;
     const long long units = (vocab + per_unit - 1) / per_unit;
-    const long long grid = (rows * units + kLpWarps - 1) / kLpWarps;
+    int warps_per_row = 1;
+    while (warps_per_row < kLpWarps && warps_per_row < units) warps_per_row *= 2;
+    const long long ctas_per_row = (units + kLpWarps - 1) / kLpWarps, rows_per_cta = kLpWarps / warps_per_row;
+    const long long grid = (rows + rows_per_cta - 1) / rows_per_cta * ctas_per_row;
     puff_logprobs_backward_kernel<T, ENT><<<static_cast<unsigned>(grid), kLpThreads, 0, st>>>(
-        static_cast<const T*>(logits), lmap, actions, amap, rows, vocab, units, inv_t,
+        static_cast<const T*>(logits), lmap, actions, amap, rows, vocab, warps_per_row, static_cast<unsigned>(ctas_per_row), inv_t,
         reinterpret_cast<const float2*>(row_stats), entropy, dlogprobs, dentropy, static_cast<T*>(dlogits));
     return cudaGetLastError();
 }
@@ -576,8 +755,8 @@ extern "C" int puff_policy_sm100_logprobs(const void* logits, int dtype, const l
     int sms = 0;
     rc = require_sm100(&sms);
     if (rc != PUFF_OK) return rc;
-    const RowMap lmap = {inner, logits_outer_stride, logits_inner_stride};
-    const RowMap amap = {inner, actions_outer_stride, actions_inner_stride};
+    const RowMap lmap = {inner, logits_outer_stride, logits_inner_stride, outer == 1};
+    const RowMap amap = {inner, actions_outer_stride, actions_inner_stride, outer == 1};
     const float inv_t = 1.0f / temperature;
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
 #define PUFF_RUN(T)                                                                                                        \
@@ -618,8 +797,8 @@ extern "C" int puff_policy_sm100_logprobs_backward(const void* logits, int dtype
     int sms = 0;
     rc = require_sm100(&sms);
     if (rc != PUFF_OK) return rc;
-    const RowMap lmap = {inner, logits_outer_stride, logits_inner_stride};
-    const RowMap amap = {inner, actions_outer_stride, actions_inner_stride};
+    const RowMap lmap = {inner, logits_outer_stride, logits_inner_stride, outer == 1};
+    const RowMap amap = {inner, actions_outer_stride, actions_inner_stride, outer == 1};
     const float inv_t = 1.0f / temperature;
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
 #define PUFF_RUN(T)                                                                                                       \
