@@ -57,6 +57,15 @@ template <typename T> T* ptr(const Tensor& t) { return t.defined() ? static_cast
 template <typename T> const T* ptr(const OptTensor& t) { return t.has_value() && t->defined() ? static_cast<const T*>(t->data_ptr()) : nullptr; }
 bool present(const OptTensor& t) { return t.has_value() && t->defined(); }
 OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+// In a backward pass that builds no graph the backward operators are called below autograd: above it they would pass
+// through the boxed kernel that refuses second derivatives.
+struct BelowUnlessGraph {
+    std::optional<at::AutoDispatchBelowADInplaceOrView> below;
+    BelowUnlessGraph()
+    {
+        if (!at::GradMode::is_enabled()) below.emplace();
+    }
+};
 cudaStream_t current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 // ---- log-probabilities ------------------------------------------------------------------------------------------
@@ -215,6 +224,7 @@ struct LogprobsNode : public torch::autograd::Function<LogprobsNode> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
+        const BelowUnlessGraph below;
         const auto saved = ctx->get_saved_variables();
         Tensor dlogits;
         if (grads[0].defined() || grads[1].defined()) {
@@ -382,6 +392,7 @@ struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
     {
         variable_list out(12);
         if (!grads[0].defined()) return out;
+        const BelowUnlessGraph below;
         const auto saved = ctx->get_saved_variables();
         const bool want_dentropy = ctx->saved_data["dentropy"].toBool();
         auto [dlp, dent] = loss_backward(saved[0], saved[1], saved[2], grads[0], optional(saved[3]),
@@ -537,6 +548,7 @@ struct RecurrenceNode : public torch::autograd::Function<RecurrenceNode> {
     {
         variable_list out(4);
         if (!grads[0].defined() && !grads[1].defined()) return out;
+        const BelowUnlessGraph below;
         const auto saved = ctx->get_saved_variables();
         const OptTensor dout = grads[0].defined() ? OptTensor(grads[0].contiguous()) : std::nullopt;
         const OptTensor dfinal = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
