@@ -8,7 +8,7 @@
 // sequences of their token means (w = 1 / (length sequences)) and the KL term.
 //
 // The forward pass writes the ratio and the per-token slope dloss/dlogprob / w; w needs the count of all tokens, so
-// the backward pass multiplies by it.  Which side of a clip border a ratio is on is decided in 64 bits, as
+// the backward pass multiplies by it.  Which side of a clip border a ratio is on is decided in 48 bits, as
 // logprob - old_logprob against log(1 - clip_low) and log(1 + clip_high).
 #include <cuda_runtime.h>
 #include <math.h>
@@ -20,6 +20,7 @@
 namespace puff {
 
 constexpr int kLossThreads = 256;
+constexpr int kLossWarps = kLossThreads / 32;
 constexpr int kLossMaxBlocks = 148 * 4;
 constexpr int kLossSums = 8;   // policy, kl, entropy, -d, e^d - 1 - d, clipped, tokens, sequences
 
@@ -34,79 +35,149 @@ struct LossArgs {
     float* slope;
     float* row_scale;
     long long rows, steps;
-    int per_row;   // one advantage per row
     float clip_low_value, clip_high_value;
-    double log_low, log_high;
+    float log_low, log_low_rest, log_high, log_high_rest;   // log(1 - clip_low), log(1 + clip_high), 48 bits each
     float kl_coef;
 };
 
-// e^x - 1 - x.  For |x| < 1 by its Taylor series x^2 (1/2! + x/3! + ...), the difference would cancel there;
-// em1 receives e^x - 1.
-__device__ __forceinline__ float exp_excess(float x, float ex, float* em1)
+// e^x - 1 - x for |x| <= 1 as x^2 (1/2 + x Q(x)): the difference itself would cancel.  Q is the polynomial of degree 6
+// through the Chebyshev nodes of ((e^x - 1 - x) / x^2 - 1/2) / x on [-1, 1]; the result is good to 3 half steps of fp32.
+__device__ __forceinline__ float exp_excess(float x)
 {
-    if (fabsf(x) < 1.0f) {
-        float p = 1.0f / 6227020800.0f;              // 1/13!
-        p = fmaf(p, x, 1.0f / 479001600.0f);
-        p = fmaf(p, x, 1.0f / 39916800.0f);
-        p = fmaf(p, x, 1.0f / 3628800.0f);
-        p = fmaf(p, x, 1.0f / 362880.0f);
-        p = fmaf(p, x, 1.0f / 40320.0f);
-        p = fmaf(p, x, 1.0f / 5040.0f);
-        p = fmaf(p, x, 1.0f / 720.0f);
-        p = fmaf(p, x, 1.0f / 120.0f);
-        p = fmaf(p, x, 1.0f / 24.0f);
-        p = fmaf(p, x, 1.0f / 6.0f);
-        p = fmaf(p, x, 0.5f);
-        const float k = x * x * p;
-        *em1 = x + k;
-        return k;
-    }
-    *em1 = ex - 1.0f;
-    return *em1 - x;
+    float p = 2.799926278385101e-06f;
+    p = fmaf(p, x, 2.5288434699177742e-05f);
+    p = fmaf(p, x, 1.9839055312331766e-04f);
+    p = fmaf(p, x, 1.3886447995901108e-03f);
+    p = fmaf(p, x, 8.333336561918259e-03f);
+    p = fmaf(p, x, 4.166669771075249e-02f);
+    p = fmaf(p, x, 0.1666666716337204f);
+    p = fmaf(p, x, 0.5f);
+    return x * x * p;
 }
-
-// e^(a - b) with the difference's rounding carried along; *diff64 and *diff receive a - b
-__device__ __forceinline__ float exp_of_difference(float a, float b, double* diff64, float* diff)
+// the rounding error of d = a - b, exactly (Knuth's two-sum).  fp32 pairs because conversions to fp64 and back bounded
+// the kernel: 415 us for 131072 x 256 tokens.
+__device__ __forceinline__ float difference_rest(float a, float b, float d)
 {
-    const double d = static_cast<double>(a) - static_cast<double>(b);
-    const float hi = static_cast<float>(d);
-    const float e = expf(hi);
-    *diff64 = d;
-    *diff = hi;
-    return fabsf(hi) < 80.0f ? fmaf(e, static_cast<float>(d - hi), e) : e;
+    const float back = __fsub_rn(d, a);
+    return __fsub_rn(__fsub_rn(a, __fsub_rn(d, back)), __fadd_rn(b, back));
 }
 
 struct TokenLoss {
-    float policy, kl, neg_d, excess, clipped, ratio, slope;
+    float policy, kl, excess, ratio, slope, d;
+    bool clipped;
 };
 __device__ __forceinline__ TokenLoss token_loss(const LossArgs& p, float lp, float old, float adv, float ref)
 {
     TokenLoss t;
-    double d64;
-    float d, em1;
-    t.ratio = exp_of_difference(lp, old, &d64, &d);
-    const bool above = d64 > p.log_high, below = d64 < p.log_low;
+    const float d = __fsub_rn(lp, old);
+    bool above = d > p.log_high, below = d < p.log_low;
+    t.d = d;
+    // the usual token: no exponential, e^d = 1 + (d + (e^d - 1 - d))
+    t.excess = exp_excess(d);
+    t.ratio = 1.0f + (d + t.excess);
+    if (!(fabsf(d) < 0.5f) || d == p.log_high || d == p.log_low) {
+        const float rest = difference_rest(lp, old, d);
+        above = above || (d == p.log_high && rest > p.log_high_rest);
+        below = below || (d == p.log_low && rest < p.log_low_rest);
+        const float e = expf(d);
+        // beyond 80 the exponential is 0, infinite, or the rest does not matter
+        t.ratio = fabsf(d) < 80.0f ? fmaf(e, rest, e) : e;
+        if (!(fabsf(d) < 1.0f)) t.excess = (t.ratio - 1.0f) - d;
+    }
     const bool cut = (above && adv > 0.0f) || (below && adv < 0.0f);
     t.policy = -adv * (cut ? (above ? p.clip_high_value : p.clip_low_value) : t.ratio);
     t.slope = cut ? 0.0f : t.policy;
-    t.neg_d = -d;
-    t.excess = exp_excess(d, t.ratio, &em1);
-    t.clipped = above || below ? 1.0f : 0.0f;
+    t.clipped = above || below;
     t.kl = 0.0f;
     if (p.ref_logprobs != nullptr) {
-        double q64;
-        float q;
-        const float eq = exp_of_difference(ref, lp, &q64, &q);
-        t.kl = exp_excess(q, eq, &em1);
+        const float q = __fsub_rn(ref, lp);
+        t.kl = exp_excess(q);
+        float em1 = q + t.kl;
+        if (!(fabsf(q) < 1.0f)) {
+            const float e = expf(q);
+            em1 = (fabsf(q) < 80.0f ? fmaf(e, difference_rest(ref, lp, q), e) : e) - 1.0f;
+            t.kl = em1 - q;
+        }
         t.slope = fmaf(-p.kl_coef, em1, t.slope);
     }
     return t;
 }
 
-// adds the sums of all threads of the CTA; thread 0 writes them
-__device__ __forceinline__ void write_partial(double (&v)[kLossSums], double* partial)
+// VEC adjacent values
+template <int VEC> struct Pack;
+template <> struct Pack<1> {
+    static __device__ __forceinline__ void load(const float* p, float* f) { f[0] = __ldg(p); }
+    static __device__ __forceinline__ void store(float* p, const float* f) { *p = f[0]; }
+    static __device__ __forceinline__ unsigned mask(const unsigned char* p) { return __ldg(p) != 0 ? 1u : 0u; }
+};
+template <> struct Pack<4> {
+    static __device__ __forceinline__ void load(const float* p, float* f)
+    {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+        f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    }
+    static __device__ __forceinline__ void store(float* p, const float* f) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+    static __device__ __forceinline__ unsigned mask(const unsigned char* p)
+    {
+        const uchar4 v = __ldg(reinterpret_cast<const uchar4*>(p));
+        return (v.x ? 1u : 0u) | (v.y ? 2u : 0u) | (v.z ? 4u : 0u) | (v.w ? 8u : 0u);
+    }
+};
+
+// Sums over a few tokens in fp32, joined in fp64; numbers of tokens are whole
+struct LossSums {
+    float policy, kl, entropy, neg_d, excess;
+};
+struct LossTotals {
+    double policy, kl, entropy, neg_d, excess;
+    int clipped, tokens, rows;
+};
+// tokens i ... i + VEC - 1, advantages from a ...: reads, writes ratio and slope, adds to the sums
+template <int VEC, bool ONE_ADVANTAGE>
+__device__ __forceinline__ void add_tokens(const LossArgs& p, long long i, long long a, LossSums& sums, int& clipped, int& tokens)
 {
-    __shared__ double s_part[kLossThreads / 32][kLossSums];
+    float lp[VEC], old[VEC], adv[VEC], ref[VEC], ent[VEC], ratio[VEC], slope[VEC];
+    Pack<VEC>::load(p.logprobs + i, lp);
+    Pack<VEC>::load(p.old_logprobs + i, old);
+    if (ONE_ADVANTAGE) {
+        adv[0] = __ldg(p.advantages + a);
+#pragma unroll
+        for (int v = 1; v < VEC; ++v) adv[v] = adv[0];
+    } else {
+        Pack<VEC>::load(p.advantages + a, adv);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) ref[v] = ent[v] = 0.0f;
+    if (p.ref_logprobs != nullptr) Pack<VEC>::load(p.ref_logprobs + i, ref);
+    if (p.entropy != nullptr) Pack<VEC>::load(p.entropy + i, ent);
+    const unsigned keep = p.mask != nullptr ? Pack<VEC>::mask(p.mask + i) : (1u << VEC) - 1u;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        ratio[v] = 1.0f;
+        slope[v] = 0.0f;
+        if (keep >> v & 1u) {
+            const TokenLoss t = token_loss(p, lp[v], old[v], adv[v], ref[v]);
+            ratio[v] = t.ratio;
+            slope[v] = t.slope;
+            sums.policy += t.policy;
+            sums.kl += t.kl;
+            sums.entropy += ent[v];
+            sums.neg_d -= t.d;
+            sums.excess += t.excess;
+            clipped += t.clipped ? 1 : 0;
+            ++tokens;
+        }
+    }
+    Pack<VEC>::store(p.ratio + i, ratio);
+    if (p.slope != nullptr) Pack<VEC>::store(p.slope + i, slope);
+}
+
+// adds the sums of all threads of the CTA; thread 0 writes them
+__device__ __forceinline__ void write_partial(const LossTotals& t, double* partial)
+{
+    double v[kLossSums] = {t.policy, t.kl, t.entropy, t.neg_d, t.excess, static_cast<double>(t.clipped),
+                           static_cast<double>(t.tokens), static_cast<double>(t.rows)};
+    __shared__ double s_part[32][kLossSums];
 #pragma unroll
     for (int k = 0; k < kLossSums; ++k)
 #pragma unroll
@@ -116,57 +187,85 @@ __device__ __forceinline__ void write_partial(double (&v)[kLossSums], double* pa
         for (int k = 0; k < kLossSums; ++k) s_part[threadIdx.x >> 5][k] = v[k];
     __syncthreads();
     if (threadIdx.x < kLossSums) {
-        double t = 0.0;
-        for (int w = 0; w < kLossThreads / 32; ++w) t += s_part[w][threadIdx.x];
-        partial[blockIdx.x * kLossSums + threadIdx.x] = t;
+        double sum = 0.0;
+        for (int w = 0; w < static_cast<int>(blockDim.x / 32); ++w) sum += s_part[w][threadIdx.x];
+        partial[threadIdx.x * static_cast<long long>(gridDim.x) + blockIdx.x] = sum;
     }
 }
 
-// One warp per row.  SEQ: the row's policy, kl and entropy sums are divided by its length.
-template <bool SEQ>
-__global__ void __launch_bounds__(kLossThreads)
+// Means over tokens, an advantage each: rows do not matter.
+template <int VEC>
+__global__ void __launch_bounds__(kLossThreads, 4)
+puff_policy_loss_kernel(LossArgs p, double* __restrict__ partial)
+{
+    LossTotals total = {};
+    const long long units = p.rows * p.steps / VEC, stride = static_cast<long long>(gridDim.x) * kLossThreads;
+    for (long long u = blockIdx.x * static_cast<long long>(kLossThreads) + threadIdx.x; u < units; u += stride) {
+        LossSums sums = {};
+        add_tokens<VEC, false>(p, u * VEC, u * VEC, sums, total.clipped, total.tokens);
+        total.policy += sums.policy;
+        total.kl += sums.kl;
+        total.entropy += sums.entropy;
+        total.neg_d += sums.neg_d;
+        total.excess += sums.excess;
+    }
+    write_partial(total, partial);
+}
+
+// Rows that matter: one advantage each, or SEQ, a mean each.  TEAM threads a row, rows side by side in a warp where they
+// are short, one a CTA (TEAM 256) where they are long and few.  SEQ: a thread's share of the row's policy, kl and entropy
+// sums is divided by the row's length.
+template <int VEC, int TEAM, bool SEQ, bool ONE_ADVANTAGE>
+__global__ void __launch_bounds__(TEAM > kLossThreads ? TEAM : kLossThreads, TEAM > kLossThreads ? 1 : 4)
 puff_policy_loss_rows_kernel(LossArgs p, double* __restrict__ partial)
 {
-    const int lane = threadIdx.x & 31;
-    const long long stride = static_cast<long long>(gridDim.x) * (kLossThreads / 32);
-    double total[kLossSums] = {};
-    for (long long r = blockIdx.x * static_cast<long long>(kLossThreads / 32) + (threadIdx.x >> 5); r < p.rows; r += stride) {
-        double v[kLossSums] = {};
-        for (long long c = lane; c < p.steps; c += 32) {
-            const long long i = r * p.steps + c;
-            const bool keep = p.mask == nullptr || p.mask[i] != 0;
-            float ratio = 1.0f, slope = 0.0f;
-            if (keep) {
-                const TokenLoss t = token_loss(p, p.logprobs[i], p.old_logprobs[i], p.advantages[p.per_row ? r : i],
-                                               p.ref_logprobs != nullptr ? p.ref_logprobs[i] : 0.0f);
-                ratio = t.ratio;
-                slope = t.slope;
-                v[0] += t.policy;
-                v[1] += t.kl;
-                if (p.entropy != nullptr) v[2] += p.entropy[i];
-                v[3] += t.neg_d;
-                v[4] += t.excess;
-                v[5] += t.clipped;
-                v[6] += 1.0;
+    constexpr int kThreads = TEAM > kLossThreads ? TEAM : kLossThreads;
+    constexpr int kTeams = kThreads / TEAM;
+    __shared__ int s_length[kThreads / 32];
+    const int member = threadIdx.x % TEAM;
+    LossTotals total = {};
+    const long long units = p.steps / VEC, stride = static_cast<long long>(gridDim.x) * kTeams;
+    const long long rounds = (p.rows + stride - 1) / stride;
+    long long r = blockIdx.x * static_cast<long long>(kTeams) + threadIdx.x / TEAM;
+    for (long long k = 0; k < rounds; ++k, r += stride) {      // all threads go round alike: they meet below
+        double policy = 0.0, kl = 0.0, entropy = 0.0;      // of the row, for SEQ
+        int length = 0;                                    // of this thread: at most steps / TEAM + VEC
+        if (r < p.rows)
+            for (long long u = member; u < units; u += TEAM) {
+                LossSums sums = {};
+                const long long i = r * p.steps + u * VEC;
+                add_tokens<VEC, ONE_ADVANTAGE>(p, i, ONE_ADVANTAGE ? r : i, sums, total.clipped, length);
+                policy += sums.policy;
+                kl += sums.kl;
+                entropy += sums.entropy;
+                total.neg_d += sums.neg_d;
+                total.excess += sums.excess;
             }
-            p.ratio[i] = ratio;
-            if (p.slope != nullptr) p.slope[i] = slope;
-        }
+        total.tokens += length;
         if (SEQ) {
-            double length = v[6];
+            long long whole;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) length += __shfl_xor_sync(0xffffffffu, length, o);
-            const double scale = length > 0.0 ? 1.0 / length : 0.0;
-            v[0] *= scale;
-            v[1] *= scale;
-            v[2] *= scale;
-            if (lane == 0) {
-                v[7] = length > 0.0 ? 1.0 : 0.0;
+            for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1) length += __shfl_xor_sync(0xffffffffu, length, o);
+            whole = length;
+            if (TEAM > 32) {
+                __syncthreads();
+                if ((threadIdx.x & 31) == 0) s_length[threadIdx.x >> 5] = length;
+                __syncthreads();
+                whole = 0;
+                for (int w = 0; w < kThreads / 32; ++w) whole += s_length[w];
+            }
+            const double scale = whole > 0 ? 1.0 / static_cast<double>(whole) : 0.0;
+            policy *= scale;
+            kl *= scale;
+            entropy *= scale;
+            if (member == 0 && r < p.rows) {
+                total.rows += whole > 0 ? 1 : 0;
                 if (p.row_scale != nullptr) p.row_scale[r] = static_cast<float>(scale);
             }
         }
-#pragma unroll
-        for (int k = 0; k < kLossSums; ++k) total[k] += v[k];
+        total.policy += policy;
+        total.kl += kl;
+        total.entropy += entropy;
     }
     write_partial(total, partial);
 }
@@ -181,7 +280,8 @@ puff_policy_loss_final_kernel(const double* __restrict__ partial, int n_partial,
     const int k = threadIdx.x >> 5, lane = threadIdx.x & 31;   // one warp per sum
     pdl_wait();
     double t = 0.0;
-    for (int i = lane; i < n_partial; i += 32) t += partial[i * kLossSums + k];
+#pragma unroll 4
+    for (int i = lane; i < n_partial; i += 32) t += partial[k * n_partial + i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (lane == 0) s_sum[k] = t;
@@ -203,6 +303,8 @@ puff_policy_loss_final_kernel(const double* __restrict__ partial, int n_partial,
     }
 }
 
+// VEC 4 with row_scale: four adjacent tokens are of one row (steps divisible by four)
+template <int VEC>
 __global__ void __launch_bounds__(kLossThreads)
 puff_policy_loss_backward_kernel(const float* __restrict__ slope, const float* __restrict__ row_scale,
                                  const float* __restrict__ weight, const float* __restrict__ dloss,
@@ -210,19 +312,59 @@ puff_policy_loss_backward_kernel(const float* __restrict__ slope, const float* _
                                  float* __restrict__ dentropy, long long rows, long long steps)
 {
     const float w = weight[0] * dloss[0];
-    const long long n = rows * steps, stride = static_cast<long long>(gridDim.x) * kLossThreads;
-    for (long long i = blockIdx.x * static_cast<long long>(kLossThreads) + threadIdx.x; i < n; i += stride) {
-        const bool keep = mask == nullptr || mask[i] != 0;
-        const float wi = row_scale != nullptr ? w * row_scale[i / steps] : w;
-        if (dlogprobs != nullptr) dlogprobs[i] = keep ? slope[i] * wi : 0.0f;
-        if (dentropy != nullptr) dentropy[i] = keep ? -ent_coef * wi : 0.0f;
+    const long long units = rows * steps / VEC, stride = static_cast<long long>(gridDim.x) * kLossThreads;
+    for (long long u = blockIdx.x * static_cast<long long>(kLossThreads) + threadIdx.x; u < units; u += stride) {
+        const long long i = u * VEC;
+        float s[VEC], g[VEC], h[VEC];
+        if (dlogprobs != nullptr) Pack<VEC>::load(slope + i, s);
+        const unsigned keep = mask != nullptr ? Pack<VEC>::mask(mask + i) : (1u << VEC) - 1u;
+        float wi = w;
+        if (row_scale != nullptr)
+            wi *= __ldg(row_scale + (((i | steps) >> 32) == 0 ? static_cast<unsigned>(i) / static_cast<unsigned>(steps) : i / steps));
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const bool k = keep >> v & 1u;
+            g[v] = k ? s[v] * wi : 0.0f;
+            h[v] = k ? -ent_coef * wi : 0.0f;
+        }
+        if (dlogprobs != nullptr) Pack<VEC>::store(dlogprobs + i, g);
+        if (dentropy != nullptr) Pack<VEC>::store(dentropy + i, h);
     }
 }
 
-static int loss_blocks(long long rows, long long)
+static int capped(long long blocks, int most) { return static_cast<int>(blocks < 1 ? 1 : blocks > most ? most : blocks); }
+
+template <int VEC, int TEAM, bool SEQ>
+static int launch_rows(const LossArgs& p, bool one_advantage, double* partial, cudaStream_t st)
 {
-    long long b = (rows + kLossThreads / 32 - 1) / (kLossThreads / 32);
-    return static_cast<int>(b < 1 ? 1 : b > kLossMaxBlocks ? kLossMaxBlocks : b);
+    constexpr int threads = TEAM > kLossThreads ? TEAM : kLossThreads;
+    const int blocks = capped((p.rows + threads / TEAM - 1) / (threads / TEAM), kLossMaxBlocks);
+    if (one_advantage) puff_policy_loss_rows_kernel<VEC, TEAM, SEQ, true><<<blocks, threads, 0, st>>>(p, partial);
+    else puff_policy_loss_rows_kernel<VEC, TEAM, SEQ, false><<<blocks, threads, 0, st>>>(p, partial);
+    return blocks;
+}
+template <int VEC, bool SEQ>
+static int launch_rows(const LossArgs& p, bool one_advantage, double* partial, cudaStream_t st)
+{
+    // as many threads a row as it has units to read, up to a warp; a CTA where a warp a row would leave SMs idle, and a
+    // large one where even a CTA a row would (100 rows of 100001: 256 threads 473 us)
+    const long long units = p.steps / VEC;
+    if (units >= 2048 && p.rows < 148 * 2) return launch_rows<VEC, 1024, SEQ>(p, one_advantage, partial, st);
+    if (units >= 256 && p.rows < 148 * kLossWarps) return launch_rows<VEC, 256, SEQ>(p, one_advantage, partial, st);
+    if (units >= 32) return launch_rows<VEC, 32, SEQ>(p, one_advantage, partial, st);
+    if (units >= 8) return launch_rows<VEC, 8, SEQ>(p, one_advantage, partial, st);
+    if (units >= 2) return launch_rows<VEC, 2, SEQ>(p, one_advantage, partial, st);
+    return launch_rows<VEC, 1, SEQ>(p, one_advantage, partial, st);
+}
+// the number of partial sums written
+static int launch_loss(const LossArgs& p, bool sequence, bool one_advantage, bool vec, double* partial, cudaStream_t st)
+{
+    if (sequence) return vec ? launch_rows<4, true>(p, one_advantage, partial, st) : launch_rows<1, true>(p, one_advantage, partial, st);
+    if (one_advantage && p.rows > 0) return vec ? launch_rows<4, false>(p, true, partial, st) : launch_rows<1, false>(p, true, partial, st);
+    const int blocks = capped((p.rows * p.steps / (vec ? 4 : 1) + kLossThreads - 1) / kLossThreads, kLossMaxBlocks);
+    if (vec) puff_policy_loss_kernel<4><<<blocks, kLossThreads, 0, st>>>(p, partial);
+    else puff_policy_loss_kernel<1><<<blocks, kLossThreads, 0, st>>>(p, partial);
+    return blocks;
 }
 }  // namespace puff
 
@@ -282,19 +424,22 @@ extern "C" int puff_policy_sm100_loss(const float* logprobs, const float* old_lo
     p.row_scale = row_scale;
     p.rows = n > 0 ? rows : 0;
     p.steps = steps;
-    p.per_row = advantage_per_row != 0;
     p.clip_low_value = static_cast<float>(1.0 - clip_low);
     p.clip_high_value = static_cast<float>(1.0 + clip_high);
-    p.log_low = clip_low < 1.0 ? log1p(-clip_low) : -HUGE_VAL;
-    p.log_high = log1p(clip_high);
+    const double low = clip_low < 1.0 ? log1p(-clip_low) : -HUGE_VAL, high = log1p(clip_high);
+    p.log_low = static_cast<float>(low);
+    p.log_low_rest = clip_low < 1.0 ? static_cast<float>(low - p.log_low) : 0.0f;
+    p.log_high = static_cast<float>(high);
+    p.log_high_rest = high < HUGE_VAL ? static_cast<float>(high - p.log_high) : 0.0f;
     p.kl_coef = kl_coef;
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-    const int blocks = loss_blocks(rows, steps);
+    // four tokens at a time where every array is aligned for it (and, where rows matter, so are they)
+    const bool rows_matter = reduction == PUFF_MEAN_SEQUENCES || advantage_per_row;
+    bool vec = (rows_matter ? steps : n) % 4 == 0 && !misaligned(mask, 4);
+    for (int i = 0; i < 5; ++i) vec = vec && ((i == 2 && advantage_per_row) || !misaligned(in[i], 16));
+    vec = vec && !misaligned(ratio, 16) && !misaligned(slope, 16);
     double* partial = static_cast<double*>(scratch);
-    if (reduction == PUFF_MEAN_SEQUENCES)
-        puff_policy_loss_rows_kernel<true><<<blocks, kLossThreads, 0, st>>>(p, partial);
-    else
-        puff_policy_loss_rows_kernel<false><<<blocks, kLossThreads, 0, st>>>(p, partial);
+    const int blocks = launch_loss(p, reduction == PUFF_MEAN_SEQUENCES, advantage_per_row != 0, vec, partial, st);
     count_launch();
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -327,10 +472,16 @@ extern "C" int puff_policy_sm100_loss_backward(const float* slope, const float* 
     int sms = 0;
     const int rc = require_sm100(&sms);
     if (rc != PUFF_OK) return rc;
-    long long blocks = (n + kLossThreads - 1) / kLossThreads;
-    if (blocks > 8LL * sms) blocks = 8LL * sms;
-    puff_policy_loss_backward_kernel<<<static_cast<int>(blocks), kLossThreads, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
-        slope, row_scale, weight, dloss, mask, ent_coef, dlogprobs, dentropy, rows, steps);
+    const bool vec = (row_scale != nullptr ? steps : n) % 4 == 0 && !misaligned(mask, 4) && !misaligned(slope, 16) &&
+                     !misaligned(dlogprobs, 16) && !misaligned(dentropy, 16);
+    cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    const int blocks = capped((n / (vec ? 4 : 1) + kLossThreads - 1) / kLossThreads, 8 * sms);
+    if (vec)
+        puff_policy_loss_backward_kernel<4><<<blocks, kLossThreads, 0, st>>>(slope, row_scale, weight, dloss, mask, ent_coef,
+                                                                             dlogprobs, dentropy, rows, steps);
+    else
+        puff_policy_loss_backward_kernel<1><<<blocks, kLossThreads, 0, st>>>(slope, row_scale, weight, dloss, mask, ent_coef,
+                                                                             dlogprobs, dentropy, rows, steps);
     count_launch();
     return static_cast<int>(cudaGetLastError());
 }
