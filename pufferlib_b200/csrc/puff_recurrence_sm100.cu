@@ -48,20 +48,73 @@ __device__ __forceinline__ bool is_reset(const RecArgs& p, long long i)
 
 // keep = sigmoid(g) and take = 1 - keep = sigmoid(-g).  The smaller of the two is e / (1 + e) with e = e^-|g|, good to
 // a few ulp however small; the larger is 1 minus it, so that the two add up to 1 and the state stays a weighted mean.
-// One register holds both: the smaller one, with the sign of g.
-__device__ __forceinline__ float gate_code(float g)
+// One register, the code, holds both: the smaller one with the sign of g.
+__device__ __forceinline__ float rcp_approx(float x)
 {
-    const float e = exp2_approx(-fabsf(g) * kLog2e);
-    return copysignf(__fdividef(e, 1.0f + e), g);
-}
-__device__ __forceinline__ void gate_pair(float code, float& keep, float& take)
-{
-    const float small = fabsf(code), large = 1.0f - small;
-    const bool negative = __float_as_int(code) < 0;
-    keep = negative ? small : large;
-    take = negative ? large : small;
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 constexpr float kHold = 0.0f;      // the code of a gate that holds the state: steps past the end
+
+// Arithmetic on the VEC channels of a lane, in packed pairs where there are two
+template <int VEC>
+__device__ __forceinline__ void v_fma(float (&d)[VEC], const float (&a)[VEC], const float (&b)[VEC], const float (&c)[VEC])
+{
+    if constexpr (VEC == 2) {
+        const float2 r = __ffma2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]), make_float2(c[0], c[1]));
+        d[0] = r.x, d[1] = r.y;
+    } else {
+        d[0] = fmaf(a[0], b[0], c[0]);
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void v_mul(float (&d)[VEC], const float (&a)[VEC], const float (&b)[VEC])
+{
+    if constexpr (VEC == 2) {
+        const float2 r = __fmul2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]));
+        d[0] = r.x, d[1] = r.y;
+    } else {
+        d[0] = a[0] * b[0];
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void v_add(float (&d)[VEC], const float (&a)[VEC], const float (&b)[VEC])
+{
+    if constexpr (VEC == 2) {
+        const float2 r = __fadd2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]));
+        d[0] = r.x, d[1] = r.y;
+    } else {
+        d[0] = a[0] + b[0];
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void gate_codes(const float (&g)[VEC], float (&code)[VEC])
+{
+    float e[VEC], one[VEC], d[VEC], r[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        e[v] = exp2_approx(fabsf(g[v]) * -kLog2e);
+        one[v] = 1.0f;
+    }
+    v_add(d, e, one);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) r[v] = rcp_approx(d[v]);
+    v_mul(d, e, r);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) code[v] = copysignf(d[v], g[v]);
+}
+template <int VEC>
+__device__ __forceinline__ void gate_pairs(const float (&code)[VEC], float (&keep)[VEC], float (&take)[VEC])
+{
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        const float small = fabsf(code[v]), large = 1.0f - small;
+        const bool negative = __float_as_int(code[v]) < 0;
+        keep[v] = negative ? small : large;
+        take[v] = negative ? large : small;
+    }
+}
 
 // h -> A h + B over a span; A < 0: the span holds a reset, h does not matter
 __device__ __forceinline__ float apply_pair(float2 ab, float h) { return ab.x < 0.0f ? ab.y : fmaf(ab.x, h, ab.y); }
@@ -105,6 +158,11 @@ template <> __device__ __forceinline__ __nv_bfloat16 zero_raw<__nv_bfloat16>() {
 template <> __device__ __forceinline__ __half2 zero_raw<__half2>() { return __float2half2_rn(0.0f); }
 template <> __device__ __forceinline__ __nv_bfloat162 zero_raw<__nv_bfloat162>() { return __float2bfloat162_rn(0.0f); }
 
+__device__ __forceinline__ long long quotient(long long a, long long b)
+{
+    return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : a / b;
+}
+
 // Where this thread's warp stands in the plan.  FLAT: the lanes of a warp are adjacent (batch, channel) pairs of any
 // rows, for channels too few to fill a warp; otherwise they are adjacent channels of one row.
 struct RecPlace {
@@ -113,6 +171,11 @@ struct RecPlace {
     int split;
     long long b, c, index;     // index: b * channels + c
     long long t_begin, t_end;
+    __device__ __forceinline__ int steps_at(long long t0) const
+    {
+        const long long left = t_end - t0;
+        return left < 0 ? 0 : left < kRecTile ? static_cast<int>(left) : kRecTile;
+    }
 };
 template <int VEC, bool FLAT>
 __device__ __forceinline__ RecPlace rec_place(const RecArgs& p, const RecPlan& plan)
@@ -123,16 +186,16 @@ __device__ __forceinline__ RecPlace rec_place(const RecArgs& p, const RecPlan& p
     q.group = warp / plan.warps;
     q.w = warp - q.group * plan.warps;
     const long long unit = blockIdx.x * static_cast<long long>(kRecWarps / plan.warps) + q.group;
-    const long long block = unit % plan.lane_blocks;
-    q.split = static_cast<int>(unit / plan.lane_blocks);
+    q.split = plan.splits == 1 && unit < plan.lane_blocks ? 0 : static_cast<int>(quotient(unit, plan.lane_blocks));
+    const long long block = unit - q.split * plan.lane_blocks;
     q.unit = q.split < plan.splits;
     if (FLAT) {
         q.index = block * 32 + q.lane;
         q.ok = q.index < p.batch * p.channels;
-        q.b = q.ok ? q.index / p.channels : 0;
+        q.b = q.ok ? quotient(q.index, p.channels) : 0;
         q.c = q.ok ? q.index - q.b * p.channels : 0;
     } else {
-        q.b = block / plan.blocks_per_row;
+        q.b = quotient(block, plan.blocks_per_row);
         q.c = (block - q.b * plan.blocks_per_row) * (32 * VEC) + q.lane * VEC;
         q.ok = q.c < p.channels;
         q.index = q.b * p.channels + q.c;
@@ -151,19 +214,28 @@ __device__ __forceinline__ unsigned reset_mask(const RecArgs& p, const RecPlace&
     if (!FLAT) return __ballot_sync(0xffffffffu, q.lane < n && is_reset(p, at + q.lane));
     unsigned m = 0;
     if (q.ok)
+#pragma unroll 4
         for (int j = 0; j < n; ++j) m |= is_reset(p, at + j) ? 1u << j : 0u;
     return m;
 }
 template <typename Raw, int VEC>
-__device__ __forceinline__ void load_tile(Raw* raw, const void* base, long long at, long long step_stride, int n, bool ok)
+__device__ __forceinline__ void load_tile(Raw (&raw)[kRecTile], const void* base, long long at, long long step_stride, int n, bool ok)
 {
     constexpr long long size = sizeof(Raw) / VEC;
     const char* ptr = static_cast<const char*>(base) + at * size;
+    const long long bytes = step_stride * size;
+    if (n == kRecTile) {
 #pragma unroll
-    for (int j = 0; j < kRecTile; ++j) {
-        raw[j] = zero_raw<Raw>();
-        if (ok && j < n) raw[j] = __ldg(reinterpret_cast<const Raw*>(ptr));
-        ptr += step_stride * size;
+        for (int j = 0; j < kRecTile; ++j, ptr += bytes) {
+            raw[j] = zero_raw<Raw>();
+            if (ok) raw[j] = __ldg(reinterpret_cast<const Raw*>(ptr));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kRecTile; ++j, ptr += bytes) {
+            raw[j] = zero_raw<Raw>();
+            if (ok && j < n) raw[j] = __ldg(reinterpret_cast<const Raw*>(ptr));
+        }
     }
 }
 __device__ __forceinline__ void group_barrier(int group, int warps)
@@ -171,17 +243,112 @@ __device__ __forceinline__ void group_barrier(int group, int warps)
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
 }
 
-// Forward.  SUMMARY: only the pairs of the ranges.  saved (nullable): the state before steps 0, 16, 32, ... as
-// [batch, ceil(steps / 16), channels].
-template <typename T, int VEC, bool FLAT, bool SUMMARY>
+// ---- what a warp does with a tile in registers.  PLAIN: sixteen steps, none a reset (for any lane of the warp).
+template <typename L, int VEC, bool PLAIN>
+__device__ __forceinline__ void tile_gates(const typename L::Raw& raw_g, const typename L::Raw& raw_x, bool there, float (&keep)[VEC],
+                                           float (&fresh)[VEC])
+{
+    float g[VEC], x[VEC], code[VEC], take[VEC];
+    L::get(raw_g, g);
+    L::get(raw_x, x);
+    gate_codes(g, code);
+    if (!PLAIN && !there)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) code[v] = kHold;
+    gate_pairs(code, keep, take);
+    v_mul(fresh, take, x);
+}
+template <int VEC, bool PLAIN>
+__device__ __forceinline__ void advance(float (&h)[VEC], const float (&keep)[VEC], const float (&fresh)[VEC], bool reset)
+{
+    v_fma(h, keep, h, fresh);
+    if (!PLAIN && reset)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = fresh[v];
+}
+// one pass: every step's state follows from the one before it
+template <typename T, int VEC, bool PLAIN>
+__device__ __forceinline__ void forward_stream(const typename Lane<T, VEC>::Raw (&raw_g)[kRecTile],
+                                               const typename Lane<T, VEC>::Raw (&raw_x)[kRecTile], unsigned cut, int n,
+                                               float (&h)[VEC], T* out, long long stride, bool ok)
+{
+    using L = Lane<T, VEC>;
+#pragma unroll
+    for (int j = 0; j < kRecTile; ++j, out += stride) {
+        float keep[VEC], fresh[VEC];
+        tile_gates<L, VEC, PLAIN>(raw_g[j], raw_x[j], j < n, keep, fresh);
+        advance<VEC, PLAIN>(h, keep, fresh, (cut >> j) & 1u);
+        if (ok && (PLAIN || j < n)) *reinterpret_cast<typename L::Raw*>(out) = L::put(h);
+    }
+}
+// two passes: the tile's pair (a, b), then its states once the one before it is known
+template <typename T, int VEC, bool PLAIN>
+__device__ __forceinline__ void forward_pair(const typename Lane<T, VEC>::Raw (&raw_g)[kRecTile],
+                                             const typename Lane<T, VEC>::Raw (&raw_x)[kRecTile], unsigned cut, int n,
+                                             float (&keep)[kRecTile][VEC], float (&fresh)[kRecTile][VEC], float (&a)[VEC], float (&b)[VEC])
+{
+#pragma unroll
+    for (int j = 0; j < kRecTile; ++j) {
+        tile_gates<Lane<T, VEC>, VEC, PLAIN>(raw_g[j], raw_x[j], j < n, keep[j], fresh[j]);
+        if (j == 0) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                a[v] = keep[0][v];
+                b[v] = fresh[0][v];
+            }
+        } else {
+            advance<VEC, PLAIN>(b, keep[j], fresh[j], (cut >> j) & 1u);
+            v_mul(a, a, keep[j]);
+        }
+    }
+}
+template <typename T, int VEC, bool PLAIN>
+__device__ __forceinline__ void forward_states(const float (&keep)[kRecTile][VEC], const float (&fresh)[kRecTile][VEC], unsigned cut,
+                                               int n, float (&h)[VEC], T* out, long long stride, bool ok)
+{
+    using L = Lane<T, VEC>;
+#pragma unroll
+    for (int j = 0; j < kRecTile; ++j, out += stride) {
+        advance<VEC, PLAIN>(h, keep[j], fresh[j], (cut >> j) & 1u);
+        if (ok && (PLAIN || j < n)) *reinterpret_cast<typename L::Raw*>(out) = L::put(h);
+    }
+}
+// joins the pairs of a group's warps: h comes out as the value before this warp's tile (in walking order), carry as the
+// one after all of them; SUMMARY keeps the product of the gains too
+template <int VEC, bool SUMMARY, bool REVERSE>
+__device__ __forceinline__ void join_warps(float2 (*s_pair)[VEC][32], const RecPlace& q, int warps, unsigned cut, const float (&a)[VEC],
+                                           const float (&b)[VEC], float (&h)[VEC], float (&carry)[VEC], float (&sum_a)[VEC])
+{
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) s_pair[q.group * warps + q.w][v][q.lane] = make_float2(cut != 0 ? -1.0f : a[v], b[v]);
+    group_barrier(q.group, warps);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) h[v] = carry[v];
+    for (int i = 0; i < warps; ++i) {
+        const int w = REVERSE ? warps - 1 - i : i;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float2 ab = s_pair[q.group * warps + w][v][q.lane];
+            if (w == q.w) h[v] = carry[v];
+            if (SUMMARY) sum_a[v] = ab.x < 0.0f || sum_a[v] < 0.0f ? -1.0f : sum_a[v] * ab.x;
+            carry[v] = apply_pair(ab, carry[v]);
+        }
+    }
+}
+
+// STREAM: one warp a group, tile after tile, the next one's loads under this one's arithmetic.  TEAM: the warps of a group
+// take a tile each.  SUMMARY: as TEAM, only the pairs of the ranges.
+enum RecMode { kStream, kTeam, kSummary };
+
+// Forward.  saved (nullable): the state before steps 0, 16, 32, ... as [batch, ceil(steps / 16), channels].
+template <typename T, int VEC, bool FLAT, RecMode MODE>
 __global__ void __launch_bounds__(kRecThreads, 2)
 puff_recurrence_kernel(RecArgs p, RecPlan plan, float2* pairs, T* __restrict__ outputs, float* __restrict__ final_state,
                        float* __restrict__ saved)
 {
-    using L = Lane<T, VEC>;
-    using Raw = typename L::Raw;
-    __shared__ float2 s_pair[2][kRecWarps][VEC][32];
-    if (!SUMMARY) pdl_wait();
+    using Raw = typename Lane<T, VEC>::Raw;
+    __shared__ float2 s_pair[MODE == kStream ? 1 : 2][MODE == kStream ? 1 : kRecWarps][VEC][32];
+    if (MODE != kSummary) pdl_wait();
     const RecPlace q = rec_place<VEC, FLAT>(p, plan);
     if (!q.unit) return;
     const long long lanes = p.batch * p.channels;
@@ -189,96 +356,152 @@ puff_recurrence_kernel(RecArgs p, RecPlan plan, float2* pairs, T* __restrict__ o
     float carry[VEC], sum_a[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        carry[v] = !SUMMARY && q.ok && p.state != nullptr ? p.state[q.index + v] : 0.0f;
+        carry[v] = MODE != kSummary && q.ok && p.state != nullptr ? p.state[q.index + v] : 0.0f;
         sum_a[v] = 1.0f;
     }
-    if (!SUMMARY)
+    if (MODE == kTeam)
         for (int r = 0; r < q.split; ++r)
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
                 if (q.ok) carry[v] = apply_pair(pairs[r * lanes + q.index + v], carry[v]);
+    const long long step = kRecTile * plan.warps;
+    long long t0 = q.t_begin + q.w * kRecTile;
+    const long long gates_at = q.b * p.gates_batch_stride + q.c, inputs_at = q.b * p.inputs_batch_stride + q.c;
+    T* out = outputs + (q.b * p.steps + t0) * p.channels + q.c;
+    float* save = saved != nullptr ? saved + (q.b * tiles + t0 / kRecTile) * p.channels + q.c : nullptr;
+    Raw raw_g[kRecTile], raw_x[kRecTile];
+    if (MODE == kStream) {
+        load_tile<Raw, VEC>(raw_g, p.gates, gates_at + t0 * p.gates_step_stride, p.gates_step_stride, q.steps_at(t0), q.ok);
+        load_tile<Raw, VEC>(raw_x, p.inputs, inputs_at + t0 * p.inputs_step_stride, p.inputs_step_stride, q.steps_at(t0), q.ok);
+    }
     int parity = 0;
-    for (long long t = q.t_begin; t < q.t_end; t += kRecTile * plan.warps, parity ^= 1) {
-        const long long t0 = t + q.w * kRecTile;
-        const int n = static_cast<int>(q.t_end - t0 < 0 ? 0 : q.t_end - t0 < kRecTile ? q.t_end - t0 : kRecTile);
-        Raw raw_g[kRecTile], raw_x[kRecTile];
-        load_tile<Raw, VEC>(raw_g, p.gates, q.b * p.gates_batch_stride + t0 * p.gates_step_stride + q.c, p.gates_step_stride, n, q.ok);
-        load_tile<Raw, VEC>(raw_x, p.inputs, q.b * p.inputs_batch_stride + t0 * p.inputs_step_stride + q.c, p.inputs_step_stride, n, q.ok);
+    for (long long t = q.t_begin; t < q.t_end; t += step, t0 += step, parity ^= 1) {
+        const int n = q.steps_at(t0);
         const unsigned cut = reset_mask<FLAT>(p, q, t0, n);
-        float keep[kRecTile][VEC], fresh[kRecTile][VEC];
+        const bool plain = n == kRecTile && !(FLAT ? __any_sync(0xffffffffu, cut != 0) : cut != 0);
+        if (MODE == kStream) {
+            Raw next_g[kRecTile], next_x[kRecTile];
+            const long long t1 = t0 + step;
+            load_tile<Raw, VEC>(next_g, p.gates, gates_at + t1 * p.gates_step_stride, p.gates_step_stride, q.steps_at(t1), q.ok);
+            load_tile<Raw, VEC>(next_x, p.inputs, inputs_at + t1 * p.inputs_step_stride, p.inputs_step_stride, q.steps_at(t1), q.ok);
+            if (save != nullptr && q.ok)
 #pragma unroll
-        for (int j = 0; j < kRecTile; ++j) {
-            float g[VEC], x[VEC];
-            L::get(raw_g[j], g);
-            L::get(raw_x[j], x);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float take;
-                gate_pair(j < n ? gate_code(g[v]) : kHold, keep[j][v], take);
-                fresh[j][v] = take * x[v];
-            }
-        }
-        float h[VEC];
-        if (plan.warps > 1 || SUMMARY) {
-            float a[VEC], b[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                a[v] = 1.0f;
-                b[v] = 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < kRecTile; ++j)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    b[v] = (cut >> j) & 1u ? fresh[j][v] : fmaf(keep[j][v], b[v], fresh[j][v]);
-                    a[v] *= keep[j][v];
-                }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) s_pair[parity][threadIdx.x >> 5][v][q.lane] = make_float2(cut != 0 ? -1.0f : a[v], b[v]);
-            group_barrier(q.group, plan.warps);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = carry[v];
-            for (int w = 0; w < plan.warps; ++w)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const float2 ab = s_pair[parity][q.group * plan.warps + w][v][q.lane];
-                    if (w == q.w) h[v] = carry[v];
-                    if (SUMMARY) sum_a[v] = ab.x < 0.0f || sum_a[v] < 0.0f ? -1.0f : sum_a[v] * ab.x;
-                    carry[v] = apply_pair(ab, carry[v]);
-                }
-        } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = carry[v];
-        }
-        if (!SUMMARY) {
-            if (saved != nullptr && q.ok && n > 0)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) saved[(q.b * tiles + t0 / kRecTile) * p.channels + q.c + v] = h[v];
-            T* out = outputs + (q.b * p.steps + t0) * p.channels + q.c;
+                for (int v = 0; v < VEC; ++v) save[v] = carry[v];
+            if (plain) forward_stream<T, VEC, true>(raw_g, raw_x, cut, n, carry, out, p.channels, q.ok);
+            else forward_stream<T, VEC, false>(raw_g, raw_x, cut, n, carry, out, p.channels, q.ok);
 #pragma unroll
             for (int j = 0; j < kRecTile; ++j) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) h[v] = (cut >> j) & 1u ? fresh[j][v] : fmaf(keep[j][v], h[v], fresh[j][v]);
-                if (q.ok && j < n) *reinterpret_cast<Raw*>(out) = L::put(h);
-                out += p.channels;
+                raw_g[j] = next_g[j];
+                raw_x[j] = next_x[j];
             }
-            if (plan.warps == 1)
+        } else {
+            load_tile<Raw, VEC>(raw_g, p.gates, gates_at + t0 * p.gates_step_stride, p.gates_step_stride, n, q.ok);
+            load_tile<Raw, VEC>(raw_x, p.inputs, inputs_at + t0 * p.inputs_step_stride, p.inputs_step_stride, n, q.ok);
+            float keep[kRecTile][VEC], fresh[kRecTile][VEC], a[VEC], b[VEC], h[VEC];
+            if (plain) forward_pair<T, VEC, true>(raw_g, raw_x, cut, n, keep, fresh, a, b);
+            else forward_pair<T, VEC, false>(raw_g, raw_x, cut, n, keep, fresh, a, b);
+            join_warps<VEC, MODE == kSummary, false>(s_pair[parity], q, plan.warps, cut, a, b, h, carry, sum_a);
+            if (MODE == kTeam) {
+                if (save != nullptr && q.ok && n > 0)
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) carry[v] = h[v];
+                    for (int v = 0; v < VEC; ++v) save[v] = h[v];
+                if (plain) forward_states<T, VEC, true>(keep, fresh, cut, n, h, out, p.channels, q.ok);
+                else forward_states<T, VEC, false>(keep, fresh, cut, n, h, out, p.channels, q.ok);
+            }
         }
+        out += step * p.channels;
+        if (save != nullptr) save += plan.warps * p.channels;
     }
     if (q.ok && q.w == 0) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            if (SUMMARY) pairs[q.split * lanes + q.index + v] = make_float2(sum_a[v], carry[v]);
+            if (MODE == kSummary) pairs[q.split * lanes + q.index + v] = make_float2(sum_a[v], carry[v]);
             else if (q.split == plan.splits - 1) final_state[q.index + v] = carry[v];
         }
     }
 }
 
-// Backward, last tile first.  The states within a tile are computed again from the saved one before it; the pairs map
-// lam after a tile (dh of the next steps times their gains) to lam before it.
-template <typename T, int VEC, bool FLAT, bool SUMMARY>
+// ---- backward: lam_t = dh_t + a_{t+1} lam_{t+1}, last tile first
+// the states again, as what dgate needs of them: slope = keep take (state before - input)
+template <typename T, int VEC, bool PLAIN>
+__device__ __forceinline__ void backward_states(const typename Lane<T, VEC>::Raw (&raw_g)[kRecTile],
+                                                const typename Lane<T, VEC>::Raw (&raw_x)[kRecTile], unsigned cut, int n,
+                                                float (&h)[VEC], float (&code)[kRecTile][VEC], float (&slope)[kRecTile][VEC])
+{
+    using L = Lane<T, VEC>;
+#pragma unroll
+    for (int j = 0; j < kRecTile; ++j) {
+        float g[VEC], x[VEC], keep[VEC], take[VEC], fresh[VEC], minus[VEC], diff[VEC], product[VEC];
+        L::get(raw_g[j], g);
+        L::get(raw_x[j], x);
+        gate_codes(g, code[j]);
+        const bool reset = !PLAIN && (cut >> j) & 1u;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            if (!PLAIN && j >= n) code[j][v] = kHold;
+            if (reset) h[v] = 0.0f;
+            minus[v] = -x[v];
+        }
+        gate_pairs(code[j], keep, take);
+        v_add(diff, h, minus);
+        v_mul(product, keep, take);
+        v_mul(slope[j], product, diff);
+        v_mul(fresh, take, x);
+        advance<VEC, PLAIN>(h, keep, fresh, reset);
+    }
+}
+// lam after the tile -> lam before it, as a pair
+template <typename T, int VEC, bool PLAIN>
+__device__ __forceinline__ void backward_pair(const float (&code)[kRecTile][VEC], const typename Lane<T, VEC>::Raw (&raw_d)[kRecTile],
+                                              unsigned cut, float (&a)[VEC], float (&b)[VEC])
+{
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        a[v] = 1.0f;
+        b[v] = 0.0f;
+    }
+#pragma unroll
+    for (int j = kRecTile - 1; j >= 0; --j) {
+        float d[VEC], keep[VEC], take[VEC];
+        Lane<T, VEC>::get(raw_d[j], d);
+        gate_pairs(code[j], keep, take);
+        v_add(b, b, d);
+        v_mul(b, b, keep);
+        v_mul(a, a, keep);
+        if (!PLAIN && (cut >> j) & 1u)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) b[v] = 0.0f;
+    }
+}
+template <typename T, int VEC, bool PLAIN>
+__device__ __forceinline__ void backward_gradients(const float (&code)[kRecTile][VEC], const float (&slope)[kRecTile][VEC],
+                                                   const typename Lane<T, VEC>::Raw (&raw_d)[kRecTile], unsigned cut, int n,
+                                                   float (&lam)[VEC], T* dgates, T* dinputs, long long stride, bool ok)
+{
+    using L = Lane<T, VEC>;
+    dgates += (kRecTile - 1) * stride;
+    dinputs += (kRecTile - 1) * stride;
+#pragma unroll
+    for (int j = kRecTile - 1; j >= 0; --j, dgates -= stride, dinputs -= stride) {
+        float d[VEC], keep[VEC], take[VEC], dx[VEC], dg[VEC];
+        L::get(raw_d[j], d);
+        gate_pairs(code[j], keep, take);
+        v_add(lam, lam, d);
+        v_mul(dx, lam, take);
+        v_mul(dg, lam, slope[j]);
+        if (ok && (PLAIN || j < n)) {
+            *reinterpret_cast<typename L::Raw*>(dinputs) = L::put(dx);
+            *reinterpret_cast<typename L::Raw*>(dgates) = L::put(dg);
+        }
+        v_mul(lam, lam, keep);
+        if (!PLAIN && (cut >> j) & 1u)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) lam[v] = 0.0f;
+    }
+}
+
+// The states within a tile are computed again from the saved one before it.
+template <typename T, int VEC, bool FLAT, RecMode MODE>
 __global__ void __launch_bounds__(kRecThreads, 2)
 puff_recurrence_backward_kernel(RecArgs p, RecPlan plan, float2* pairs, const float* __restrict__ saved,
                                 const T* __restrict__ doutputs, const float* __restrict__ dfinal, T* __restrict__ dgates,
@@ -286,8 +509,8 @@ puff_recurrence_backward_kernel(RecArgs p, RecPlan plan, float2* pairs, const fl
 {
     using L = Lane<T, VEC>;
     using Raw = typename L::Raw;
-    __shared__ float2 s_pair[2][kRecWarps][VEC][32];
-    if (!SUMMARY) pdl_wait();
+    __shared__ float2 s_pair[MODE == kStream ? 1 : 2][MODE == kStream ? 1 : kRecWarps][VEC][32];
+    if (MODE != kSummary) pdl_wait();
     const RecPlace q = rec_place<VEC, FLAT>(p, plan);
     if (!q.unit) return;
     const long long lanes = p.batch * p.channels;
@@ -295,117 +518,66 @@ puff_recurrence_backward_kernel(RecArgs p, RecPlan plan, float2* pairs, const fl
     float carry[VEC], sum_a[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        carry[v] = !SUMMARY && q.ok && dfinal != nullptr ? dfinal[q.index + v] : 0.0f;
+        carry[v] = MODE != kSummary && q.ok && dfinal != nullptr ? dfinal[q.index + v] : 0.0f;
         sum_a[v] = 1.0f;
     }
-    if (!SUMMARY)
+    if (MODE == kTeam)
         for (int r = plan.splits - 1; r > q.split; --r)
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
                 if (q.ok) carry[v] = apply_pair(pairs[r * lanes + q.index + v], carry[v]);
-    const long long span = kRecTile * plan.warps;
+    const long long step = kRecTile * plan.warps;
+    const long long gates_at = q.b * p.gates_batch_stride + q.c, inputs_at = q.b * p.inputs_batch_stride + q.c;
     int parity = 0;
-    for (long long t = q.t_begin + (q.t_end - q.t_begin - 1) / span * span; t >= q.t_begin; t -= span, parity ^= 1) {
+    for (long long t = q.t_begin + quotient(q.t_end > q.t_begin ? q.t_end - q.t_begin - 1 : 0, step) * step; t >= q.t_begin;
+         t -= step, parity ^= 1) {
         const long long t0 = t + q.w * kRecTile;
-        const int n = static_cast<int>(q.t_end - t0 < 0 ? 0 : q.t_end - t0 < kRecTile ? q.t_end - t0 : kRecTile);
+        const int n = q.steps_at(t0);
         const long long at = (q.b * p.steps + t0) * p.channels + q.c;
         Raw raw_g[kRecTile], raw_x[kRecTile], raw_d[kRecTile];
-        load_tile<Raw, VEC>(raw_g, p.gates, q.b * p.gates_batch_stride + t0 * p.gates_step_stride + q.c, p.gates_step_stride, n, q.ok);
+        load_tile<Raw, VEC>(raw_g, p.gates, gates_at + t0 * p.gates_step_stride, p.gates_step_stride, n, q.ok);
+        if (MODE != kSummary)
+            load_tile<Raw, VEC>(raw_x, p.inputs, inputs_at + t0 * p.inputs_step_stride, p.inputs_step_stride, n, q.ok);
         load_tile<Raw, VEC>(raw_d, doutputs, at, p.channels, n, q.ok && doutputs != nullptr);
-        if (!SUMMARY)
-            load_tile<Raw, VEC>(raw_x, p.inputs, q.b * p.inputs_batch_stride + t0 * p.inputs_step_stride + q.c, p.inputs_step_stride, n, q.ok);
-        const unsigned cut = reset_mask<FLAT>(p, q, t0, n);
-        float code[kRecTile][VEC], diff[kRecTile][VEC];   // diff: the state a step starts from, minus its input
         float h[VEC];
-        if (!SUMMARY)
+        if (MODE != kSummary)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) h[v] = q.ok && n > 0 ? saved[(q.b * tiles + t0 / kRecTile) * p.channels + q.c + v] : 0.0f;
+        const unsigned cut = reset_mask<FLAT>(p, q, t0, n);
+        const bool plain = n == kRecTile && !(FLAT ? __any_sync(0xffffffffu, cut != 0) : cut != 0);
+        float code[kRecTile][VEC], slope[kRecTile][VEC];
+        if (MODE == kSummary) {
 #pragma unroll
-        for (int j = 0; j < kRecTile; ++j) {
-            float g[VEC], x[VEC];
-            L::get(raw_g[j], g);
-            if (!SUMMARY) L::get(raw_x[j], x);
+            for (int j = 0; j < kRecTile; ++j) {
+                float g[VEC];
+                L::get(raw_g[j], g);
+                gate_codes(g, code[j]);
+                if (j >= n)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                code[j][v] = j < n ? gate_code(g[v]) : kHold;
-                if (!SUMMARY) {
-                    float keep, take;
-                    gate_pair(code[j][v], keep, take);
-                    const float before = (cut >> j) & 1u ? 0.0f : h[v], fresh = take * x[v];
-                    diff[j][v] = before - x[v];
-                    h[v] = (cut >> j) & 1u ? fresh : fmaf(keep, h[v], fresh);
-                }
+                    for (int v = 0; v < VEC; ++v) code[j][v] = kHold;
             }
+        } else if (plain) {
+            backward_states<T, VEC, true>(raw_g, raw_x, cut, n, h, code, slope);
+        } else {
+            backward_states<T, VEC, false>(raw_g, raw_x, cut, n, h, code, slope);
         }
         float lam[VEC];
-        if (plan.warps > 1 || SUMMARY) {
+        if (MODE != kStream) {
             float a[VEC], b[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                a[v] = 1.0f;
-                b[v] = 0.0f;
-            }
-#pragma unroll
-            for (int j = kRecTile - 1; j >= 0; --j) {
-                float d[VEC];
-                L::get(raw_d[j], d);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    float keep, take;
-                    gate_pair(code[j][v], keep, take);
-                    b[v] = (cut >> j) & 1u ? 0.0f : (b[v] + d[v]) * keep;
-                    a[v] *= keep;
-                }
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) s_pair[parity][threadIdx.x >> 5][v][q.lane] = make_float2(cut != 0 ? -1.0f : a[v], b[v]);
-            group_barrier(q.group, plan.warps);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) lam[v] = carry[v];
-            for (int w = plan.warps - 1; w >= 0; --w)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const float2 ab = s_pair[parity][q.group * plan.warps + w][v][q.lane];
-                    if (w == q.w) lam[v] = carry[v];
-                    if (SUMMARY) sum_a[v] = ab.x < 0.0f || sum_a[v] < 0.0f ? -1.0f : sum_a[v] * ab.x;
-                    carry[v] = apply_pair(ab, carry[v]);
-                }
-        } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) lam[v] = carry[v];
+            if (plain) backward_pair<T, VEC, true>(code, raw_d, cut, a, b);
+            else backward_pair<T, VEC, false>(code, raw_d, cut, a, b);
+            join_warps<VEC, MODE == kSummary, true>(s_pair[parity], q, plan.warps, cut, a, b, lam, carry, sum_a);
         }
-        if (!SUMMARY) {
-            T* out_x = dinputs + at + (kRecTile - 1) * p.channels;
-            T* out_g = dgates + at + (kRecTile - 1) * p.channels;
-#pragma unroll
-            for (int j = kRecTile - 1; j >= 0; --j) {
-                float d[VEC], dx[VEC], dg[VEC];
-                L::get(raw_d[j], d);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    float keep, take;
-                    gate_pair(code[j][v], keep, take);
-                    lam[v] += d[v];
-                    dx[v] = lam[v] * take;
-                    dg[v] = dx[v] * keep * diff[j][v];
-                    lam[v] = (cut >> j) & 1u ? 0.0f : lam[v] * keep;
-                }
-                if (q.ok && j < n) {
-                    *reinterpret_cast<Raw*>(out_x) = L::put(dx);
-                    *reinterpret_cast<Raw*>(out_g) = L::put(dg);
-                }
-                out_x -= p.channels;
-                out_g -= p.channels;
-            }
-            if (plan.warps == 1)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) carry[v] = lam[v];
+        if (MODE != kSummary) {
+            float (&l)[VEC] = MODE == kStream ? carry : lam;
+            if (plain) backward_gradients<T, VEC, true>(code, slope, raw_d, cut, n, l, dgates + at, dinputs + at, p.channels, q.ok);
+            else backward_gradients<T, VEC, false>(code, slope, raw_d, cut, n, l, dgates + at, dinputs + at, p.channels, q.ok);
         }
     }
     if (q.ok && q.w == 0) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            if (SUMMARY) pairs[q.split * lanes + q.index + v] = make_float2(sum_a[v], carry[v]);
+            if (MODE == kSummary) pairs[q.split * lanes + q.index + v] = make_float2(sum_a[v], carry[v]);
             else if (q.split == 0 && dstate != nullptr) dstate[q.index + v] = carry[v];
         }
     }
@@ -421,13 +593,14 @@ puff_recurrence_step_kernel(const T* __restrict__ gates, const T* __restrict__ i
     const long long n = batch * channels, stride = static_cast<long long>(gridDim.x) * 256;
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += stride) {
         const long long b = i / channels, c = i - b * channels;
-        float keep, take;
-        gate_pair(gate_code(to_f32(gates[b * gates_stride + c])), keep, take);
-        const float fresh = take * to_f32(inputs[b * inputs_stride + c]);
+        float g[1] = {to_f32(gates[b * gates_stride + c])}, code[1], keep[1], take[1];
+        gate_codes(g, code);
+        gate_pairs(code, keep, take);
+        const float fresh = take[0] * to_f32(inputs[b * inputs_stride + c]);
         bool reset = false;
         if (reset_bytes == 4) reset = static_cast<const float*>(resets)[b] != 0.0f;
         else if (reset_bytes == 1) reset = static_cast<const unsigned char*>(resets)[b] != 0;
-        const float h = reset ? fresh : fmaf(keep, state[i], fresh);
+        const float h = reset ? fresh : fmaf(keep[0], state[i], fresh);
         new_state[i] = h;
         outputs[i] = from_f32<T>(h);
     }
@@ -570,9 +743,9 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
 #define PUFF_RUN2(T, VEC, FLAT)                                                                                          \
-    rec_launch(plan.splits > 1 ? puff_recurrence_kernel<T, VEC, FLAT, true> : nullptr,                                    \
-               puff_recurrence_kernel<T, VEC, FLAT, false>, plan, st, p, plan, pairs, static_cast<T*>(outputs),           \
-               final_state, saved)
+    rec_launch(plan.splits > 1 ? puff_recurrence_kernel<T, VEC, FLAT, kSummary> : nullptr,                                \
+               plan.warps > 1 ? puff_recurrence_kernel<T, VEC, FLAT, kTeam> : puff_recurrence_kernel<T, VEC, FLAT, kStream>, \
+               plan, st, p, plan, pairs, static_cast<T*>(outputs), final_state, saved)
     if (dtype == PUFF_DTYPE_F32) e = flat ? PUFF_RUN2(float, 1, true) : PUFF_RUN2(float, 1, false);
     else if (dtype == PUFF_DTYPE_F16) e = pair ? PUFF_RUN2(__half, 2, false) : flat ? PUFF_RUN2(__half, 1, true) : PUFF_RUN2(__half, 1, false);
     else e = pair ? PUFF_RUN2(__nv_bfloat16, 2, false) : flat ? PUFF_RUN2(__nv_bfloat16, 1, true) : PUFF_RUN2(__nv_bfloat16, 1, false);
@@ -624,8 +797,9 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
 #define PUFF_RUN2(T, VEC, FLAT)                                                                                          \
-    rec_launch(plan.splits > 1 ? puff_recurrence_backward_kernel<T, VEC, FLAT, true> : nullptr,                           \
-               puff_recurrence_backward_kernel<T, VEC, FLAT, false>, plan, st, p, plan, pairs, saved,                     \
+    rec_launch(plan.splits > 1 ? puff_recurrence_backward_kernel<T, VEC, FLAT, kSummary> : nullptr,                       \
+               plan.warps > 1 ? puff_recurrence_backward_kernel<T, VEC, FLAT, kTeam>                                      \
+                              : puff_recurrence_backward_kernel<T, VEC, FLAT, kStream>, plan, st, p, plan, pairs, saved,  \
                static_cast<const T*>(doutputs), dfinal, static_cast<T*>(dgates), static_cast<T*>(dinputs), dstate)
     if (dtype == PUFF_DTYPE_F32) e = flat ? PUFF_RUN2(float, 1, true) : PUFF_RUN2(float, 1, false);
     else if (dtype == PUFF_DTYPE_F16) e = pair ? PUFF_RUN2(__half, 2, false) : flat ? PUFF_RUN2(__half, 1, true) : PUFF_RUN2(__half, 1, false);
