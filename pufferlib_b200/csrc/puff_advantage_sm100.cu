@@ -630,6 +630,7 @@ extern "C" long long puff_advantage_sm100_launch_count(void)
 namespace puff {
 void count_launch() { g_launch_count.fetch_add(1, std::memory_order_relaxed); }
 int tune_value(int knob, int fallback) { return tune(knob, fallback); }
+void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_tiled_fn()); }
 int require_sm100(int* sm_count)
 {
     int code = PUFF_OK;

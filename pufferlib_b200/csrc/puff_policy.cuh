@@ -12,7 +12,10 @@
 
 namespace puff {
 void count_launch();
-int require_sm100(int* sm_count);   // puff_advantage_sm100.cu: PUFF_OK, or why nothing can be launched here
+// puff_advantage_sm100.cu: PUFF_OK, or why nothing can be launched here; the status word; cuTensorMapEncodeTiled
+int require_sm100(int* sm_count);
+int* device_status_ptr();
+void* tensor_map_encoder();
 
 // ---- element types: read to fp32, rounded once (to nearest even) when written ----------------------------------
 __device__ __forceinline__ float to_f32(float v) { return v; }

@@ -46,8 +46,8 @@ __device__ __forceinline__ bool is_reset(const RecArgs& p, long long i)
     return p.reset_bytes == 1 && static_cast<const unsigned char*>(p.resets)[i] != 0;
 }
 
-// keep = sigmoid(g) and take = 1 - keep = sigmoid(-g).  The smaller of the two is e / (1 + e) with e = e^-|g|, good to
-// a few ulp however small; the larger is 1 minus it, so that the two add up to 1 and the state stays a weighted mean.
+// keep = sigmoid(g) and take = 1 - keep = sigmoid(-g).  The smaller of the two is 1 / (1 + e^|g|), good to a few
+// ulp however small; the larger is 1 minus it, so that the two add up to 1 and the state stays a weighted mean.
 // One register, the code, holds both: the smaller one with the sign of g.
 __device__ __forceinline__ float rcp_approx(float x)
 {
@@ -91,18 +91,15 @@ __device__ __forceinline__ void v_add(float (&d)[VEC], const float (&a)[VEC], co
 template <int VEC>
 __device__ __forceinline__ void gate_codes(const float (&g)[VEC], float (&code)[VEC])
 {
-    float e[VEC], one[VEC], d[VEC], r[VEC];
+    float e[VEC], one[VEC], d[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        e[v] = exp2_approx(fabsf(g[v]) * -kLog2e);
+        e[v] = exp2_approx(fabsf(g[v]) * kLog2e);
         one[v] = 1.0f;
     }
     v_add(d, e, one);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) r[v] = rcp_approx(d[v]);
-    v_mul(d, e, r);
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) code[v] = copysignf(d[v], g[v]);
+    for (int v = 0; v < VEC; ++v) code[v] = copysignf(rcp_approx(d[v]), g[v]);
 }
 template <int VEC>
 __device__ __forceinline__ void gate_pairs(const float (&code)[VEC], float (&keep)[VEC], float (&take)[VEC])
@@ -267,10 +264,8 @@ __device__ __forceinline__ void advance(float (&h)[VEC], const float (&keep)[VEC
         for (int v = 0; v < VEC; ++v) h[v] = fresh[v];
 }
 // one pass: every step's state follows from the one before it
-template <typename T, int VEC, bool PLAIN>
-__device__ __forceinline__ void forward_stream(const typename Lane<T, VEC>::Raw (&raw_g)[kRecTile],
-                                               const typename Lane<T, VEC>::Raw (&raw_x)[kRecTile], unsigned cut, int n,
-                                               float (&h)[VEC], T* out, long long stride, bool ok)
+template <typename T, int VEC, bool PLAIN, typename Tile>
+__device__ __forceinline__ void forward_stream(const Tile& raw_g, const Tile& raw_x, unsigned cut, int n, float (&h)[VEC], T* out, long long stride, bool ok)
 {
     using L = Lane<T, VEC>;
 #pragma unroll
@@ -282,10 +277,8 @@ __device__ __forceinline__ void forward_stream(const typename Lane<T, VEC>::Raw 
     }
 }
 // two passes: the tile's pair (a, b), then its states once the one before it is known
-template <typename T, int VEC, bool PLAIN>
-__device__ __forceinline__ void forward_pair(const typename Lane<T, VEC>::Raw (&raw_g)[kRecTile],
-                                             const typename Lane<T, VEC>::Raw (&raw_x)[kRecTile], unsigned cut, int n,
-                                             float (&keep)[kRecTile][VEC], float (&fresh)[kRecTile][VEC], float (&a)[VEC], float (&b)[VEC])
+template <typename T, int VEC, bool PLAIN, typename Tile>
+__device__ __forceinline__ void forward_pair(const Tile& raw_g, const Tile& raw_x, unsigned cut, int n, float (&keep)[kRecTile][VEC], float (&fresh)[kRecTile][VEC], float (&a)[VEC], float (&b)[VEC])
 {
 #pragma unroll
     for (int j = 0; j < kRecTile; ++j) {
@@ -423,10 +416,8 @@ puff_recurrence_kernel(RecArgs p, RecPlan plan, float2* pairs, T* __restrict__ o
 
 // ---- backward: lam_t = dh_t + a_{t+1} lam_{t+1}, last tile first
 // the states again, as what dgate needs of them: slope = keep take (state before - input)
-template <typename T, int VEC, bool PLAIN>
-__device__ __forceinline__ void backward_states(const typename Lane<T, VEC>::Raw (&raw_g)[kRecTile],
-                                                const typename Lane<T, VEC>::Raw (&raw_x)[kRecTile], unsigned cut, int n,
-                                                float (&h)[VEC], float (&code)[kRecTile][VEC], float (&slope)[kRecTile][VEC])
+template <typename T, int VEC, bool PLAIN, typename Tile>
+__device__ __forceinline__ void backward_states(const Tile& raw_g, const Tile& raw_x, unsigned cut, int n, float (&h)[VEC], float (&code)[kRecTile][VEC], float (&slope)[kRecTile][VEC])
 {
     using L = Lane<T, VEC>;
 #pragma unroll
@@ -451,9 +442,8 @@ __device__ __forceinline__ void backward_states(const typename Lane<T, VEC>::Raw
     }
 }
 // lam after the tile -> lam before it, as a pair
-template <typename T, int VEC, bool PLAIN>
-__device__ __forceinline__ void backward_pair(const float (&code)[kRecTile][VEC], const typename Lane<T, VEC>::Raw (&raw_d)[kRecTile],
-                                              unsigned cut, float (&a)[VEC], float (&b)[VEC])
+template <typename T, int VEC, bool PLAIN, typename Tile>
+__device__ __forceinline__ void backward_pair(const float (&code)[kRecTile][VEC], const Tile& raw_d, unsigned cut, float (&a)[VEC], float (&b)[VEC])
 {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
@@ -473,9 +463,9 @@ __device__ __forceinline__ void backward_pair(const float (&code)[kRecTile][VEC]
             for (int v = 0; v < VEC; ++v) b[v] = 0.0f;
     }
 }
-template <typename T, int VEC, bool PLAIN>
+template <typename T, int VEC, bool PLAIN, typename Tile>
 __device__ __forceinline__ void backward_gradients(const float (&code)[kRecTile][VEC], const float (&slope)[kRecTile][VEC],
-                                                   const typename Lane<T, VEC>::Raw (&raw_d)[kRecTile], unsigned cut, int n,
+                                                   const Tile& raw_d, unsigned cut, int n,
                                                    float (&lam)[VEC], T* dgates, T* dinputs, long long stride, bool ok)
 {
     using L = Lane<T, VEC>;
@@ -583,6 +573,11 @@ puff_recurrence_backward_kernel(RecArgs p, RecPlan plan, float2* pairs, const fl
     }
 }
 
+}  // namespace puff
+
+#include "puff_recurrence_tma.cuh"
+
+namespace puff {
 // One step of every row; new_state may be state.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -643,20 +638,27 @@ static int rec_grid(const RecPlan& plan)
 }
 // The pairs of the ranges first where there are several, then the pass itself behind it
 template <typename... KArgs, typename... Args>
-static cudaError_t rec_launch(void (*summary)(KArgs...), void (*kernel)(KArgs...), const RecPlan& plan, cudaStream_t st, Args... args)
+static cudaError_t rec_launch(void (*summary)(KArgs...), void (*kernel)(KArgs...), size_t smem, const RecPlan& plan, cudaStream_t st,
+                              const Args&... args)
 {
     const int grid = rec_grid(plan);
+    if (smem > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e == cudaSuccess && summary != nullptr)
+            e = cudaFuncSetAttribute(summary, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
     if (summary == nullptr) {
-        kernel<<<grid, kRecThreads, 0, st>>>(static_cast<KArgs>(args)...);
+        kernel<<<grid, kRecThreads, smem, st>>>(static_cast<KArgs>(args)...);
         count_launch();
         return cudaGetLastError();
     }
-    summary<<<grid, kRecThreads, 0, st>>>(static_cast<KArgs>(args)...);
+    summary<<<grid, kRecThreads, smem, st>>>(static_cast<KArgs>(args)...);
     count_launch();
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     count_launch();
-    return launch_neighbour(kernel, grid, kRecThreads, 0, st, args...);
+    return launch_neighbour(kernel, grid, kRecThreads, smem, st, args...);
 }
 // channels too few to fill half a warp's lanes: rows share warps
 static bool rec_flat(long long channels, int vec) { return channels < 16 * vec; }
@@ -738,14 +740,31 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
                       inputs_batch_stride % 2 == 0 && inputs_step_stride % 2 == 0 && !misaligned(gates, 4) &&
                       !misaligned(inputs, 4) && !misaligned(outputs, 4) && !rec_flat(channels, 2);
     const bool flat = rec_flat(channels, 1);
-    const RecPlan plan = rec_plan(batch, steps, channels, pair ? 2 : 1, flat);
+    const ViewStrides gs = {gates_batch_stride, gates_step_stride}, xs = {inputs_batch_stride, inputs_step_stride};
+    const ViewStrides dense = {steps * channels, channels};
+    const bool tma = tma_shape(p, size) && tma_view(p, gates, gs, size) && tma_view(p, inputs, xs, size) && tma_view(p, outputs, dense, size);
+    const RecPlan plan = rec_plan(batch, steps, channels, tma ? 4 / size : pair ? 2 : 1, flat);
     float2* pairs = static_cast<float2*>(scratch);
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
+    if (tma) {
+        CUtensorMap mg, mx, mo;
+        int* status = device_status_ptr();
+        if (status == nullptr || !tma_map(&mg, p, gates, gs, dtype) || !tma_map(&mx, p, inputs, xs, dtype) ||
+            !tma_map(&mo, p, outputs, dense, dtype))
+            return PUFF_ERR_DRIVER;
+#define PUFF_RUN2(T, VEC)                                                                                                \
+    rec_launch(plan.splits > 1 ? puff_recurrence_tma_kernel<T, VEC, kSummary> : nullptr,                                  \
+               plan.warps > 1 ? puff_recurrence_tma_kernel<T, VEC, kTeam> : puff_recurrence_tma_kernel<T, VEC, kStream>,  \
+               tma_smem(2, kTmaForwardStages), plan, st, mg, mx, mo, p, plan, pairs, final_state, saved, status)
+        e = dtype == PUFF_DTYPE_F32 ? PUFF_RUN2(float, 1) : dtype == PUFF_DTYPE_F16 ? PUFF_RUN2(__half, 2) : PUFF_RUN2(__nv_bfloat16, 2);
+#undef PUFF_RUN2
+        return static_cast<int>(e);
+    }
 #define PUFF_RUN2(T, VEC, FLAT)                                                                                          \
     rec_launch(plan.splits > 1 ? puff_recurrence_kernel<T, VEC, FLAT, kSummary> : nullptr,                                \
                plan.warps > 1 ? puff_recurrence_kernel<T, VEC, FLAT, kTeam> : puff_recurrence_kernel<T, VEC, FLAT, kStream>, \
-               plan, st, p, plan, pairs, static_cast<T*>(outputs), final_state, saved)
+               size_t{0}, plan, st, p, plan, pairs, static_cast<T*>(outputs), final_state, saved)
     if (dtype == PUFF_DTYPE_F32) e = flat ? PUFF_RUN2(float, 1, true) : PUFF_RUN2(float, 1, false);
     else if (dtype == PUFF_DTYPE_F16) e = pair ? PUFF_RUN2(__half, 2, false) : flat ? PUFF_RUN2(__half, 1, true) : PUFF_RUN2(__half, 1, false);
     else e = pair ? PUFF_RUN2(__nv_bfloat16, 2, false) : flat ? PUFF_RUN2(__nv_bfloat16, 1, true) : PUFF_RUN2(__nv_bfloat16, 1, false);
@@ -792,14 +811,33 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
                       !misaligned(inputs, 4) && !misaligned(doutputs, 4) && !misaligned(dgates, 4) &&
                       !misaligned(dinputs, 4) && !rec_flat(channels, 2);
     const bool flat = rec_flat(channels, 1);
-    const RecPlan plan = rec_plan(batch, steps, channels, pair ? 2 : 1, flat);
+    const ViewStrides gs = {gates_batch_stride, gates_step_stride}, xs = {inputs_batch_stride, inputs_step_stride};
+    const ViewStrides dense = {steps * channels, channels};
+    const bool tma = tma_shape(p, size) && tma_view(p, gates, gs, size) && tma_view(p, inputs, xs, size) &&
+                     tma_view(p, doutputs, dense, size) && tma_view(p, dgates, dense, size) && tma_view(p, dinputs, dense, size);
+    const RecPlan plan = rec_plan(batch, steps, channels, tma ? 4 / size : pair ? 2 : 1, flat);
     float2* pairs = static_cast<float2*>(scratch);
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
+    if (tma) {
+        CUtensorMap mg, mx, md, mdg, mdx;
+        int* status = device_status_ptr();
+        if (status == nullptr || !tma_map(&mg, p, gates, gs, dtype) || !tma_map(&mx, p, inputs, xs, dtype) ||
+            !tma_map(&md, p, doutputs, dense, dtype) || !tma_map(&mdg, p, dgates, dense, dtype) || !tma_map(&mdx, p, dinputs, dense, dtype))
+            return PUFF_ERR_DRIVER;
+#define PUFF_RUN2(T, VEC)                                                                                                \
+    rec_launch(plan.splits > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kSummary> : nullptr,                         \
+               plan.warps > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kTeam>                                        \
+                              : puff_recurrence_backward_tma_kernel<T, VEC, kStream>,                                     \
+               tma_smem(3, kTmaBackwardStages), plan, st, mg, mx, md, mdg, mdx, p, plan, pairs, saved, dfinal, dstate, status)
+        e = dtype == PUFF_DTYPE_F32 ? PUFF_RUN2(float, 1) : dtype == PUFF_DTYPE_F16 ? PUFF_RUN2(__half, 2) : PUFF_RUN2(__nv_bfloat16, 2);
+#undef PUFF_RUN2
+        return static_cast<int>(e);
+    }
 #define PUFF_RUN2(T, VEC, FLAT)                                                                                          \
     rec_launch(plan.splits > 1 ? puff_recurrence_backward_kernel<T, VEC, FLAT, kSummary> : nullptr,                       \
                plan.warps > 1 ? puff_recurrence_backward_kernel<T, VEC, FLAT, kTeam>                                      \
-                              : puff_recurrence_backward_kernel<T, VEC, FLAT, kStream>, plan, st, p, plan, pairs, saved,  \
+                              : puff_recurrence_backward_kernel<T, VEC, FLAT, kStream>, size_t{0}, plan, st, p, plan, pairs, saved,  \
                static_cast<const T*>(doutputs), dfinal, static_cast<T*>(dgates), static_cast<T*>(dinputs), dstate)
     if (dtype == PUFF_DTYPE_F32) e = flat ? PUFF_RUN2(float, 1, true) : PUFF_RUN2(float, 1, false);
     else if (dtype == PUFF_DTYPE_F16) e = pair ? PUFF_RUN2(__half, 2, false) : flat ? PUFF_RUN2(__half, 1, true) : PUFF_RUN2(__half, 1, false);
