@@ -202,18 +202,30 @@ __device__ __forceinline__ RecPlace rec_place(const RecArgs& p, const RecPlan& p
     q.t_end = q.t_begin + plan.split_steps < p.steps ? q.t_begin + plan.split_steps : p.steps;
     return q;
 }
-// bit j: step t0 + j is a reset.  All lanes of a row share the mask; FLAT lanes have one each.
+// The resets of a tile as a mask, bit j for step t0 + j, in two halves so that the load is a round old when its value is
+// needed (asked for and used at once, it stalled every round).  All lanes of a row share the mask; FLAT lanes have one each.
 template <bool FLAT>
-__device__ __forceinline__ unsigned reset_mask(const RecArgs& p, const RecPlace& q, long long t0, int n)
+__device__ __forceinline__ unsigned resets_ahead(const RecArgs& p, const RecPlace& q, long long t0, int n)
 {
     if (p.reset_bytes == 0) return 0u;
     const long long at = q.b * p.steps + t0;
-    if (!FLAT) return __ballot_sync(0xffffffffu, q.lane < n && is_reset(p, at + q.lane));
+    if (!FLAT) {
+        if (q.lane >= n) return 0u;
+        return p.reset_bytes == 4 ? __ldg(static_cast<const unsigned*>(p.resets) + at + q.lane)
+                                  : __ldg(static_cast<const unsigned char*>(p.resets) + at + q.lane);
+    }
     unsigned m = 0;
     if (q.ok)
 #pragma unroll 4
         for (int j = 0; j < n; ++j) m |= is_reset(p, at + j) ? 1u << j : 0u;
     return m;
+}
+template <bool FLAT>
+__device__ __forceinline__ unsigned reset_mask(const RecArgs& p, unsigned ahead)
+{
+    if (FLAT || p.reset_bytes == 0) return ahead;
+    // fp32: anything but +0 and -0
+    return __ballot_sync(0xffffffffu, (p.reset_bytes == 4 ? ahead << 1 : ahead) != 0);
 }
 template <typename Raw, int VEC>
 __device__ __forceinline__ void load_tile(Raw (&raw)[kRecTile], const void* base, long long at, long long step_stride, int n, bool ok)
@@ -370,7 +382,7 @@ puff_recurrence_kernel(RecArgs p, RecPlan plan, float2* pairs, T* __restrict__ o
     int parity = 0;
     for (long long t = q.t_begin; t < q.t_end; t += step, t0 += step, parity ^= 1) {
         const int n = q.steps_at(t0);
-        const unsigned cut = reset_mask<FLAT>(p, q, t0, n);
+        const unsigned cut = reset_mask<FLAT>(p, resets_ahead<FLAT>(p, q, t0, n));
         const bool plain = n == kRecTile && !(FLAT ? __any_sync(0xffffffffu, cut != 0) : cut != 0);
         if (MODE == kStream) {
             Raw next_g[kRecTile], next_x[kRecTile];
@@ -533,7 +545,7 @@ puff_recurrence_backward_kernel(RecArgs p, RecPlan plan, float2* pairs, const fl
         if (MODE != kSummary)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) h[v] = q.ok && n > 0 ? saved[(q.b * tiles + t0 / kRecTile) * p.channels + q.c + v] : 0.0f;
-        const unsigned cut = reset_mask<FLAT>(p, q, t0, n);
+        const unsigned cut = reset_mask<FLAT>(p, resets_ahead<FLAT>(p, q, t0, n));
         const bool plain = n == kRecTile && !(FLAT ? __any_sync(0xffffffffu, cut != 0) : cut != 0);
         float code[kRecTile][VEC], slope[kRecTile][VEC];
         if (MODE == kSummary) {
@@ -607,10 +619,11 @@ static long long view_span(long long batch, long long steps, long long channels,
     return ((batch - 1) * bs + (steps - 1) * ss + channels) * size;
 }
 
-// Enough warps to keep the memory busy (about twenty on each of 148 SMs, 4 KB of loads each), first by giving tiles
-// along the steps to several warps of a CTA, then to several CTAs; the second costs reading the inputs twice.
-constexpr long long kRecWantWarps = 148 * 20;
-constexpr int kRecMaxSplits = 64;
+// Two CTAs of eight warps are resident on each of 148 SMs.  Tiles along the steps go to several warps of a CTA while a
+// warp a lane block would leave more than a fifth of that idle, then ranges of steps to several CTAs, as many as one wave
+// holds; the second costs reading the inputs twice.
+constexpr long long kRecSlots = 148 * 2;
+constexpr int kRecMaxSplits = 148;
 static RecPlan rec_plan(long long batch, long long steps, long long channels, int vec, bool flat)
 {
     RecPlan plan;
@@ -618,12 +631,12 @@ static RecPlan rec_plan(long long batch, long long steps, long long channels, in
     plan.lane_blocks = flat ? (batch * channels + 31) / 32 : batch * plan.blocks_per_row;
     const long long tiles = (steps + kRecTile - 1) / kRecTile;
     plan.warps = 1;
-    while (plan.warps < kRecWarps && plan.warps < tiles && plan.lane_blocks * plan.warps < kRecWantWarps) plan.warps *= 2;
+    while (plan.warps < kRecWarps && plan.warps < tiles && plan.lane_blocks * plan.warps * 5 < kRecSlots * kRecWarps * 4) plan.warps *= 2;
     const long long rounds = (tiles + plan.warps - 1) / plan.warps;
     long long splits = 1;
-    // a range of fewer than four rounds would spend its time on the join
-    if (plan.warps == kRecWarps) splits = kRecWantWarps / (plan.lane_blocks * plan.warps);
-    if (splits > rounds / 4) splits = rounds / 4;
+    if (plan.warps == kRecWarps) splits = kRecSlots / plan.lane_blocks;
+    // a range of one round would spend its time on the join
+    if (splits > rounds / 2) splits = rounds / 2;
     if (splits > kRecMaxSplits) splits = kRecMaxSplits;
     if (splits < 1) splits = 1;
     const long long per = rounds > 0 ? (rounds + splits - 1) / splits : 1;

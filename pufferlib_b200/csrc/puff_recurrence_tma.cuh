@@ -132,7 +132,7 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
         sum_a[v] = 1.0f;
     }
     long long t0 = q.t_begin + q.w * kRecTile;
-    unsigned cut_next = reset_mask<false>(p, q, t0, q.steps_at(t0));
+    unsigned resets = resets_ahead<false>(p, q, t0, q.steps_at(t0));
     if (MODE == kTeam)
         for (int r = 0; r < q.split; ++r)
 #pragma unroll
@@ -144,9 +144,9 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
     bool given_up = false;
     for (int t = t_begin; t < t_end; t += step, t0 += step, parity ^= 1) {
         const int n = q.steps_at(t0);
-        const unsigned cut = cut_next;
+        const unsigned cut = reset_mask<false>(p, resets);
         const bool plain = n == kRecTile && cut == 0;
-        cut_next = reset_mask<false>(p, q, t0 + step, q.steps_at(t0 + step));
+        resets = resets_ahead<false>(p, q, t0 + step, q.steps_at(t0 + step));
         ring.bar(stage).wait(phase, given_up, status);
         uint32_t* const g_words = ring.words(stage, 0);
         uint32_t* const x_words = ring.words(stage, 1);
@@ -240,7 +240,7 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
             h_next[v] = MODE != kSummary && q.ok && at >= q.t_begin && at < q.t_end ? saved[(q.b * tiles + at / kRecTile) * p.channels + q.c + v] : 0.0f;
     };
     saved_before(first + q.w * kRecTile);
-    unsigned cut_next = reset_mask<false>(p, q, first + q.w * kRecTile, q.steps_at(first + q.w * kRecTile));
+    unsigned resets = resets_ahead<false>(p, q, first + q.w * kRecTile, q.steps_at(first + q.w * kRecTile));
     if (MODE == kTeam)
         for (int r = plan.splits - 1; r > q.split; --r)
 #pragma unroll
@@ -252,13 +252,13 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
     for (int t = first; t >= t_begin; t -= step) {
         const int t0 = t + q.w * kRecTile, t1 = t0 - step;
         const int n = q.steps_at(t0);
-        const unsigned cut = cut_next;
+        const unsigned cut = reset_mask<false>(p, resets);
         float h[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) h[v] = h_next[v];
         const bool plain = n == kRecTile && cut == 0;
         saved_before(t1);
-        cut_next = t1 >= t_begin ? reset_mask<false>(p, q, t1, q.steps_at(t1)) : 0u;
+        resets = t1 >= t_begin ? resets_ahead<false>(p, q, t1, q.steps_at(t1)) : 0u;
         ring.bar(stage).wait(phase, given_up, status);
         const TmaTile<Raw> raw_g = {ring.words(stage, 0)}, raw_d = {ring.words(stage, 1)}, raw_x = {ring.words(stage, A - 1)};
         float code[kRecTile][VEC], slope[kRecTile][VEC];
