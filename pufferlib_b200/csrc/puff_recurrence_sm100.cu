@@ -379,10 +379,12 @@ puff_recurrence_kernel(RecArgs p, RecPlan plan, float2* pairs, T* __restrict__ o
         load_tile<Raw, VEC>(raw_g, p.gates, gates_at + t0 * p.gates_step_stride, p.gates_step_stride, q.steps_at(t0), q.ok);
         load_tile<Raw, VEC>(raw_x, p.inputs, inputs_at + t0 * p.inputs_step_stride, p.inputs_step_stride, q.steps_at(t0), q.ok);
     }
+    unsigned resets = resets_ahead<FLAT>(p, q, t0, q.steps_at(t0));
     int parity = 0;
     for (long long t = q.t_begin; t < q.t_end; t += step, t0 += step, parity ^= 1) {
         const int n = q.steps_at(t0);
-        const unsigned cut = reset_mask<FLAT>(p, resets_ahead<FLAT>(p, q, t0, n));
+        const unsigned cut = reset_mask<FLAT>(p, resets);
+        resets = resets_ahead<FLAT>(p, q, t0 + step, q.steps_at(t0 + step));
         const bool plain = n == kRecTile && !(FLAT ? __any_sync(0xffffffffu, cut != 0) : cut != 0);
         if (MODE == kStream) {
             Raw next_g[kRecTile], next_x[kRecTile];
@@ -530,9 +532,10 @@ puff_recurrence_backward_kernel(RecArgs p, RecPlan plan, float2* pairs, const fl
                 if (q.ok) carry[v] = apply_pair(pairs[r * lanes + q.index + v], carry[v]);
     const long long step = kRecTile * plan.warps;
     const long long gates_at = q.b * p.gates_batch_stride + q.c, inputs_at = q.b * p.inputs_batch_stride + q.c;
+    const long long last = q.t_begin + quotient(q.t_end > q.t_begin ? q.t_end - q.t_begin - 1 : 0, step) * step;
+    unsigned resets = resets_ahead<FLAT>(p, q, last + q.w * kRecTile, q.steps_at(last + q.w * kRecTile));
     int parity = 0;
-    for (long long t = q.t_begin + quotient(q.t_end > q.t_begin ? q.t_end - q.t_begin - 1 : 0, step) * step; t >= q.t_begin;
-         t -= step, parity ^= 1) {
+    for (long long t = last; t >= q.t_begin; t -= step, parity ^= 1) {
         const long long t0 = t + q.w * kRecTile;
         const int n = q.steps_at(t0);
         const long long at = (q.b * p.steps + t0) * p.channels + q.c;
@@ -545,7 +548,8 @@ puff_recurrence_backward_kernel(RecArgs p, RecPlan plan, float2* pairs, const fl
         if (MODE != kSummary)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) h[v] = q.ok && n > 0 ? saved[(q.b * tiles + t0 / kRecTile) * p.channels + q.c + v] : 0.0f;
-        const unsigned cut = reset_mask<FLAT>(p, resets_ahead<FLAT>(p, q, t0, n));
+        const unsigned cut = reset_mask<FLAT>(p, resets);
+        resets = t > q.t_begin ? resets_ahead<FLAT>(p, q, t0 - step, q.steps_at(t0 - step)) : 0u;
         const bool plain = n == kRecTile && !(FLAT ? __any_sync(0xffffffffu, cut != 0) : cut != 0);
         float code[kRecTile][VEC], slope[kRecTile][VEC];
         if (MODE == kSummary) {

@@ -6,14 +6,17 @@
 // checked, buffers allocated, and the C ABI of include/puff_advantage.h is called on the current stream of the
 // tensors' device.
 //
-// Each differentiable operator has an autograd kernel whose node keeps what the backward operator needs and calls it.
+// Each differentiable operator has an autograd kernel whose node keeps what the backward operator needs and calls it (nodes
+// of their own rather than torch::autograd::Function, whose context costs several microseconds a pass at the host).
 // The *_forward and *_backward operators can be called without autograd (for a program that captures a whole update
 // into a CUDA graph); their results are not differentiable, and a second derivative raises.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/all.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -27,7 +30,8 @@ namespace {
 
 using torch::Tensor;
 using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 void check_rc(int rc, const char* what)
@@ -67,6 +71,14 @@ struct BelowUnlessGraph {
     }
 };
 cudaStream_t current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+template <typename N> std::shared_ptr<N> new_node(torch::autograd::edge_list&& edges)
+{
+    std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+    node->set_next_edges(std::move(edges));
+    return node;
+}
+SavedVariable saved(const OptTensor& t) { return present(t) ? SavedVariable(*t, false) : SavedVariable(); }
 
 // ---- log-probabilities ------------------------------------------------------------------------------------------
 
@@ -210,29 +222,24 @@ Tensor logprobs_backward(const Tensor& logits, const Tensor& actions, double tem
     return op.call(logits, actions, temperature, row_stats, entropy, dlogprobs, dentropy);
 }
 
-struct LogprobsNode : public torch::autograd::Function<LogprobsNode> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& actions, double temperature,
-                                 bool want_entropy)
+struct LogprobsNode : public Node {
+    SavedVariable logits, actions, row_stats, entropy;
+    double temperature = 1.0;
+    std::string name() const override { return "PuffActionLogprobsBackward"; }
+    void release_variables() override
     {
-        at::AutoDispatchBelowADInplaceOrView below;
-        auto [logprobs, entropy, stats] = logprobs_forward(logits, actions, temperature, want_entropy, true);
-        ctx->set_materialize_grads(false);
-        if (!want_entropy) ctx->mark_non_differentiable({entropy});
-        ctx->save_for_backward({logits, actions, stats, entropy});
-        ctx->saved_data["temperature"] = temperature;
-        return {logprobs, entropy};
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable* v : {&logits, &actions, &row_stats, &entropy}) v->reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    variable_list apply(variable_list&& grads) override
     {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if ((!grads[0].defined() && !grads[1].defined()) || !task_should_compute_output(0)) return {Tensor()};
         const BelowUnlessGraph below;
-        const auto saved = ctx->get_saved_variables();
-        Tensor dlogits;
-        if (grads[0].defined() || grads[1].defined()) {
-            const Tensor dlp = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(grads[1], at::MemoryFormat::Contiguous);
-            const OptTensor dh = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
-            dlogits = logprobs_backward(saved[0], saved[1], ctx->saved_data["temperature"].toDouble(), saved[2], saved[3], dlp, dh);
-        }
-        return {dlogits, Tensor(), Tensor(), Tensor()};
+        const Tensor dlp = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(grads[1], at::MemoryFormat::Contiguous);
+        const OptTensor dh = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
+        return {logprobs_backward(logits.unpack(), actions.unpack(), temperature, row_stats.unpack(),
+                                  optional(entropy.unpack(shared_from_this())), dlp, dh)};
     }
 };
 std::tuple<Tensor, Tensor> action_logprobs_autograd(const Tensor& logits, const Tensor& actions, double temperature,
@@ -242,8 +249,21 @@ std::tuple<Tensor, Tensor> action_logprobs_autograd(const Tensor& logits, const 
         at::AutoDispatchBelowADInplaceOrView below;
         return action_logprobs(logits, actions, temperature, want_entropy);
     }
-    auto out = LogprobsNode::apply(logits, actions, temperature, want_entropy);
-    return {out[0], out[1]};
+    auto node = new_node<LogprobsNode>(torch::autograd::collect_next_edges(logits));
+    Tensor logprobs, entropy, stats;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        std::tie(logprobs, entropy, stats) = logprobs_forward(logits, actions, temperature, want_entropy, true);
+    }
+    torch::autograd::set_history(logprobs, node);
+    if (want_entropy) torch::autograd::set_history(entropy, node);
+    else node->add_input_metadata(Node::undefined_input());
+    node->logits = SavedVariable(logits, false);
+    node->actions = SavedVariable(actions, false);
+    node->row_stats = SavedVariable(stats, false);
+    if (want_entropy) node->entropy = SavedVariable(entropy, true);
+    node->temperature = temperature;
+    return {logprobs, entropy};
 }
 
 // ---- policy loss -------------------------------------------------------------------------------------------------
@@ -371,35 +391,24 @@ std::tuple<Tensor, Tensor> loss_backward(const Tensor& slope, const Tensor& row_
     return op.call(slope, row_scale, weight, dloss, mask, ent_coef, want_dentropy);
 }
 
-struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& logprobs, const Tensor& old_logprobs,
-                                 const Tensor& advantages, double clip_low, double clip_high,
-                                 const OptTensor& ref_logprobs, double kl_coef, const OptTensor& entropy, double ent_coef,
-                                 const OptTensor& mask, const std::string& reduction, double denominator)
+struct PolicyLossNode : public Node {
+    SavedVariable slope, row_scale, weight, mask;
+    double ent_coef = 0.0;
+    std::string name() const override { return "PuffPolicyLossBackward"; }
+    void release_variables() override
     {
-        at::AutoDispatchBelowADInplaceOrView below;
-        auto [loss, ratio, stats, slope, row_scale, weight] =
-            loss_forward(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy, ent_coef,
-                         mask, reduction, denominator, true);
-        ctx->mark_non_differentiable({ratio, stats});
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({slope, row_scale, weight, mask.value_or(Tensor())});
-        ctx->saved_data["ent_coef"] = ent_coef;
-        ctx->saved_data["dentropy"] = present(entropy) && entropy->requires_grad();
-        return {loss, ratio, stats};
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable* v : {&slope, &row_scale, &weight, &mask}) v->reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    variable_list apply(variable_list&& grads) override
     {
-        variable_list out(12);
-        if (!grads[0].defined()) return out;
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return {Tensor(), Tensor()};
         const BelowUnlessGraph below;
-        const auto saved = ctx->get_saved_variables();
-        const bool want_dentropy = ctx->saved_data["dentropy"].toBool();
-        auto [dlp, dent] = loss_backward(saved[0], saved[1], saved[2], grads[0], optional(saved[3]),
-                                         ctx->saved_data["ent_coef"].toDouble(), want_dentropy);
-        out[0] = dlp;
-        if (want_dentropy) out[7] = dent;
-        return out;
+        const bool want_dentropy = task_should_compute_output(1);
+        auto [dlogprobs, dentropy] = loss_backward(slope.unpack(), row_scale.unpack(), weight.unpack(), grads[0],
+                                                   optional(mask.unpack()), ent_coef, want_dentropy);
+        return {dlogprobs, want_dentropy ? dentropy : Tensor()};
     }
 };
 bool wants_grad(const OptTensor& t) { return present(t) && t->requires_grad(); }
@@ -417,9 +426,21 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor& logprobs, 
         return policy_loss(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
                            ent_coef, mask, reduction, denominator);
     }
-    auto out = PolicyLossNode::apply(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
-                                     ent_coef, mask, std::string(reduction), denominator);
-    return {out[0], out[1], out[2]};
+    auto node = new_node<PolicyLossNode>(torch::autograd::collect_next_edges(logprobs, entropy.value_or(Tensor())));
+    LossOut out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        out = loss_forward(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy, ent_coef,
+                           mask, reduction, denominator, true);
+    }
+    auto& [loss, ratio, stats, slope, row_scale, weight] = out;
+    torch::autograd::set_history(loss, node);
+    node->slope = SavedVariable(slope, false);
+    node->row_scale = SavedVariable(row_scale, false);
+    node->weight = SavedVariable(weight, false);
+    node->mask = saved(mask);
+    node->ent_coef = ent_coef;
+    return {loss, ratio, stats};
 }
 
 // ---- gated recurrence --------------------------------------------------------------------------------------------
@@ -533,30 +554,24 @@ RecOut recurrence_backward(const Tensor& gates, const Tensor& inputs, const OptT
     return op.call(gates, inputs, resets, saved, doutputs, dfinal);
 }
 
-struct RecurrenceNode : public torch::autograd::Function<RecurrenceNode> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& gates, const Tensor& inputs, const OptTensor& resets,
-                                 const OptTensor& state)
+struct RecurrenceNode : public Node {
+    SavedVariable gates, inputs, resets, states;
+    std::string name() const override { return "PuffGatedRecurrenceBackward"; }
+    void release_variables() override
     {
-        at::AutoDispatchBelowADInplaceOrView below;
-        auto [outputs, final_state, saved] = recurrence_forward(gates, inputs, resets, state, true);
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({gates, inputs, resets.value_or(Tensor()), saved});
-        ctx->saved_data["dstate"] = present(state) && state->requires_grad();
-        return {outputs, final_state};
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable* v : {&gates, &inputs, &resets, &states}) v->reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    variable_list apply(variable_list&& grads) override
     {
-        variable_list out(4);
-        if (!grads[0].defined() && !grads[1].defined()) return out;
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
         const BelowUnlessGraph below;
-        const auto saved = ctx->get_saved_variables();
         const OptTensor dout = grads[0].defined() ? OptTensor(grads[0].contiguous()) : std::nullopt;
         const OptTensor dfinal = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
-        auto [dgates, dinputs, dstate] = recurrence_backward(saved[0], saved[1], optional(saved[2]), saved[3], dout, dfinal);
-        out[0] = dgates;
-        out[1] = dinputs;
-        if (ctx->saved_data["dstate"].toBool()) out[3] = dstate;
-        return out;
+        auto [dgates, dinputs, dstate] = recurrence_backward(gates.unpack(), inputs.unpack(), optional(resets.unpack()),
+                                                             states.unpack(), dout, dfinal);
+        return {dgates, dinputs, dstate};
     }
 };
 std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor& gates, const Tensor& inputs, const OptTensor& resets,
@@ -566,8 +581,19 @@ std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor& gates, const 
         at::AutoDispatchBelowADInplaceOrView below;
         return gated_recurrence(gates, inputs, resets, state);
     }
-    auto out = RecurrenceNode::apply(gates, inputs, resets, state);
-    return {out[0], out[1]};
+    auto node = new_node<RecurrenceNode>(torch::autograd::collect_next_edges(gates, inputs, state.value_or(Tensor())));
+    Tensor outputs, final_state, states;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        std::tie(outputs, final_state, states) = recurrence_forward(gates, inputs, resets, state, true);
+    }
+    torch::autograd::set_history(outputs, node);
+    torch::autograd::set_history(final_state, node);
+    node->gates = SavedVariable(gates, false);
+    node->inputs = SavedVariable(inputs, false);
+    node->resets = saved(resets);
+    node->states = SavedVariable(states, false);
+    return {outputs, final_state};
 }
 
 void step_args(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, const Tensor& new_state)
