@@ -35,7 +35,7 @@ struct LossArgs {
     float* slope;
     float* row_scale;
     long long rows, steps;
-    float clip_low_value, clip_high_value;
+    float clip_low_value, clip_low_rest, clip_high_value, clip_high_rest;                     // 1 - clip_low, 1 + clip_high
     float log_low, log_low_rest, log_high, log_high_rest;   // log(1 - clip_low), log(1 + clip_high), 48 bits each
     float kl_coef;
 };
@@ -63,7 +63,7 @@ __device__ __forceinline__ float difference_rest(float a, float b, float d)
 }
 
 struct TokenLoss {
-    float policy, kl, excess, ratio, slope, d;
+    float policy, policy_rest, kl, excess, ratio, slope, d;
     bool clipped;
 };
 __device__ __forceinline__ TokenLoss token_loss(const LossArgs& p, float lp, float old, float adv, float ref)
@@ -74,7 +74,9 @@ __device__ __forceinline__ TokenLoss token_loss(const LossArgs& p, float lp, flo
     t.d = d;
     // the usual token: no exponential, e^d = 1 + (d + (e^d - 1 - d))
     t.excess = exp_excess(d);
-    t.ratio = 1.0f + (d + t.excess);
+    const float em1 = d + t.excess;
+    t.ratio = __fadd_rn(1.0f, em1);
+    float ratio_rest = __fsub_rn(em1, __fsub_rn(t.ratio, 1.0f));
     if (!(fabsf(d) < 0.5f) || d == p.log_high || d == p.log_low) {
         const float rest = difference_rest(lp, old, d);
         above = above || (d == p.log_high && rest > p.log_high_rest);
@@ -82,10 +84,15 @@ __device__ __forceinline__ TokenLoss token_loss(const LossArgs& p, float lp, flo
         const float e = expf(d);
         // beyond 80 the exponential is 0, infinite, or the rest does not matter
         t.ratio = fabsf(d) < 80.0f ? fmaf(e, rest, e) : e;
+        ratio_rest = 0.0f;
         if (!(fabsf(d) < 1.0f)) t.excess = (t.ratio - 1.0f) - d;
     }
     const bool cut = (above && adv > 0.0f) || (below && adv < 0.0f);
-    t.policy = -adv * (cut ? (above ? p.clip_high_value : p.clip_low_value) : t.ratio);
+    // the policy term as a rounded product and its error: the terms of a batch nearly cancel, their rounding does not
+    const float held = cut ? (above ? p.clip_high_value : p.clip_low_value) : t.ratio;
+    const float held_rest = cut ? (above ? p.clip_high_rest : p.clip_low_rest) : ratio_rest;
+    t.policy = __fmul_rn(-adv, held);
+    t.policy_rest = fmaf(-adv, held_rest, fmaf(-adv, held, -t.policy));
     t.slope = cut ? 0.0f : t.policy;
     t.clipped = above || below;
     t.kl = 0.0f;
@@ -126,8 +133,13 @@ template <> struct Pack<4> {
 
 // Sums over a few tokens in fp32, joined in fp64; numbers of tokens are whole
 struct LossSums {
-    float policy, kl, entropy, neg_d, excess;
+    float policy, policy_rest, kl, entropy, neg_d, excess;
 };
+// an infinite or NaN term has no rest
+__device__ __forceinline__ double policy_sum(const LossSums& s)
+{
+    return static_cast<double>(s.policy) + (fabsf(s.policy) < CUDART_INF_F ? static_cast<double>(s.policy_rest) : 0.0);
+}
 struct LossTotals {
     double policy, kl, entropy, neg_d, excess;
     int clipped, tokens, rows;
@@ -159,7 +171,9 @@ __device__ __forceinline__ void add_tokens(const LossArgs& p, long long i, long 
             const TokenLoss t = token_loss(p, lp[v], old[v], adv[v], ref[v]);
             ratio[v] = t.ratio;
             slope[v] = t.slope;
-            sums.policy += t.policy;
+            const float sum = __fadd_rn(sums.policy, t.policy), back = __fsub_rn(sum, sums.policy);
+            sums.policy_rest += t.policy_rest + (__fsub_rn(sums.policy, __fsub_rn(sum, back)) + __fsub_rn(t.policy, back));
+            sums.policy = sum;
             sums.kl += t.kl;
             sums.entropy += ent[v];
             sums.neg_d -= t.d;
@@ -203,7 +217,7 @@ puff_policy_loss_kernel(LossArgs p, double* __restrict__ partial)
     for (long long u = blockIdx.x * static_cast<long long>(kLossThreads) + threadIdx.x; u < units; u += stride) {
         LossSums sums = {};
         add_tokens<VEC, false>(p, u * VEC, u * VEC, sums, total.clipped, total.tokens);
-        total.policy += sums.policy;
+        total.policy += policy_sum(sums);
         total.kl += sums.kl;
         total.entropy += sums.entropy;
         total.neg_d += sums.neg_d;
@@ -235,7 +249,7 @@ puff_policy_loss_rows_kernel(LossArgs p, double* __restrict__ partial)
                 LossSums sums = {};
                 const long long i = r * p.steps + u * VEC;
                 add_tokens<VEC, ONE_ADVANTAGE>(p, i, ONE_ADVANTAGE ? r : i, sums, total.clipped, length);
-                policy += sums.policy;
+                policy += policy_sum(sums);
                 kl += sums.kl;
                 entropy += sums.entropy;
                 total.neg_d += sums.neg_d;
@@ -425,7 +439,9 @@ extern "C" int puff_policy_sm100_loss(const float* logprobs, const float* old_lo
     p.rows = n > 0 ? rows : 0;
     p.steps = steps;
     p.clip_low_value = static_cast<float>(1.0 - clip_low);
+    p.clip_low_rest = static_cast<float>((1.0 - clip_low) - p.clip_low_value);
     p.clip_high_value = static_cast<float>(1.0 + clip_high);
+    p.clip_high_rest = clip_high < 1e30 ? static_cast<float>((1.0 + clip_high) - p.clip_high_value) : 0.0f;
     const double low = clip_low < 1.0 ? log1p(-clip_low) : -HUGE_VAL, high = log1p(clip_high);
     p.log_low = static_cast<float>(low);
     p.log_low_rest = clip_low < 1.0 ? static_cast<float>(low - p.log_low) : 0.0f;

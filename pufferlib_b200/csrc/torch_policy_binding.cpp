@@ -146,24 +146,28 @@ LogprobArgs logprob_args(const Tensor& logits, const Tensor& actions)
     return g;
 }
 
-// (logprobs, entropy or an empty tensor, row_stats or an empty tensor)
+// (logprobs, entropy or an empty tensor, row_stats or an empty tensor; undefined tensors for those with `bare`)
+std::tuple<Tensor, Tensor, Tensor> logprobs_buffers(const Tensor& logits, const Tensor& actions, double temperature,
+                                                    bool want_entropy, bool save, bool bare)
+{
+    TORCH_CHECK(temperature > 0, "temperature must be positive");
+    const auto opts = logits.options().dtype(torch::kFloat32);
+    return {torch::empty(actions.sizes(), opts),
+            want_entropy ? torch::empty(actions.sizes(), opts) : bare ? Tensor() : torch::empty({0}, opts),
+            save ? torch::empty({actions.numel(), 2}, opts) : bare ? Tensor() : torch::empty({0, 2}, opts)};
+}
 std::tuple<Tensor, Tensor, Tensor> logprobs_forward_meta(const Tensor& logits, const Tensor& actions, double temperature,
                                                          bool want_entropy, bool save)
 {
     logprob_args(logits, actions);
-    TORCH_CHECK(temperature > 0, "temperature must be positive");
-    const auto opts = logits.options().dtype(torch::kFloat32);
-    Tensor logprobs = torch::empty(actions.sizes(), opts);
-    Tensor entropy = torch::empty(want_entropy ? actions.sizes() : at::IntArrayRef({0}), opts);
-    Tensor stats = torch::empty({save ? actions.numel() : 0, 2}, opts);
-    return {logprobs, entropy, stats};
+    return logprobs_buffers(logits, actions, temperature, want_entropy, save, false);
 }
-std::tuple<Tensor, Tensor, Tensor> logprobs_forward_cuda(const Tensor& logits, const Tensor& actions, double temperature,
-                                                         bool want_entropy, bool save)
+std::tuple<Tensor, Tensor, Tensor> logprobs_run(const Tensor& logits, const Tensor& actions, double temperature,
+                                                bool want_entropy, bool save, bool bare)
 {
     const LogprobArgs g = logprob_args(logits, actions);
     const c10::cuda::CUDAGuard guard(logits.device());
-    auto out = logprobs_forward_meta(logits, actions, temperature, want_entropy, save);
+    auto out = logprobs_buffers(logits, actions, temperature, want_entropy, save, bare);
     if (g.rows == 0) return out;
     check_rc(puff_policy_sm100_logprobs(logits.data_ptr(), g.dtype, ptr<const long long>(actions), g.l.outer, g.l.inner,
                                         g.vocab, g.l.outer_stride, g.l.inner_stride, g.a.outer_stride, g.a.inner_stride,
@@ -172,6 +176,11 @@ std::tuple<Tensor, Tensor, Tensor> logprobs_forward_cuda(const Tensor& logits, c
                                         save ? ptr<float>(std::get<2>(out)) : nullptr, current_stream()),
              "puff_action_logprobs");
     return out;
+}
+std::tuple<Tensor, Tensor, Tensor> logprobs_forward_cuda(const Tensor& logits, const Tensor& actions, double temperature,
+                                                         bool want_entropy, bool save)
+{
+    return logprobs_run(logits, actions, temperature, want_entropy, save, false);
 }
 std::tuple<Tensor, Tensor, Tensor> logprobs_forward(const Tensor& logits, const Tensor& actions, double temperature,
                                                     bool want_entropy, bool save)
@@ -182,8 +191,9 @@ std::tuple<Tensor, Tensor, Tensor> logprobs_forward(const Tensor& logits, const 
 }
 std::tuple<Tensor, Tensor> action_logprobs(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
 {
-    auto out = logprobs_forward(logits, actions, temperature, want_entropy, false);
-    return {std::get<0>(out), std::get<1>(out)};
+    auto [logprobs, entropy, stats] = logits.is_cuda() ? logprobs_run(logits, actions, temperature, want_entropy, false, true)
+                                                       : logprobs_forward(logits, actions, temperature, want_entropy, false);
+    return {logprobs, entropy.defined() ? entropy : torch::empty({0}, logprobs.options())};
 }
 
 Tensor logprobs_backward_meta(const Tensor& logits, const Tensor& actions, double, const Tensor&, const OptTensor&,
@@ -299,29 +309,33 @@ bool loss_args(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor&
 }
 
 using LossOut = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
-// (loss, ratio, stats, slope, row_scale, weight); the last three hold nothing unless `save`
+// (loss, ratio, stats, slope, row_scale, weight); the last three hold nothing unless `save` (undefined with `bare`)
+LossOut loss_buffers(const Tensor& logprobs, bool sequence, bool save, bool bare)
+{
+    const auto opts = logprobs.options();
+    auto kept = [&](bool there, at::IntArrayRef sizes) {
+        return there ? torch::empty(sizes, opts) : bare ? Tensor() : torch::empty({0}, opts);
+    };
+    return {torch::empty({}, opts), torch::empty(logprobs.sizes(), opts), torch::empty({6}, opts), kept(save, logprobs.sizes()),
+            kept(save && sequence, {logprobs.size(0)}), kept(save, {1})};
+}
 LossOut loss_forward_meta(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
                           double clip_high, const OptTensor& ref_logprobs, double, const OptTensor& entropy, double,
                           const OptTensor& mask, c10::string_view reduction, double denominator, bool save)
 {
     loss_args(logprobs, old_logprobs, advantages, ref_logprobs, entropy, mask, clip_low, clip_high, denominator);
-    const bool sequence = reduction_code(reduction) == PUFF_MEAN_SEQUENCES;
-    const auto opts = logprobs.options();
-    return {torch::empty({}, opts), torch::empty(logprobs.sizes(), opts), torch::empty({6}, opts),
-            torch::empty(save ? logprobs.sizes() : at::IntArrayRef({0}), opts),
-            torch::empty({save && sequence ? logprobs.size(0) : 0}, opts), torch::empty({save ? 1 : 0}, opts)};
+    return loss_buffers(logprobs, reduction_code(reduction) == PUFF_MEAN_SEQUENCES, save, false);
 }
-LossOut loss_forward_cuda(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
+LossOut loss_run(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
                           double clip_high, const OptTensor& ref_logprobs, double kl_coef, const OptTensor& entropy,
-                          double ent_coef, const OptTensor& mask, c10::string_view reduction, double denominator, bool save)
+                 double ent_coef, const OptTensor& mask, c10::string_view reduction, double denominator, bool save, bool bare)
 {
     const bool per_row = loss_args(logprobs, old_logprobs, advantages, ref_logprobs, entropy, mask, clip_low, clip_high, denominator);
     const c10::cuda::CUDAGuard guard(logprobs.device());
-    LossOut out = loss_forward_meta(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
-                                    ent_coef, mask, reduction, denominator, save);
+    const bool sequence = reduction_code(reduction) == PUFF_MEAN_SEQUENCES;
+    LossOut out = loss_buffers(logprobs, sequence, save, bare);
     auto& [loss, ratio, stats, slope, row_scale, weight] = out;
     const int64_t rows = logprobs.size(0), steps = logprobs.size(1);
-    const bool sequence = reduction_code(reduction) == PUFF_MEAN_SEQUENCES;
     const size_t sbytes = puff_policy_sm100_loss_scratch_bytes(rows, steps);
     Tensor scratch = torch::empty({static_cast<int64_t>((sbytes + 7) / 8)}, logprobs.options().dtype(torch::kFloat64));
     check_rc(puff_policy_sm100_loss(ptr<const float>(logprobs), ptr<const float>(old_logprobs), ptr<const float>(advantages),
@@ -333,6 +347,13 @@ LossOut loss_forward_cuda(const Tensor& logprobs, const Tensor& old_logprobs, co
                                     save ? ptr<float>(weight) : nullptr, scratch.data_ptr(), sbytes, current_stream()),
              "puff_policy_loss");
     return out;
+}
+LossOut loss_forward_cuda(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
+                          double clip_high, const OptTensor& ref_logprobs, double kl_coef, const OptTensor& entropy,
+                          double ent_coef, const OptTensor& mask, c10::string_view reduction, double denominator, bool save)
+{
+    return loss_run(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy, ent_coef, mask,
+                    reduction, denominator, save, false);
 }
 LossOut loss_forward(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
                      double clip_high, const OptTensor& ref_logprobs, double kl_coef, const OptTensor& entropy,
@@ -348,8 +369,10 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logprobs, const Ten
                                                double kl_coef, const OptTensor& entropy, double ent_coef,
                                                const OptTensor& mask, c10::string_view reduction, double denominator)
 {
-    LossOut out = loss_forward(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
-                               ent_coef, mask, reduction, denominator, false);
+    LossOut out = logprobs.is_cuda() ? loss_run(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef,
+                                                entropy, ent_coef, mask, reduction, denominator, false, true)
+                                     : loss_forward(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef,
+                                                    entropy, ent_coef, mask, reduction, denominator, false);
     return {std::get<0>(out), std::get<1>(out), std::get<2>(out)};
 }
 
