@@ -415,64 +415,44 @@ __device__ __forceinline__ float logit_gradient(float x, const RowGradient& g)
     return p * (ENT ? fmaf(g.b, fmaxf(t, -1e4f), g.a) : g.a);
 }
 
-// Backward of rows beyond the small kernel's: a warp takes 128 16-byte vectors of a row of dlogits (contiguous).  The
+// Backward of rows beyond the small kernel's: a warp takes 256 16-byte vectors of a row of dlogits (contiguous).  The
 // vectors are those of the output; where the row of logits lies at another offset from a 16-byte boundary, a vector is
 // cut out of the two aligned ones that hold it.  The first warp of a row also does the elements at its ends.
-constexpr int kLpUnitVecs = 4;      // vectors a lane
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(kLpThreads, 4)
-puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions,
-                              RowMap amap, long long rows, long long vocab, int warps_per_row, unsigned ctas_per_row,
-                              float inv_temperature, const float2* __restrict__ row_stats, const float* __restrict__ entropy,
-                              const float* __restrict__ dlogprobs, const float* __restrict__ dentropy,
-                              T* __restrict__ dlogits)
+struct GradientRow {
+    const uint4* in;
+    uint4* to;
+    long long head, nvec, action;
+    unsigned shift;
+    bool none;
+};
+// vectors first, first + 32, ... of the row, U of them; 4 x 131072 rows: eight at once 337 us, four 369; shifted ones need
+// twice the registers, and eight of those spill (143 us against 94 for 2040 x 50001)
+template <typename T, bool ENT, int U, bool SHIFTED>
+__device__ __forceinline__ void gradient_vectors(const GradientRow& row, const RowGradient& grad, long long first)
 {
     constexpr int N = Vec16<T>::N;
-    const int lane = threadIdx.x & 31;
-    // 8 / warps_per_row rows a CTA, or ctas_per_row CTAs a row
-    const unsigned block_row = blockIdx.x / ctas_per_row;
-    const int warp = threadIdx.x >> 5;
-    const long long r = static_cast<long long>(block_row) * (kLpWarps / warps_per_row) + warp / warps_per_row;
-    if (r >= rows) return;
-    const long long chunk = (blockIdx.x - block_row * ctas_per_row) * kLpWarps + warp % warps_per_row;
-    const long long action = actions[amap.at(r)];
-    const float2 st = row_stats[r];
-    const float dlp = dlogprobs[r], dh = ENT ? dentropy[r] : 0.0f, h = ENT ? entropy[r] : 0.0f;
-    const T* row = logits + lmap.at(r);
-    T* out = dlogits + r * vocab;
-    const bool none = action < 0 || action >= vocab || (st.x == -CUDART_INF_F && st.y == 0.0f);
-    const RowGradient grad = row_gradient<T, ENT>(st.x, st.y, h, dlp, dh, inv_temperature);
     const float2 a2 = make_float2(grad.a, grad.a), b2 = make_float2(grad.b, grad.b);
     const float2 c2 = make_float2(grad.c, grad.c), l2 = make_float2(-grad.l, -grad.l);
-    // vectors [0, nvec) start at element `head` of the row; shift: how far behind a boundary the logits' bytes lie
-    long long head = static_cast<long long>(((16u - (reinterpret_cast<uintptr_t>(out) & 15u)) & 15u) / sizeof(T));
-    const unsigned shift = static_cast<unsigned>(reinterpret_cast<uintptr_t>(row + head) & 15u);
-    if (shift != 0 && head * static_cast<long long>(sizeof(T)) < shift) head += N;   // the aligned vector would start before the row
-    long long nvec = shift == 0 ? (vocab - head) / N : ((vocab - head) * static_cast<long long>(sizeof(T)) + shift) / 16 - 1;
-    if (nvec < 0) nvec = 0;
-    const uint4* in = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row + head) & ~static_cast<uintptr_t>(15));
-    uint4* to = reinterpret_cast<uint4*>(out + head);
-    const long long first = chunk * (32 * kLpUnitVecs) + lane;
-    uint4 q[kLpUnitVecs];
-    if (!none) {
+    uint4 q[U];
+    if (!row.none) {
 #pragma unroll
-        for (int k = 0; k < kLpUnitVecs; ++k)
-            if (first + 32 * k < nvec) q[k] = __ldg(in + first + 32 * k);
-        if (shift != 0) {
-            uint4 next[kLpUnitVecs];
+        for (int k = 0; k < U; ++k)
+            if (first + 32 * k < row.nvec) q[k] = __ldg(row.in + first + 32 * k);
+        if (SHIFTED) {
+            uint4 next[U];
 #pragma unroll
-            for (int k = 0; k < kLpUnitVecs; ++k)
-                if (first + 32 * k < nvec) next[k] = __ldg(in + first + 32 * k + 1);
+            for (int k = 0; k < U; ++k)
+                if (first + 32 * k < row.nvec) next[k] = __ldg(row.in + first + 32 * k + 1);
 #pragma unroll
-            for (int k = 0; k < kLpUnitVecs; ++k) q[k] = cut_vector(q[k], next[k], shift);
+            for (int k = 0; k < U; ++k) q[k] = cut_vector(q[k], next[k], row.shift);
         }
     }
 #pragma unroll
-    for (int k = 0; k < kLpUnitVecs; ++k) {
+    for (int k = 0; k < U; ++k) {
         const long long i = first + 32 * k;
-        if (i >= nvec) break;
+        if (i >= row.nvec) break;
         float f[N];
-        if (none) {
+        if (row.none) {
 #pragma unroll
             for (int v = 0; v < N; ++v) f[v] = 0.0f;
         } else {
@@ -491,25 +471,67 @@ puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const l
                     f[v + 1] = d.y;
                 }
             }
-            const long long at = action - (head + i * N);
+            const long long at = row.action - (row.head + i * N);
             if (at >= 0 && at < N) {                         // the chosen one is among these
 #pragma unroll
                 for (int v = 0; v < N; ++v) f[v] += at == v ? grad.dlp : 0.0f;
             }
         }
-        to[i] = Vec16<T>::pack(f);
+        row.to[i] = Vec16<T>::pack(f);
+    }
+}
+
+constexpr int kLpUnitVecs = 8;      // vectors a lane
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kLpThreads, 4)
+puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions,
+                              RowMap amap, long long rows, long long vocab, int warps_per_row, unsigned ctas_per_row,
+                              float inv_temperature, const float2* __restrict__ row_stats, const float* __restrict__ entropy,
+                              const float* __restrict__ dlogprobs, const float* __restrict__ dentropy,
+                              T* __restrict__ dlogits)
+{
+    constexpr int N = Vec16<T>::N;
+    const int lane = threadIdx.x & 31;
+    // 8 / warps_per_row rows a CTA, or ctas_per_row CTAs a row
+    const unsigned block_row = blockIdx.x / ctas_per_row;
+    const int warp = threadIdx.x >> 5;
+    const long long r = static_cast<long long>(block_row) * (kLpWarps / warps_per_row) + warp / warps_per_row;
+    if (r >= rows) return;
+    const long long chunk = (blockIdx.x - block_row * ctas_per_row) * kLpWarps + warp % warps_per_row;
+    GradientRow g;
+    g.action = actions[amap.at(r)];
+    const float2 st = row_stats[r];
+    const float dlp = dlogprobs[r], dh = ENT ? dentropy[r] : 0.0f, h = ENT ? entropy[r] : 0.0f;
+    const T* row = logits + lmap.at(r);
+    T* out = dlogits + r * vocab;
+    g.none = g.action < 0 || g.action >= vocab || (st.x == -CUDART_INF_F && st.y == 0.0f);
+    const RowGradient grad = row_gradient<T, ENT>(st.x, st.y, h, dlp, dh, inv_temperature);
+    // vectors [0, nvec) start at element `head` of the row; shift: how far behind a boundary the logits' bytes lie
+    g.head = static_cast<long long>(((16u - (reinterpret_cast<uintptr_t>(out) & 15u)) & 15u) / sizeof(T));
+    g.shift = static_cast<unsigned>(reinterpret_cast<uintptr_t>(row + g.head) & 15u);
+    if (g.shift != 0 && g.head * static_cast<long long>(sizeof(T)) < g.shift) g.head += N;   // the aligned vector would start before the row
+    g.nvec = g.shift == 0 ? (vocab - g.head) / N : ((vocab - g.head) * static_cast<long long>(sizeof(T)) + g.shift) / 16 - 1;
+    if (g.nvec < 0) g.nvec = 0;
+    g.in = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row + g.head) & ~static_cast<uintptr_t>(15));
+    g.to = reinterpret_cast<uint4*>(out + g.head);
+    const long long first = chunk * (32 * kLpUnitVecs) + lane;
+    if (g.shift == 0) {
+        gradient_vectors<T, ENT, kLpUnitVecs, false>(g, grad, first);
+    } else {
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) gradient_vectors<T, ENT, kLpUnitVecs / 2, true>(g, grad, first + part * (16 * kLpUnitVecs));
     }
     if (chunk == 0) {
-        const long long tail = head + nvec * N;
-        for (long long j = lane; j < head + (vocab - tail); j += 32) {
-            const long long e = j < head ? j : tail + (j - head);
+        const long long tail = g.head + g.nvec * N;
+        for (long long j = lane; j < g.head + (vocab - tail); j += 32) {
+            const long long e = j < g.head ? j : tail + (j - g.head);
             if (e >= vocab) break;
-            float g = 0.0f;
-            if (!none) {
-                g = logit_gradient<ENT>(to_f32(row[e]), grad);
-                if (e == action) g += grad.dlp;
+            float d = 0.0f;
+            if (!g.none) {
+                d = logit_gradient<ENT>(to_f32(row[e]), grad);
+                if (e == g.action) d += grad.dlp;
             }
-            out[e] = from_f32<T>(g);
+            out[e] = from_f32<T>(d);
         }
     }
 }
