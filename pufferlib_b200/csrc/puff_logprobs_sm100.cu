@@ -586,23 +586,37 @@ puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long
         }
     }
     __syncthreads();
-    // ---- the sums of this thread's row
+    // ---- the sums of this thread's row, element by element from `start` on and around the end
     constexpr int kBankElems = 128 / sizeof(T);
     const int skew = G == 1 ? (sizeof(T) == 4 ? 1 - (vocab & 1) : (2 - vocab) & 3)
                             : ((G * (kBankElems / 32) - vocab) & (kBankElems - 1));
     const int start = (local * skew) % vocab;
-    T* row = tile + local * vocab;
+    T* const row = tile + local * vocab;
+    T* const wrapped = row - vocab;
+    // (one loop with a select: as two loops, up to the end and from the beginning, lanes diverge and it takes twice as long)
+    auto each = [&](auto&& f) {
+        if (live)
+#pragma unroll 4
+            for (int j = start + g; j < start + vocab; j += G) f((j < vocab ? row : wrapped)[j]);
+    };
     const float c = inv_temperature * kLog2e;
+    const float chosen = live ? to_f32(row[action]) : 0.0f;
     SoftSums a = {-CUDART_INF_F, 0.0f, 0.0f};
-    if (live) {
-        int j = start + g;
-        for (int k = g; k < vocab; k += G, j += G) a.m = fmaxf(a.m, to_f32(row[j < vocab ? j : j - vocab]));
-    }
+    each([&](T& x) { a.m = fmaxf(a.m, to_f32(x)); });
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(0xffffffffu, a.m, o));
-    if (live) {
-        int j = start + g;
-        for (int k = g; k < vocab; k += G, j += G) soft_add<ENT>(a, to_f32(row[j < vocab ? j : j - vocab]), c);
+    const SoftScale z = soft_scale<T>(a.m, c);
+    if (z.direct) {
+        each([&](T& x) { soft_add<ENT>(a, to_f32(x), c); });
+    } else {
+        float s = 0.0f, u = 0.0f;
+        each([&](T& x) {
+            const float t = fmaf(to_f32(x), c, -z.sc), e = exp2_approx(t);
+            s += e;
+            if (ENT) u = fmaf(e, fmaxf(t, -1e4f), u);
+        });
+        a.s = s * z.k;
+        if (ENT) a.u = fmaf(-z.d, s, u) * z.k;
     }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) {
@@ -611,28 +625,33 @@ puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long
     }
     if (!BACKWARD) {
         if (has && g == 0) {
-            if (live) write_row<ENT>(out, r0 + local, a, to_f32(row[action]), inv_temperature);
+            if (live) write_row<ENT>(out, r0 + local, a, chosen, inv_temperature);
             else write_padding<ENT>(out, r0 + local, action >= vocab);
         }
         return;
     }
-    // ---- gradients over the logits
-    if (has) {
-        const bool none = !live || (a.m == -CUDART_INF_F && a.s == 0.0f);
-        const float log_s = none ? 0.0f : logf(a.s);
-        const float h = ENT && !none ? log_s - kLn2 * (a.u / a.s) : 0.0f;
+    // ---- gradients over the logits; the chosen one's is written again, with its own term
+    const bool none = !live || (a.m == -CUDART_INF_F && a.s == 0.0f);
+    float d_chosen = 0.0f;
+    if (none) {
+        if (has)
+            for (int k = g; k < vocab; k += G) row[k] = from_f32<T>(0.0f);
+    } else {
+        const float log_s = logf(a.s);
+        const float h = ENT ? log_s - kLn2 * (a.u / a.s) : 0.0f;
         const RowGradient grad = row_gradient<T, ENT>(a.m, log_s, h, dlp, dh, inv_temperature);
-        int j = start + g;
-        for (int k = g; k < vocab; k += G, j += G) {
-            const int e = j < vocab ? j : j - vocab;
-            float d = 0.0f;
-            if (!none) {
-                d = logit_gradient<ENT>(to_f32(row[e]), grad);
-                if (e == action) d += grad.dlp;
-            }
-            row[e] = from_f32<T>(d);
+        if (grad.direct) {
+            each([&](T& x) { x = from_f32<T>(logit_gradient<ENT>(to_f32(x), grad)); });
+        } else {
+            each([&](T& x) {
+                const float t = fmaf(to_f32(x), grad.c, -grad.l);
+                x = from_f32<T>(exp2_approx(t) * (ENT ? fmaf(grad.b, fmaxf(t, -1e4f), grad.a) : grad.a));
+            });
         }
+        d_chosen = logit_gradient<ENT>(chosen, grad) + grad.dlp;
     }
+    __syncwarp();
+    if (!none && g == 0) row[action] = from_f32<T>(d_chosen);
     __syncthreads();
     // ---- out
     T* dst = dlogits + r0 * vocab;
