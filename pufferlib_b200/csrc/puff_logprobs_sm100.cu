@@ -693,9 +693,10 @@ static cudaError_t launch_logprobs(const void* logits, RowMap lmap, const long l
                                    long long vocab, float inv_t, float* logprobs, float* entropy, float* row_stats,
                                    cudaStream_t st)
 {
+    if (vocab <= kLpSmall)      // its backward pass works the statistics out again
+        return launch_small<T, ENT, false>(logits, lmap, actions, amap, rows, vocab, inv_t, LogprobOut{logprobs, entropy, nullptr},
+                                           nullptr, nullptr, nullptr, st);
     const LogprobOut out = {logprobs, entropy, reinterpret_cast<float2*>(row_stats)};
-    if (vocab <= kLpSmall)
-        return launch_small<T, ENT, false>(logits, lmap, actions, amap, rows, vocab, inv_t, out, nullptr, nullptr, nullptr, st);
     const T* z = static_cast<const T*>(logits);
     const long long bytes = vocab * static_cast<long long>(sizeof(T));
     // a warp a row while rows are short and many enough to give every SM sixteen warps

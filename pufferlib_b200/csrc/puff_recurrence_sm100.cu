@@ -775,17 +775,17 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
     const bool flat = rec_flat(channels, 1);
     const ViewStrides gs = {gates_batch_stride, gates_step_stride}, xs = {inputs_batch_stride, inputs_step_stride};
     const ViewStrides dense = {steps * channels, channels};
-    const bool tma = tma_shape(p, size) && tma_view(p, gates, gs, size) && tma_view(p, inputs, xs, size) && tma_view(p, outputs, dense, size);
+    CUtensorMap mg, mx, mo;
+    const bool tma = tma_shape(p, size) && tma_view(p, gates, gs, size) && tma_view(p, inputs, xs, size) &&
+                     tma_view(p, outputs, dense, size) && tma_map(&mg, p, gates, gs, dtype) && tma_map(&mx, p, inputs, xs, dtype) &&
+                     tma_map(&mo, p, outputs, dense, dtype);
     const RecPlan plan = rec_plan(batch, steps, channels, tma ? 4 / size : pair ? 2 : 1, flat);
     float2* pairs = static_cast<float2*>(scratch);
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
     if (tma) {
-        CUtensorMap mg, mx, mo;
         int* status = device_status_ptr();
-        if (status == nullptr || !tma_map(&mg, p, gates, gs, dtype) || !tma_map(&mx, p, inputs, xs, dtype) ||
-            !tma_map(&mo, p, outputs, dense, dtype))
-            return PUFF_ERR_DRIVER;
+        if (status == nullptr) return PUFF_ERR_DRIVER;
 #define PUFF_RUN2(T, VEC)                                                                                                \
     rec_launch(plan.splits > 1 ? puff_recurrence_tma_kernel<T, VEC, kSummary> : nullptr,                                  \
                plan.warps > 1 ? puff_recurrence_tma_kernel<T, VEC, kTeam> : puff_recurrence_tma_kernel<T, VEC, kStream>,  \
@@ -846,18 +846,18 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
     const bool flat = rec_flat(channels, 1);
     const ViewStrides gs = {gates_batch_stride, gates_step_stride}, xs = {inputs_batch_stride, inputs_step_stride};
     const ViewStrides dense = {steps * channels, channels};
+    CUtensorMap mg, mx, md, mdg, mdx;
     const bool tma = tma_shape(p, size) && tma_view(p, gates, gs, size) && tma_view(p, inputs, xs, size) &&
-                     tma_view(p, doutputs, dense, size) && tma_view(p, dgates, dense, size) && tma_view(p, dinputs, dense, size);
+                     tma_view(p, doutputs, dense, size) && tma_view(p, dgates, dense, size) && tma_view(p, dinputs, dense, size) &&
+                     tma_map(&mg, p, gates, gs, dtype) && tma_map(&mx, p, inputs, xs, dtype) && tma_map(&md, p, doutputs, dense, dtype) &&
+                     tma_map(&mdg, p, dgates, dense, dtype) && tma_map(&mdx, p, dinputs, dense, dtype);
     const RecPlan plan = rec_plan(batch, steps, channels, tma ? 4 / size : pair ? 2 : 1, flat);
     float2* pairs = static_cast<float2*>(scratch);
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
     if (tma) {
-        CUtensorMap mg, mx, md, mdg, mdx;
         int* status = device_status_ptr();
-        if (status == nullptr || !tma_map(&mg, p, gates, gs, dtype) || !tma_map(&mx, p, inputs, xs, dtype) ||
-            !tma_map(&md, p, doutputs, dense, dtype) || !tma_map(&mdg, p, dgates, dense, dtype) || !tma_map(&mdx, p, dinputs, dense, dtype))
-            return PUFF_ERR_DRIVER;
+        if (status == nullptr) return PUFF_ERR_DRIVER;
 #define PUFF_RUN2(T, VEC)                                                                                                \
     rec_launch(plan.splits > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kSummary> : nullptr,                         \
                plan.warps > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kTeam>                                        \

@@ -189,11 +189,21 @@ std::tuple<Tensor, Tensor, Tensor> logprobs_forward(const Tensor& logits, const 
                          .typed<decltype(logprobs_forward_meta)>();
     return op.call(logits, actions, temperature, want_entropy, save);
 }
+std::tuple<Tensor, Tensor> action_logprobs_cuda(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
+{
+    auto [logprobs, entropy, stats] = logprobs_run(logits, actions, temperature, want_entropy, false, true);
+    return {logprobs, entropy.defined() ? entropy : torch::empty({0}, logprobs.options())};
+}
+std::tuple<Tensor, Tensor> action_logprobs_meta(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
+{
+    auto out = logprobs_forward_meta(logits, actions, temperature, want_entropy, false);
+    return {std::get<0>(out), std::get<1>(out)};
+}
 std::tuple<Tensor, Tensor> action_logprobs(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
 {
-    auto [logprobs, entropy, stats] = logits.is_cuda() ? logprobs_run(logits, actions, temperature, want_entropy, false, true)
-                                                       : logprobs_forward(logits, actions, temperature, want_entropy, false);
-    return {logprobs, entropy.defined() ? entropy : torch::empty({0}, logprobs.options())};
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_action_logprobs", "")
+                         .typed<decltype(action_logprobs_meta)>();
+    return op.call(logits, actions, temperature, want_entropy);
 }
 
 Tensor logprobs_backward_meta(const Tensor& logits, const Tensor& actions, double, const Tensor&, const OptTensor&,
@@ -364,16 +374,33 @@ LossOut loss_forward(const Tensor& logprobs, const Tensor& old_logprobs, const T
     return op.call(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy, ent_coef, mask,
                    reduction, denominator, save);
 }
+std::tuple<Tensor, Tensor, Tensor> policy_loss_cuda(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages,
+                                                    double clip_low, double clip_high, const OptTensor& ref_logprobs,
+                                                    double kl_coef, const OptTensor& entropy, double ent_coef,
+                                                    const OptTensor& mask, c10::string_view reduction, double denominator)
+{
+    LossOut out = loss_run(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy, ent_coef,
+                           mask, reduction, denominator, false, true);
+    return {std::get<0>(out), std::get<1>(out), std::get<2>(out)};
+}
+std::tuple<Tensor, Tensor, Tensor> policy_loss_meta(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages,
+                                                    double clip_low, double clip_high, const OptTensor& ref_logprobs,
+                                                    double kl_coef, const OptTensor& entropy, double ent_coef,
+                                                    const OptTensor& mask, c10::string_view reduction, double denominator)
+{
+    LossOut out = loss_forward_meta(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy,
+                                    ent_coef, mask, reduction, denominator, false);
+    return {std::get<0>(out), std::get<1>(out), std::get<2>(out)};
+}
 std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages,
                                                double clip_low, double clip_high, const OptTensor& ref_logprobs,
                                                double kl_coef, const OptTensor& entropy, double ent_coef,
                                                const OptTensor& mask, c10::string_view reduction, double denominator)
 {
-    LossOut out = logprobs.is_cuda() ? loss_run(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef,
-                                                entropy, ent_coef, mask, reduction, denominator, false, true)
-                                     : loss_forward(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef,
-                                                    entropy, ent_coef, mask, reduction, denominator, false);
-    return {std::get<0>(out), std::get<1>(out), std::get<2>(out)};
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pufferlib::puff_policy_loss", "")
+                         .typed<decltype(policy_loss_meta)>();
+    return op.call(logprobs, old_logprobs, advantages, clip_low, clip_high, ref_logprobs, kl_coef, entropy, ent_coef, mask,
+                   reduction, denominator);
 }
 
 // (dlogprobs, dentropy or an empty tensor)
@@ -673,10 +700,10 @@ TORCH_LIBRARY_FRAGMENT(pufferlib, m)
 
 TORCH_LIBRARY_IMPL(pufferlib, CUDA, m)
 {
-    m.impl("puff_action_logprobs", &action_logprobs);
+    m.impl("puff_action_logprobs", &action_logprobs_cuda);
     m.impl("puff_action_logprobs_forward", &logprobs_forward_cuda);
     m.impl("puff_action_logprobs_backward", &logprobs_backward_cuda);
-    m.impl("puff_policy_loss", &policy_loss);
+    m.impl("puff_policy_loss", &policy_loss_cuda);
     m.impl("puff_policy_loss_forward", &loss_forward_cuda);
     m.impl("puff_policy_loss_backward", &loss_backward_cuda);
     m.impl("puff_gated_recurrence", &gated_recurrence);
@@ -687,10 +714,10 @@ TORCH_LIBRARY_IMPL(pufferlib, CUDA, m)
 
 TORCH_LIBRARY_IMPL(pufferlib, Meta, m)
 {
-    m.impl("puff_action_logprobs", &action_logprobs);
+    m.impl("puff_action_logprobs", &action_logprobs_meta);
     m.impl("puff_action_logprobs_forward", &logprobs_forward_meta);
     m.impl("puff_action_logprobs_backward", &logprobs_backward_meta);
-    m.impl("puff_policy_loss", &policy_loss);
+    m.impl("puff_policy_loss", &policy_loss_meta);
     m.impl("puff_policy_loss_forward", &loss_forward_meta);
     m.impl("puff_policy_loss_backward", &loss_backward_meta);
     m.impl("puff_gated_recurrence", &gated_recurrence);

@@ -363,7 +363,10 @@ def check_recurrence(gates, x, resets, state, seed=0, use=(True, True)):
 
 @pytest.mark.parametrize("shape", [(1, 1, 1), (1, 2, 3), (2, 15, 8), (3, 16, 16), (2, 17, 33), (1, 31, 64), (4, 32, 130), (2, 33, 31),
                                    (1, 100, 256), (5, 64, 65), (2, 127, 128), (1, 128, 7), (1, 129, 500), (3, 257, 96),
-                                   (1, 1000, 32), (1, 2049, 40), (2, 513, 1030), (200, 20, 24), (2, 5003, 2)])
+                                   (1, 1000, 32), (1, 2049, 40), (2, 513, 1030), (200, 20, 24), (2, 5003, 2),
+                                   # rows of a multiple of 16 bytes: tiles at every edge of steps, channels and rounds
+                                   (3, 1, 64), (2, 5, 32), (5, 16, 40), (3, 48, 72), (2, 130, 200), (1, 777, 1024),
+                                   (1, 4097, 64), (3, 2100, 96), (700, 33, 64), (70000, 2, 32)])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_recurrence_shapes(shape, dtype):
     check_recurrence(*rec_inputs(*shape, dtype, seed=sum(shape)))
@@ -600,6 +603,13 @@ def test_operators_on_side_streams():
                 got.append(update(pb, weights, *data)[0].detach())
     torch.cuda.synchronize()
     assert all(torch.equal(v, want) for v in got)
+
+
+def test_no_wait_has_given_up():
+    """The bounded waits of the kernels above all ended with their data."""
+    from pufferlib_b200 import cabi
+    check_recurrence(*rec_inputs(3, 300, 64, BF16, seed=30))
+    assert cabi.device_status() == 0
 
 
 def test_second_derivatives_are_refused():
