@@ -191,8 +191,9 @@ std::tuple<Tensor, Tensor, Tensor> logprobs_forward(const Tensor& logits, const 
 }
 std::tuple<Tensor, Tensor> action_logprobs_cuda(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
 {
+    // without entropy an undefined tensor, None in Python: an empty one would cost a tenth of a small call
     auto [logprobs, entropy, stats] = logprobs_run(logits, actions, temperature, want_entropy, false, true);
-    return {logprobs, entropy.defined() ? entropy : torch::empty({0}, logprobs.options())};
+    return {logprobs, entropy};
 }
 std::tuple<Tensor, Tensor> action_logprobs_meta(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
 {

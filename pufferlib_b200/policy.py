@@ -9,7 +9,17 @@ is missing.  No second derivatives.
 """
 import torch
 
-from .advantage import _ops
+from .advantage import _ops as _load_ops
+
+_loaded = None
+
+
+def _ops():
+    """torch.ops.pufferlib, looked up once: these calls are made for every generated token."""
+    global _loaded
+    if _loaded is None:
+        _loaded = _load_ops()
+    return _loaded
 
 
 def action_logprobs(logits, actions, temperature=1.0, entropy=True):
