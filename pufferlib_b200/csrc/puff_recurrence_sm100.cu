@@ -8,6 +8,11 @@
 // The recurrent layer of a policy over the experience buffers' [segments, horizon] rows, cut where an episode ends
 // (`terminals`, pufferl.py:295) as the recurrent state of pufferl.py:112-117 is; the same first-order linear
 // recurrence as the advantages, with gates for discounts.  The state is carried in fp32 whatever the tensors' type.
+//
+// Memory-bound: three elements moved a step forward, five backward; the arithmetic behind them, two special functions and
+// some twenty instructions a step for two channels, is close to the bound, so what surrounds it (addresses, joins, waits)
+// decides.  8192 x 64 x 128 bf16: 76 us forward (5.3 TB/s of 6.55) and 117 backward (5.7); fp32 125 and 211 (6.4);
+// 256 x 4096 x 128 fp32 281 and 453.  One thread a channel, step after step, took 1904 us for the first pair.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
