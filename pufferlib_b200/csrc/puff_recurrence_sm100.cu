@@ -13,6 +13,7 @@
 // some twenty instructions a step for two channels, is close to the bound, so what surrounds it (addresses, joins, waits)
 // decides.  8192 x 64 x 128 bf16: 76 us forward (5.3 TB/s of 6.55) and 117 backward (5.7); fp32 125 and 211 (6.4);
 // 256 x 4096 x 128 fp32 281 and 453.  One thread a channel, step after step, took 1904 us for the first pair.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -40,8 +41,10 @@ struct RecArgs {
 // go to different CTAs where lanes are few.  A tile (or range) maps the state before it to the state after it as
 // h -> A h + B; those pairs are joined over the warps through shared memory, and over the ranges through global memory
 // by a first launch that computes nothing else.
+// Where TMA moves the tiles, a cluster of `shares` CTAs can take consecutive parts of a round instead: it joins its pairs
+// through distributed shared memory and reads everything once.
 struct RecPlan {
-    int warps, splits;
+    int warps, splits, shares;
     long long split_steps, lane_blocks, blocks_per_row;
 };
 
@@ -170,6 +173,7 @@ __device__ __forceinline__ long long quotient(long long a, long long b)
 struct RecPlace {
     int group, w, lane;
     bool unit, ok;             // the group has work; this lane has a channel
+    int slot;                  // this warp among those of its group, or of its cluster
     int split;
     long long b, c, index;     // index: b * channels + c
     long long t_begin, t_end;
@@ -187,7 +191,9 @@ __device__ __forceinline__ RecPlace rec_place(const RecArgs& p, const RecPlan& p
     q.lane = threadIdx.x & 31;
     q.group = warp / plan.warps;
     q.w = warp - q.group * plan.warps;
-    const long long unit = blockIdx.x * static_cast<long long>(kRecWarps / plan.warps) + q.group;
+    const unsigned shared_by = static_cast<unsigned>(plan.shares), block_id = blockIdx.x / shared_by;
+    q.slot = q.w + static_cast<int>(blockIdx.x - block_id * shared_by) * plan.warps;
+    const long long unit = block_id * static_cast<long long>(kRecWarps / plan.warps) + q.group;
     q.split = plan.splits == 1 && unit < plan.lane_blocks ? 0 : static_cast<int>(quotient(unit, plan.lane_blocks));
     const long long block = unit - q.split * plan.lane_blocks;
     q.unit = q.split < plan.splits;
@@ -348,7 +354,56 @@ __device__ __forceinline__ void join_warps(float2 (*s_pair)[VEC][32], const RecP
 
 // STREAM: one warp a group, tile after tile, the next one's loads under this one's arithmetic.  TEAM: the warps of a group
 // take a tile each.  SUMMARY: as TEAM, only the pairs of the ranges.
-enum RecMode { kStream, kTeam, kSummary };
+// CLUSTER: as TEAM, by all warps of a cluster.
+enum RecMode { kStream, kTeam, kSummary, kCluster };
+
+// the pair of x, then y
+__device__ __forceinline__ float2 then_pair(float2 x, float2 y)
+{
+    if (y.x < 0.0f) return y;
+    return make_float2(x.x < 0.0f ? -1.0f : x.x * y.x, fmaf(y.x, x.y, y.y));
+}
+// As join_warps for a cluster whose CTAs have one group each: the warps' pairs within the CTA first, then the CTAs' through
+// s_cta, into which every CTA writes its own at all the others.  s_pair is free again after the cluster's barrier, s_cta
+// (written from outside) only after the next one: the caller alternates between two.
+template <int VEC, bool REVERSE>
+__device__ __forceinline__ void join_cluster(float2 (*s_pair)[VEC][32], float2 (*s_cta)[VEC][32], const RecPlace& q, const RecPlan& plan,
+                                             unsigned cut, const float (&a)[VEC], const float (&b)[VEC], float (&h)[VEC], float (&carry)[VEC])
+{
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int rank = static_cast<int>(cluster.block_rank());
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) s_pair[q.w][v][q.lane] = make_float2(cut != 0 ? -1.0f : a[v], b[v]);
+    __syncthreads();
+    float2 before[VEC], all[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) before[v] = all[v] = make_float2(1.0f, 0.0f);
+    for (int i = 0; i < kRecWarps; ++i) {
+        const int w = REVERSE ? kRecWarps - 1 - i : i;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            if (w == q.w) before[v] = all[v];
+            all[v] = then_pair(all[v], s_pair[w][v][q.lane]);
+        }
+    }
+    if (q.w < plan.shares) {       // warp k tells CTA k
+        float2* to = cluster.map_shared_rank(&s_cta[rank][0][q.lane], q.w);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) to[32 * v] = all[v];
+    }
+    cluster.sync();
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) h[v] = carry[v];
+    for (int i = 0; i < plan.shares; ++i) {
+        const int k = REVERSE ? plan.shares - 1 - i : i;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            if (k == rank) h[v] = apply_pair(before[v], carry[v]);
+            carry[v] = apply_pair(s_cta[k][v][q.lane], carry[v]);
+        }
+    }
+}
 
 // Forward.  saved (nullable): the state before steps 0, 16, 32, ... as [batch, ceil(steps / 16), channels].
 template <typename T, int VEC, bool FLAT, RecMode MODE>
@@ -652,6 +707,7 @@ constexpr int kRecMaxSplits = 148;
 static RecPlan rec_plan(long long batch, long long steps, long long channels, int vec, bool flat)
 {
     RecPlan plan;
+    plan.shares = 1;
     plan.blocks_per_row = (channels + 32 * vec - 1) / (32 * vec);
     plan.lane_blocks = flat ? (batch * channels + 31) / 32 : batch * plan.blocks_per_row;
     const long long tiles = (steps + kRecTile - 1) / kRecTile;
@@ -697,6 +753,39 @@ static cudaError_t rec_launch(void (*summary)(KArgs...), void (*kernel)(KArgs...
     if (e != cudaSuccess) return e;
     count_launch();
     return launch_neighbour(kernel, grid, kRecThreads, smem, st, args...);
+}
+// One launch of clusters of plan.shares CTAs
+template <typename... KArgs, typename... Args>
+static cudaError_t rec_launch_cluster(void (*kernel)(KArgs...), size_t smem, const RecPlan& plan, cudaStream_t st, const Args&... args)
+{
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(plan.lane_blocks * plan.shares));
+    cfg.blockDim = dim3(kRecThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(plan.shares);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+// Turns ranges into clusters of two or four where those fill most of one wave.  Measured, ranges / clusters, us forward, bf16:
+// 256 CTAs 4 x 8192 x 1024 92 / 70, 280 140 x 3000 x 64 77 / 55, 192 3 x 4000 x 1024 42 / 39, but 160 5 x 10000 x 1024 138 /
+// 150, and clusters of eight, which do not all find room at once, 1 x 20000 x 2368 112 / 136.
+static RecPlan with_cluster(RecPlan plan, long long steps)
+{
+    if (plan.splits == 1) return plan;
+    const int shares = plan.lane_blocks * 4 <= kRecSlots ? 4 : 2;
+    if (plan.lane_blocks * shares > kRecSlots || plan.lane_blocks * shares < 190 || steps < 2LL * shares * kRecWarps * kRecTile) return plan;
+    plan.shares = shares;
+    plan.splits = 1;
+    plan.split_steps = steps;
+    return plan;
 }
 // channels too few to fill half a warp's lanes: rows share warps
 static bool rec_flat(long long channels, int vec) { return channels < 16 * vec; }
@@ -784,7 +873,8 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
     const bool tma = tma_shape(p, size) && tma_view(p, gates, gs, size) && tma_view(p, inputs, xs, size) &&
                      tma_view(p, outputs, dense, size) && tma_map(&mg, p, gates, gs, dtype) && tma_map(&mx, p, inputs, xs, dtype) &&
                      tma_map(&mo, p, outputs, dense, dtype);
-    const RecPlan plan = rec_plan(batch, steps, channels, tma ? 4 / size : pair ? 2 : 1, flat);
+    RecPlan plan = rec_plan(batch, steps, channels, tma ? 4 / size : pair ? 2 : 1, flat);
+    if (tma) plan = with_cluster(plan, steps);
     float2* pairs = static_cast<float2*>(scratch);
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
@@ -792,9 +882,10 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
         int* status = device_status_ptr();
         if (status == nullptr) return PUFF_ERR_DRIVER;
 #define PUFF_RUN2(T, VEC)                                                                                                \
+    (plan.shares > 1 ? rec_launch_cluster(puff_recurrence_tma_kernel<T, VEC, kCluster>, tma_smem(2, kTmaForwardStages), plan, st, mg, mx, mo, p, plan, pairs, final_state, saved, status) : \
     rec_launch(plan.splits > 1 ? puff_recurrence_tma_kernel<T, VEC, kSummary> : nullptr,                                  \
                plan.warps > 1 ? puff_recurrence_tma_kernel<T, VEC, kTeam> : puff_recurrence_tma_kernel<T, VEC, kStream>,  \
-               tma_smem(2, kTmaForwardStages), plan, st, mg, mx, mo, p, plan, pairs, final_state, saved, status)
+               tma_smem(2, kTmaForwardStages), plan, st, mg, mx, mo, p, plan, pairs, final_state, saved, status))
         e = dtype == PUFF_DTYPE_F32 ? PUFF_RUN2(float, 1) : dtype == PUFF_DTYPE_F16 ? PUFF_RUN2(__half, 2) : PUFF_RUN2(__nv_bfloat16, 2);
 #undef PUFF_RUN2
         return static_cast<int>(e);
@@ -856,7 +947,8 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
                      tma_view(p, doutputs, dense, size) && tma_view(p, dgates, dense, size) && tma_view(p, dinputs, dense, size) &&
                      tma_map(&mg, p, gates, gs, dtype) && tma_map(&mx, p, inputs, xs, dtype) && tma_map(&md, p, doutputs, dense, dtype) &&
                      tma_map(&mdg, p, dgates, dense, dtype) && tma_map(&mdx, p, dinputs, dense, dtype);
-    const RecPlan plan = rec_plan(batch, steps, channels, tma ? 4 / size : pair ? 2 : 1, flat);
+    RecPlan plan = rec_plan(batch, steps, channels, tma ? 4 / size : pair ? 2 : 1, flat);
+    if (tma) plan = with_cluster(plan, steps);
     float2* pairs = static_cast<float2*>(scratch);
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t e;
@@ -864,10 +956,11 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
         int* status = device_status_ptr();
         if (status == nullptr) return PUFF_ERR_DRIVER;
 #define PUFF_RUN2(T, VEC)                                                                                                \
+    (plan.shares > 1 ? rec_launch_cluster(puff_recurrence_backward_tma_kernel<T, VEC, kCluster>, tma_smem(3, kTmaBackwardStages), plan, st, mg, mx, md, mdg, mdx, p, plan, pairs, saved, dfinal, dstate, status) : \
     rec_launch(plan.splits > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kSummary> : nullptr,                         \
                plan.warps > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kTeam>                                        \
                               : puff_recurrence_backward_tma_kernel<T, VEC, kStream>,                                     \
-               tma_smem(3, kTmaBackwardStages), plan, st, mg, mx, md, mdg, mdx, p, plan, pairs, saved, dfinal, dstate, status)
+               tma_smem(3, kTmaBackwardStages), plan, st, mg, mx, md, mdg, mdx, p, plan, pairs, saved, dfinal, dstate, status))
         e = dtype == PUFF_DTYPE_F32 ? PUFF_RUN2(float, 1) : dtype == PUFF_DTYPE_F16 ? PUFF_RUN2(__half, 2) : PUFF_RUN2(__nv_bfloat16, 2);
 #undef PUFF_RUN2
         return static_cast<int>(e);

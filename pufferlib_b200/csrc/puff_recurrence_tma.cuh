@@ -105,7 +105,8 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
     using Raw = typename Lane<T, VEC>::Raw;
     constexpr int S = kTmaForwardStages;
     extern __shared__ char s_ring[];
-    __shared__ float2 s_pair[MODE == kStream ? 1 : 2][MODE == kStream ? 1 : kRecWarps][VEC][32];
+    __shared__ float2 s_pair[MODE == kStream || MODE == kCluster ? 1 : 2][MODE == kStream ? 1 : kRecWarps][VEC][32];
+    __shared__ float2 s_cta[MODE == kCluster ? 2 : 1][MODE == kCluster ? 4 : 1][VEC][32];
     const RecPlace q = rec_place<VEC, false>(p, plan);
     const TileRing<2, S> ring(s_ring);
     ring.init();
@@ -113,14 +114,14 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
     if (!q.unit) return;
     const long long lanes = p.batch * p.channels;
     const long long tiles = (p.steps + kRecTile - 1) / kRecTile;
-    const int step = kRecTile * plan.warps, c0 = static_cast<int>(q.c) - q.lane * VEC, b0 = static_cast<int>(q.b);
+    const int step = kRecTile * plan.warps * plan.shares, c0 = static_cast<int>(q.c) - q.lane * VEC, b0 = static_cast<int>(q.b);
     const int t_end = static_cast<int>(q.t_end), t_begin = static_cast<int>(q.t_begin);
     auto request = [&](int t, int stage) {      // the tile of this warp in the round that begins at t
         if (q.lane == 0 && t < t_end) {
             const TileBarrier bar = ring.bar(stage);
             bar.expect(2 * kTmaTileBytes);
-            tile_load(ring.at(stage, 0), &gates, c0, t + q.w * kRecTile, b0, bar);
-            tile_load(ring.at(stage, 1), &inputs, c0, t + q.w * kRecTile, b0, bar);
+            tile_load(ring.at(stage, 0), &gates, c0, t + q.slot * kRecTile, b0, bar);
+            tile_load(ring.at(stage, 1), &inputs, c0, t + q.slot * kRecTile, b0, bar);
         }
     };
     request(t_begin, 0);
@@ -131,7 +132,7 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
         carry[v] = MODE != kSummary && q.ok && p.state != nullptr ? p.state[q.index + v] : 0.0f;
         sum_a[v] = 1.0f;
     }
-    long long t0 = q.t_begin + q.w * kRecTile;
+    long long t0 = q.t_begin + q.slot * kRecTile;
     unsigned resets = resets_ahead<false>(p, q, t0, q.steps_at(t0));
     if (MODE == kTeam)
         for (int r = 0; r < q.split; ++r)
@@ -162,8 +163,9 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
             float keep[kRecTile][VEC], fresh[kRecTile][VEC], a[VEC], b[VEC], h[VEC];
             if (plain) forward_pair<T, VEC, true>(raw_g, raw_x, cut, n, keep, fresh, a, b);
             else forward_pair<T, VEC, false>(raw_g, raw_x, cut, n, keep, fresh, a, b);
-            join_warps<VEC, MODE == kSummary, false>(s_pair[parity], q, plan.warps, cut, a, b, h, carry, sum_a);
-            if (MODE == kTeam) {
+            if constexpr (MODE == kCluster) join_cluster<VEC, false>(s_pair[0], s_cta[parity], q, plan, cut, a, b, h, carry);
+            else join_warps<VEC, MODE == kSummary, false>(s_pair[parity], q, plan.warps, cut, a, b, h, carry, sum_a);
+            if (MODE != kSummary) {
                 if (save != nullptr && q.ok && n > 0)
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) save[v] = h[v];
@@ -178,11 +180,11 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
             tile_store(&outputs, c0, static_cast<int>(t0), b0, ring.at(stage, 1));
             tile_store_commit();
         }
-        if (save != nullptr) save += plan.warps * p.channels;
+        if (save != nullptr) save += step / kRecTile * p.channels;
         stage = stage == S - 1 ? 0 : stage + 1;
         phase ^= stage == 0 ? 1u : 0u;
     }
-    if (q.ok && q.w == 0) {
+    if (q.ok && q.slot == 0) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             if (MODE == kSummary) pairs[q.split * lanes + q.index + v] = make_float2(sum_a[v], carry[v]);
@@ -206,7 +208,8 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
     using Raw = typename L::Raw;
     constexpr int S = kTmaBackwardStages, A = MODE == kSummary ? 2 : 3;      // gates, doutputs, inputs
     extern __shared__ char s_ring[];
-    __shared__ float2 s_pair[MODE == kStream ? 1 : 2][MODE == kStream ? 1 : kRecWarps][VEC][32];
+    __shared__ float2 s_pair[MODE == kStream || MODE == kCluster ? 1 : 2][MODE == kStream ? 1 : kRecWarps][VEC][32];
+    __shared__ float2 s_cta[MODE == kCluster ? 2 : 1][MODE == kCluster ? 4 : 1][VEC][32];
     const RecPlace q = rec_place<VEC, false>(p, plan);
     const TileRing<A, S> ring(s_ring);
     ring.init();
@@ -214,16 +217,16 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
     if (!q.unit) return;
     const long long lanes = p.batch * p.channels;
     const long long tiles = (p.steps + kRecTile - 1) / kRecTile;
-    const int step = kRecTile * plan.warps, c0 = static_cast<int>(q.c) - q.lane * VEC, b0 = static_cast<int>(q.b);
+    const int step = kRecTile * plan.warps * plan.shares, c0 = static_cast<int>(q.c) - q.lane * VEC, b0 = static_cast<int>(q.b);
     const int t_begin = static_cast<int>(q.t_begin);
     const int first = t_begin + (static_cast<int>(q.t_end) - t_begin - 1) / step * step;
     auto request = [&](int t, int stage) {
         if (q.lane == 0 && t >= t_begin) {
             const TileBarrier bar = ring.bar(stage);
             bar.expect(A * kTmaTileBytes);
-            tile_load(ring.at(stage, 0), &gates, c0, t + q.w * kRecTile, b0, bar);
-            if (MODE != kSummary) tile_load(ring.at(stage, A - 1), &inputs, c0, t + q.w * kRecTile, b0, bar);
-            tile_load(ring.at(stage, 1), &doutputs, c0, t + q.w * kRecTile, b0, bar);
+            tile_load(ring.at(stage, 0), &gates, c0, t + q.slot * kRecTile, b0, bar);
+            if (MODE != kSummary) tile_load(ring.at(stage, A - 1), &inputs, c0, t + q.slot * kRecTile, b0, bar);
+            tile_load(ring.at(stage, 1), &doutputs, c0, t + q.slot * kRecTile, b0, bar);
         }
     };
     request(first, 0);
@@ -239,8 +242,8 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
         for (int v = 0; v < VEC; ++v)
             h_next[v] = MODE != kSummary && q.ok && at >= q.t_begin && at < q.t_end ? saved[(q.b * tiles + at / kRecTile) * p.channels + q.c + v] : 0.0f;
     };
-    saved_before(first + q.w * kRecTile);
-    unsigned resets = resets_ahead<false>(p, q, first + q.w * kRecTile, q.steps_at(first + q.w * kRecTile));
+    saved_before(first + q.slot * kRecTile);
+    unsigned resets = resets_ahead<false>(p, q, first + q.slot * kRecTile, q.steps_at(first + q.slot * kRecTile));
     if (MODE == kTeam)
         for (int r = plan.splits - 1; r > q.split; --r)
 #pragma unroll
@@ -250,7 +253,7 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
     uint32_t phase = 0;
     bool given_up = false;
     for (int t = first; t >= t_begin; t -= step) {
-        const int t0 = t + q.w * kRecTile, t1 = t0 - step;
+        const int t0 = t + q.slot * kRecTile, t1 = t0 - step;
         const int n = q.steps_at(t0);
         const unsigned cut = reset_mask<false>(p, resets);
         float h[VEC];
@@ -286,7 +289,8 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
             float a[VEC], b[VEC];
             if (plain) backward_pair<T, VEC, true>(code, raw_d, cut, a, b);
             else backward_pair<T, VEC, false>(code, raw_d, cut, a, b);
-            join_warps<VEC, MODE == kSummary, true>(s_pair[stage], q, plan.warps, cut, a, b, lam, carry, sum_a);
+            if constexpr (MODE == kCluster) join_cluster<VEC, true>(s_pair[0], s_cta[stage], q, plan, cut, a, b, lam, carry);
+            else join_warps<VEC, MODE == kSummary, true>(s_pair[stage], q, plan.warps, cut, a, b, lam, carry, sum_a);
         }
         if (MODE != kSummary) {
             float (&l)[VEC] = MODE == kStream ? carry : lam;
@@ -306,7 +310,7 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
         stage ^= 1;
         phase ^= stage == 0 ? 1u : 0u;
     }
-    if (q.ok && q.w == 0) {
+    if (q.ok && q.slot == 0) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             if (MODE == kSummary) pairs[q.split * lanes + q.index + v] = make_float2(sum_a[v], carry[v]);
