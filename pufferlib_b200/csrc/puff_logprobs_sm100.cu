@@ -352,6 +352,9 @@ puff_logprobs_cta_kernel(const T* __restrict__ logits, RowMap lmap, const long l
     const VectorRing ring = {s_ring + threadIdx.x};
     const float c = inv_temperature * kLog2e;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // the first CTA's shared memory may be written only once that CTA runs: all arrive here, and wait before the first write
+    bool waited = shares == 1;
+    if (!waited) cluster.barrier_arrive();
     for (long long r = blockIdx.x / shares; r < rows; r += gridDim.x / shares) {
         const long long action = actions[amap.at(r)];
         const bool none = action < 0 || action >= vocab;
@@ -365,6 +368,8 @@ puff_logprobs_cta_kernel(const T* __restrict__ logits, RowMap lmap, const long l
         soft_warp_join<ENT>(a, c);
         if (lane == 0) s_part[warp] = a;
         __syncthreads();
+        if (!waited) cluster.barrier_wait();
+        waited = true;
         if (warp == 0) {
             a = lane < kLpWarps ? s_part[lane] : SoftSums{-CUDART_INF_F, 0.0f, 0.0f};
             soft_warp_join<ENT>(a, c);
@@ -386,6 +391,7 @@ puff_logprobs_cta_kernel(const T* __restrict__ logits, RowMap lmap, const long l
             __syncthreads();
         }
     }
+    if (!waited) cluster.barrier_wait();
 }
 
 // The gradient of a row's logits as p (A + B t) with t = log2 p: A = -(dlp + dh H) / temperature, B = -dh ln 2 /
@@ -771,7 +777,7 @@ static int check_logprobs(const void* logits, int dtype, const long long* action
     if (!(temperature > 0.0f) || temperature > 3.0e38f || 1.5f / temperature > 3.0e38f) return PUFF_ERR_VALUE;
     if (outer == 0 || inner == 0) return PUFF_OK;
     if (vocab == 0) return PUFF_ERR_SHAPE;
-    if (inner > (1LL << 40) / outer) return PUFF_ERR_SIZE;
+    if (inner > (1LL << 40) / outer || vocab > (1LL << 46) / (outer * inner)) return PUFF_ERR_SIZE;
     if (logits == nullptr || actions == nullptr) return PUFF_ERR_NULL;
     if (misaligned(logits, size) || misaligned(actions, 8)) return PUFF_ERR_ALIGN;
     *rows = outer * inner;

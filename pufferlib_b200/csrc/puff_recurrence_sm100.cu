@@ -798,8 +798,8 @@ static int check_recurrence(const RecArgs& p, int dtype)
         p.inputs_batch_stride < 0 || p.inputs_step_stride < 0)
         return PUFF_ERR_SHAPE;
     if (p.resets != nullptr && p.reset_bytes != 1 && p.reset_bytes != 4) return PUFF_ERR_DTYPE;
-    const long long lanes = p.batch * p.channels;
     if (p.batch > 0 && p.channels > (1LL << 36) / p.batch) return PUFF_ERR_SIZE;
+    const long long lanes = p.batch * p.channels;
     if (lanes > 0 && p.steps > (1LL << 40) / lanes) return PUFF_ERR_SIZE;
     if (misaligned(p.gates, size) || misaligned(p.inputs, size) || misaligned(p.state, 4) ||
         (p.reset_bytes == 4 && misaligned(p.resets, 4)))

@@ -58,6 +58,13 @@ __device__ __forceinline__ void tile_fence()
     __syncwarp();
 }
 
+// every CTA of the cluster has begun: their shared memory may be written
+__device__ __forceinline__ void cluster_runs()
+{
+    __syncwarp();
+    cooperative_groups::this_cluster().sync();
+}
+
 // a lane's word of every step of a tile
 template <typename Raw>
 struct TmaTile {
@@ -126,6 +133,7 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
     };
     request(t_begin, 0);
     request(t_begin + step, 1);
+    if (MODE == kCluster) cluster_runs();
     float carry[VEC], sum_a[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
@@ -231,6 +239,7 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
     };
     request(first, 0);
     request(first - step, 1);
+    if (MODE == kCluster) cluster_runs();
     float carry[VEC], sum_a[VEC], h_next[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
