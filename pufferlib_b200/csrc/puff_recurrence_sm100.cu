@@ -881,11 +881,14 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
     if (tma) {
         int* status = device_status_ptr();
         if (status == nullptr) return PUFF_ERR_DRIVER;
+        const size_t smem = tma_smem(2, kTmaForwardStages);
 #define PUFF_RUN2(T, VEC)                                                                                                \
-    (plan.shares > 1 ? rec_launch_cluster(puff_recurrence_tma_kernel<T, VEC, kCluster>, tma_smem(2, kTmaForwardStages), plan, st, mg, mx, mo, p, plan, pairs, final_state, saved, status) : \
-    rec_launch(plan.splits > 1 ? puff_recurrence_tma_kernel<T, VEC, kSummary> : nullptr,                                  \
-               plan.warps > 1 ? puff_recurrence_tma_kernel<T, VEC, kTeam> : puff_recurrence_tma_kernel<T, VEC, kStream>,  \
-               tma_smem(2, kTmaForwardStages), plan, st, mg, mx, mo, p, plan, pairs, final_state, saved, status))
+    (plan.shares > 1                                                                                                     \
+         ? rec_launch_cluster(puff_recurrence_tma_kernel<T, VEC, kCluster>, smem, plan, st, mg, mx, mo, p, plan, pairs,   \
+                              final_state, saved, status)                                                                \
+         : rec_launch(plan.splits > 1 ? puff_recurrence_tma_kernel<T, VEC, kSummary> : nullptr,                           \
+                      plan.warps > 1 ? puff_recurrence_tma_kernel<T, VEC, kTeam> : puff_recurrence_tma_kernel<T, VEC, kStream>, \
+                      smem, plan, st, mg, mx, mo, p, plan, pairs, final_state, saved, status))
         e = dtype == PUFF_DTYPE_F32 ? PUFF_RUN2(float, 1) : dtype == PUFF_DTYPE_F16 ? PUFF_RUN2(__half, 2) : PUFF_RUN2(__nv_bfloat16, 2);
 #undef PUFF_RUN2
         return static_cast<int>(e);
@@ -955,12 +958,15 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
     if (tma) {
         int* status = device_status_ptr();
         if (status == nullptr) return PUFF_ERR_DRIVER;
+        const size_t smem = tma_smem(3, kTmaBackwardStages);
 #define PUFF_RUN2(T, VEC)                                                                                                \
-    (plan.shares > 1 ? rec_launch_cluster(puff_recurrence_backward_tma_kernel<T, VEC, kCluster>, tma_smem(3, kTmaBackwardStages), plan, st, mg, mx, md, mdg, mdx, p, plan, pairs, saved, dfinal, dstate, status) : \
-    rec_launch(plan.splits > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kSummary> : nullptr,                         \
-               plan.warps > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kTeam>                                        \
-                              : puff_recurrence_backward_tma_kernel<T, VEC, kStream>,                                     \
-               tma_smem(3, kTmaBackwardStages), plan, st, mg, mx, md, mdg, mdx, p, plan, pairs, saved, dfinal, dstate, status))
+    (plan.shares > 1                                                                                                     \
+         ? rec_launch_cluster(puff_recurrence_backward_tma_kernel<T, VEC, kCluster>, smem, plan, st, mg, mx, md, mdg, mdx, \
+                              p, plan, pairs, saved, dfinal, dstate, status)                                             \
+         : rec_launch(plan.splits > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kSummary> : nullptr,                  \
+                      plan.warps > 1 ? puff_recurrence_backward_tma_kernel<T, VEC, kTeam>                                 \
+                                     : puff_recurrence_backward_tma_kernel<T, VEC, kStream>,                              \
+                      smem, plan, st, mg, mx, md, mdg, mdx, p, plan, pairs, saved, dfinal, dstate, status))
         e = dtype == PUFF_DTYPE_F32 ? PUFF_RUN2(float, 1) : dtype == PUFF_DTYPE_F16 ? PUFF_RUN2(__half, 2) : PUFF_RUN2(__nv_bfloat16, 2);
 #undef PUFF_RUN2
         return static_cast<int>(e);
@@ -968,8 +974,9 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
 #define PUFF_RUN2(T, VEC, FLAT)                                                                                          \
     rec_launch(plan.splits > 1 ? puff_recurrence_backward_kernel<T, VEC, FLAT, kSummary> : nullptr,                       \
                plan.warps > 1 ? puff_recurrence_backward_kernel<T, VEC, FLAT, kTeam>                                      \
-                              : puff_recurrence_backward_kernel<T, VEC, FLAT, kStream>, size_t{0}, plan, st, p, plan, pairs, saved,  \
-               static_cast<const T*>(doutputs), dfinal, static_cast<T*>(dgates), static_cast<T*>(dinputs), dstate)
+                              : puff_recurrence_backward_kernel<T, VEC, FLAT, kStream>,                                   \
+               size_t{0}, plan, st, p, plan, pairs, saved, static_cast<const T*>(doutputs), dfinal,                       \
+               static_cast<T*>(dgates), static_cast<T*>(dinputs), dstate)
     if (dtype == PUFF_DTYPE_F32) e = flat ? PUFF_RUN2(float, 1, true) : PUFF_RUN2(float, 1, false);
     else if (dtype == PUFF_DTYPE_F16) e = pair ? PUFF_RUN2(__half, 2, false) : flat ? PUFF_RUN2(__half, 1, true) : PUFF_RUN2(__half, 1, false);
     else e = pair ? PUFF_RUN2(__nv_bfloat16, 2, false) : flat ? PUFF_RUN2(__nv_bfloat16, 1, true) : PUFF_RUN2(__nv_bfloat16, 1, false);
@@ -1007,9 +1014,16 @@ extern "C" int puff_policy_sm100_recurrence_step(const void* gates, const void* 
     puff_recurrence_step_kernel<T, VEC><<<static_cast<int>(blocks), 256, 0, st>>>(static_cast<const T*>(gates),           \
         static_cast<const T*>(inputs), state, resets, p.reset_bytes, batch, channels, gates_stride, inputs_stride,        \
         static_cast<T*>(outputs), new_state)
-    if (dtype == PUFF_DTYPE_F32) { if (four) PUFF_RUN2(float, 4); else PUFF_RUN2(float, 1); }
-    else if (dtype == PUFF_DTYPE_F16) { if (four) PUFF_RUN2(__half, 4); else PUFF_RUN2(__half, 1); }
-    else { if (four) PUFF_RUN2(__nv_bfloat16, 4); else PUFF_RUN2(__nv_bfloat16, 1); }
+    if (dtype == PUFF_DTYPE_F32) {
+        if (four) PUFF_RUN2(float, 4);
+        else PUFF_RUN2(float, 1);
+    } else if (dtype == PUFF_DTYPE_F16) {
+        if (four) PUFF_RUN2(__half, 4);
+        else PUFF_RUN2(__half, 1);
+    } else {
+        if (four) PUFF_RUN2(__nv_bfloat16, 4);
+        else PUFF_RUN2(__nv_bfloat16, 1);
+    }
 #undef PUFF_RUN2
     count_launch();
     return static_cast<int>(cudaGetLastError());
