@@ -551,13 +551,15 @@ puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const l
     }
 }
 
-// Rows of up to kLpSmall entries, both directions.  A CTA brings 256 / G rows into shared memory by 16-byte copies of
-// their common span, wherever rows begin; G threads then work on a row from there (fewer than 33 elements each), and
-// the backward pass writes gradients over the logits and copies the span out.  The maximum and the sums are computed
+// Small rows, both directions.  A CTA brings 256 / G rows into shared memory by 16-byte copies of their common span,
+// wherever rows begin; G threads then work on a row from there (fewer than 33 elements each), and the backward pass
+// writes gradients over the logits and copies the span out.  The maximum and the sums are computed
 // again in the backward pass: reading them back would cost more than the arithmetic.  Rows start at different banks:
 // row i of the tile begins its walk i * skew elements in.  524288 x 18 fp32: 20 us forward and 29 backward, where a warp a
 // row took 316 and 278; instruction issue (81 and 87 %) bounds it, DRAM stands at 40 %.
-constexpr int kLpSmall = 128;
+// Up to which size a row is small, against a warp a row (us, small / warp): 500000 x 256 bf16 forward 131 / 283 and backward
+// 207 / 260; 200000 x 333 86 / 131 and 131 / 133; 200000 x 500 117 / 131 and 184 / 139.
+constexpr int kLpSmall = 512, kLpSmallBackward = 384;
 template <typename T, bool ENT, int G, bool BACKWARD>
 __global__ void __launch_bounds__(kLpThreads)
 puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,
@@ -699,7 +701,9 @@ static cudaError_t launch_small(const void* logits, RowMap lmap, const long long
         static_cast<T*>(dlogits))
     if (g == 1) PUFF_SMALL(1);
     else if (g == 2) PUFF_SMALL(2);
-    else PUFF_SMALL(4);
+    else if (g == 4) PUFF_SMALL(4);
+    else if (g == 8) PUFF_SMALL(8);
+    else PUFF_SMALL(16);
 #undef PUFF_SMALL
     return cudaGetLastError();
 }
@@ -709,10 +713,10 @@ static cudaError_t launch_logprobs(const void* logits, RowMap lmap, const long l
                                    long long vocab, float inv_t, float* logprobs, float* entropy, float* row_stats,
                                    cudaStream_t st)
 {
-    if (vocab <= kLpSmall)      // its backward pass works the statistics out again
-        return launch_small<T, ENT, false>(logits, lmap, actions, amap, rows, vocab, inv_t, LogprobOut{logprobs, entropy, nullptr},
-                                           nullptr, nullptr, nullptr, st);
-    const LogprobOut out = {logprobs, entropy, reinterpret_cast<float2*>(row_stats)};
+    // (a small backward pass works the statistics out again)
+    const LogprobOut out = {logprobs, entropy, vocab <= kLpSmallBackward ? nullptr : reinterpret_cast<float2*>(row_stats)};
+    if (vocab <= kLpSmall)
+        return launch_small<T, ENT, false>(logits, lmap, actions, amap, rows, vocab, inv_t, out, nullptr, nullptr, nullptr, st);
     const T* z = static_cast<const T*>(logits);
     const long long bytes = vocab * static_cast<long long>(sizeof(T));
     // a warp a row while rows are short and many enough to give every SM sixteen warps
@@ -744,7 +748,7 @@ static cudaError_t launch_logprobs_backward(const void* logits, RowMap lmap, con
                                             const float* entropy, const float* dlogprobs, const float* dentropy,
                                             void* dlogits, cudaStream_t st)
 {
-    if (vocab <= kLpSmall)
+    if (vocab <= kLpSmallBackward)
         return launch_small<T, ENT, true>(logits, lmap, actions, amap, rows, vocab, inv_t, LogprobOut{}, dlogprobs, dentropy,
                                           dlogits, st);
     constexpr long long per_unit = 32LL * kLpUnitVecs * Vec16<T>::N;

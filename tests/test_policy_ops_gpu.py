@@ -42,7 +42,7 @@ def check_logprobs(logits, actions, temperature=1.0, entropy=True, seed=0):
     return lp, H, dlogits
 
 
-VOCABS = [1, 2, 3, 4, 5, 7, 8, 15, 18, 31, 32, 33, 64, 65, 127, 128, 200, 255, 256, 257, 500, 512, 513, 1000, 1024,
+VOCABS = [1, 2, 3, 4, 5, 7, 8, 15, 18, 31, 32, 33, 64, 65, 127, 128, 200, 255, 256, 257, 384, 385, 500, 512, 513, 1000, 1024,
           1025, 2047, 2048, 2049, 4097, 10007, 33000, 70001]
 
 
