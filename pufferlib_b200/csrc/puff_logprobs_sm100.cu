@@ -694,6 +694,7 @@ static cudaError_t launch_small(const void* logits, RowMap lmap, const long long
     while (vocab > 32 * g) g *= 2;
     const long long tile = kLpThreads / g;
     const size_t smem = static_cast<size_t>(tile) * vocab * sizeof(T) + 32;
+    if ((rows + tile - 1) / tile > 0x7fffffffLL) return cudaErrorInvalidConfiguration;   // rows that repeat with stride 0
     const int grid = static_cast<int>((rows + tile - 1) / tile);
 #define PUFF_SMALL(G)                                                                                                       \
     puff_logprobs_small_kernel<T, ENT, G, BACKWARD><<<grid, kLpThreads, smem, st>>>(                                        \

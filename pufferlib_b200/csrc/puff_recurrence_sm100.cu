@@ -693,6 +693,122 @@ puff_recurrence_step_kernel(const T* __restrict__ gates, const T* __restrict__ i
     }
 }
 
+// Up to eight steps, N of them known to the compiler: a thread takes VEC adjacent channels through all of them, every input
+// asked for before the first is used.  Two channels where everything is aligned for them, one otherwise.  Against the tiles
+// of sixteen, which compute steps that are not there (us, tiles / here, forward and backward): 6525 x 1 x 1888 bf16 274 / 56
+// and 370 / 56, x 8 x 1888 277 / 175 and 384 / 288, x 4 x 1891 629 / 137 and 684 / 184, 700000 x 8 x 18 1141 / 193 and
+// 1249 / 316.  With one kernel of eight steps and a branch at each 175 and 288 were 240 and 604; four channels a thread
+// are faster forward (8 steps 164) and slower backward (326).
+constexpr int kRecShort = 8;
+template <typename T, int VEC> struct alignas(VEC * sizeof(T)) Adjacent {
+    T v[VEC];
+};
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void load_short(Adjacent<T, VEC> (&to)[N], const T* from, long long stride)
+{
+#pragma unroll
+    for (int j = 0; j < N; ++j, from += stride)
+        to[j] = *reinterpret_cast<const Adjacent<T, VEC>*>(from);
+}
+template <int VEC>
+__device__ __forceinline__ Adjacent<float, VEC> load_or_zero(const float* from, long long at)
+{
+    Adjacent<float, VEC> a = {};
+    if (from != nullptr) a = *reinterpret_cast<const Adjacent<float, VEC>*>(from + at);
+    return a;
+}
+template <int N>
+__device__ __forceinline__ unsigned resets_short(const RecArgs& p, long long b)
+{
+    unsigned cut = 0;
+    if (p.reset_bytes != 0)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (is_reset(p, b * N + j)) cut |= 1u << j;
+    return cut;
+}
+template <typename T, int VEC, int N>
+__global__ void __launch_bounds__(256)
+puff_recurrence_short_kernel(RecArgs p, T* __restrict__ outputs, float* __restrict__ final_state, float* __restrict__ saved)
+{
+    const long long groups = p.channels / VEC, n = p.batch * groups, stride = static_cast<long long>(gridDim.x) * 256;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += stride) {
+        const long long b = quotient(i, groups), c = (i - b * groups) * VEC;
+        Adjacent<T, VEC> gate[N], input[N];
+        load_short(gate, static_cast<const T*>(p.gates) + b * p.gates_batch_stride + c, p.gates_step_stride);
+        load_short(input, static_cast<const T*>(p.inputs) + b * p.inputs_batch_stride + c, p.inputs_step_stride);
+        Adjacent<float, VEC> h = load_or_zero<VEC>(p.state, i * VEC);
+        const unsigned cut = resets_short<N>(p, b);
+        if (saved != nullptr) *reinterpret_cast<Adjacent<float, VEC>*>(saved + i * VEC) = h;
+        T* out = outputs + b * N * p.channels + c;
+#pragma unroll
+        for (int j = 0; j < N; ++j, out += p.channels) {
+            Adjacent<T, VEC> o;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                float g[1] = {to_f32(gate[j].v[v])}, code[1], keep[1], take[1];
+                gate_codes(g, code);
+                gate_pairs(code, keep, take);
+                const float fresh = take[0] * to_f32(input[j].v[v]);
+                h.v[v] = cut >> j & 1u ? fresh : fmaf(keep[0], h.v[v], fresh);
+                o.v[v] = from_f32<T>(h.v[v]);
+            }
+            *reinterpret_cast<Adjacent<T, VEC>*>(out) = o;
+        }
+        *reinterpret_cast<Adjacent<float, VEC>*>(final_state + i * VEC) = h;
+    }
+}
+template <typename T, int VEC, int N>
+__global__ void __launch_bounds__(256)
+puff_recurrence_backward_short_kernel(RecArgs p, const float* __restrict__ saved, const T* __restrict__ doutputs,
+                                      const float* __restrict__ dfinal, T* __restrict__ dgates, T* __restrict__ dinputs,
+                                      float* __restrict__ dstate)
+{
+    const long long groups = p.channels / VEC, n = p.batch * groups, stride = static_cast<long long>(gridDim.x) * 256;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += stride) {
+        const long long b = quotient(i, groups), c = (i - b * groups) * VEC, at = b * N * p.channels + c;
+        Adjacent<T, VEC> gate[N], input[N], dout[N];
+        load_short(gate, static_cast<const T*>(p.gates) + b * p.gates_batch_stride + c, p.gates_step_stride);
+        load_short(input, static_cast<const T*>(p.inputs) + b * p.inputs_batch_stride + c, p.inputs_step_stride);
+        if (doutputs != nullptr) load_short(dout, doutputs + at, p.channels);
+        const Adjacent<float, VEC> before = load_or_zero<VEC>(saved, i * VEC);
+        Adjacent<float, VEC> lam = load_or_zero<VEC>(dfinal, i * VEC);
+        const unsigned cut = resets_short<N>(p, b);
+        float h[VEC], code[N][VEC], slope[N][VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = before.v[v];
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float x = to_f32(input[j].v[v]);
+                float g[1] = {to_f32(gate[j].v[v])}, cd[1], keep[1], take[1];
+                gate_codes(g, cd);
+                gate_pairs(cd, keep, take);
+                if (cut >> j & 1u) h[v] = 0.0f;
+                code[j][v] = cd[0];
+                slope[j][v] = keep[0] * take[0] * (h[v] - x);
+                h[v] = cut >> j & 1u ? take[0] * x : fmaf(keep[0], h[v], take[0] * x);
+            }
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j) {
+            Adjacent<T, VEC> dx, dg;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                float cd[1] = {code[j][v]}, keep[1], take[1];
+                gate_pairs(cd, keep, take);
+                if (doutputs != nullptr) lam.v[v] += to_f32(dout[j].v[v]);
+                dx.v[v] = from_f32<T>(lam.v[v] * take[0]);
+                dg.v[v] = from_f32<T>(lam.v[v] * slope[j][v]);
+                lam.v[v] = cut >> j & 1u ? 0.0f : lam.v[v] * keep[0];
+            }
+            *reinterpret_cast<Adjacent<T, VEC>*>(dinputs + at + j * p.channels) = dx;
+            *reinterpret_cast<Adjacent<T, VEC>*>(dgates + at + j * p.channels) = dg;
+        }
+        if (dstate != nullptr) *reinterpret_cast<Adjacent<float, VEC>*>(dstate + i * VEC) = lam;
+    }
+}
+
 // bytes from the first to one past the last element of a [batch, steps, channels] view
 static long long view_span(long long batch, long long steps, long long channels, long long bs, long long ss, int size)
 {
@@ -790,6 +906,53 @@ static RecPlan with_cluster(RecPlan plan, long long steps)
 // channels too few to fill half a warp's lanes: rows share warps
 static bool rec_flat(long long channels, int vec) { return channels < 16 * vec; }
 
+// do `vec` adjacent channels of the inputs stay together, and aligned, in every row?
+static bool together(const RecArgs& p, int size, int vec)
+{
+    return p.channels % vec == 0 && p.gates_batch_stride % vec == 0 && p.gates_step_stride % vec == 0 && p.inputs_batch_stride % vec == 0 &&
+           p.inputs_step_stride % vec == 0 && !misaligned(p.gates, static_cast<unsigned>(vec * size)) &&
+           !misaligned(p.inputs, static_cast<unsigned>(vec * size));
+}
+static int short_grid(const RecArgs& p, int vec)
+{
+    const long long blocks = (p.batch * p.channels / vec + 255) / 256;
+    return static_cast<int>(blocks < (1 << 30) ? blocks : (1 << 30));
+}
+// the kernel of N steps, from N = 1 on
+template <typename T, int N = 1>
+static cudaError_t launch_short(const RecArgs& p, void* outputs, float* final_state, float* saved, cudaStream_t st)
+{
+    if constexpr (N < kRecShort)
+        if (p.steps > N) return launch_short<T, N + 1>(p, outputs, final_state, saved, st);
+    constexpr int V = 2;
+    const unsigned bytes = V * sizeof(T);
+    if (together(p, sizeof(T), V) && !misaligned(outputs, bytes) && !misaligned(p.state, 4 * V) && !misaligned(final_state, 4 * V) &&
+        !misaligned(saved, 4 * V))
+        puff_recurrence_short_kernel<T, V, N><<<short_grid(p, V), 256, 0, st>>>(p, static_cast<T*>(outputs), final_state, saved);
+    else
+        puff_recurrence_short_kernel<T, 1, N><<<short_grid(p, 1), 256, 0, st>>>(p, static_cast<T*>(outputs), final_state, saved);
+    count_launch();
+    return cudaGetLastError();
+}
+template <typename T, int N = 1>
+static cudaError_t launch_backward_short(const RecArgs& p, const float* saved, const void* doutputs, const float* dfinal, void* dgates,
+                                         void* dinputs, float* dstate, cudaStream_t st)
+{
+    if constexpr (N < kRecShort)
+        if (p.steps > N) return launch_backward_short<T, N + 1>(p, saved, doutputs, dfinal, dgates, dinputs, dstate, st);
+    constexpr int V = 2;
+    const unsigned bytes = V * sizeof(T);
+    const T* d = static_cast<const T*>(doutputs);
+    T *dg = static_cast<T*>(dgates), *dx = static_cast<T*>(dinputs);
+    if (together(p, sizeof(T), V) && !misaligned(d, bytes) && !misaligned(dg, bytes) && !misaligned(dx, bytes) &&
+        !misaligned(saved, 4 * V) && !misaligned(dfinal, 4 * V) && !misaligned(dstate, 4 * V))
+        puff_recurrence_backward_short_kernel<T, V, N><<<short_grid(p, V), 256, 0, st>>>(p, saved, d, dfinal, dg, dx, dstate);
+    else
+        puff_recurrence_backward_short_kernel<T, 1, N><<<short_grid(p, 1), 256, 0, st>>>(p, saved, d, dfinal, dg, dx, dstate);
+    count_launch();
+    return cudaGetLastError();
+}
+
 static int check_recurrence(const RecArgs& p, int dtype)
 {
     const int size = dtype_bytes(dtype);
@@ -862,6 +1025,12 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
     int sms = 0;
     rc = require_sm100(&sms);
     if (rc != PUFF_OK) return rc;
+    if (steps > 0 && steps <= kRecShort) {
+        cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+        return static_cast<int>(dtype == PUFF_DTYPE_F32   ? launch_short<float>(p, outputs, final_state, saved, st)
+                                : dtype == PUFF_DTYPE_F16 ? launch_short<__half>(p, outputs, final_state, saved, st)
+                                                          : launch_short<__nv_bfloat16>(p, outputs, final_state, saved, st));
+    }
     // two channels a lane where every address of the 16-bit tensors stays 4-byte aligned
     const bool pair = size == 2 && channels % 2 == 0 && gates_batch_stride % 2 == 0 && gates_step_stride % 2 == 0 &&
                       inputs_batch_stride % 2 == 0 && inputs_step_stride % 2 == 0 && !misaligned(gates, 4) &&
@@ -938,6 +1107,13 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
     int sms = 0;
     rc = require_sm100(&sms);
     if (rc != PUFF_OK) return rc;
+    if (steps > 0 && steps <= kRecShort) {
+        cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+        return static_cast<int>(
+            dtype == PUFF_DTYPE_F32   ? launch_backward_short<float>(p, saved, doutputs, dfinal, dgates, dinputs, dstate, st)
+            : dtype == PUFF_DTYPE_F16 ? launch_backward_short<__half>(p, saved, doutputs, dfinal, dgates, dinputs, dstate, st)
+                                      : launch_backward_short<__nv_bfloat16>(p, saved, doutputs, dfinal, dgates, dinputs, dstate, st));
+    }
     const bool pair = size == 2 && channels % 2 == 0 && gates_batch_stride % 2 == 0 && gates_step_stride % 2 == 0 &&
                       inputs_batch_stride % 2 == 0 && inputs_step_stride % 2 == 0 && !misaligned(gates, 4) &&
                       !misaligned(inputs, 4) && !misaligned(doutputs, 4) && !misaligned(dgates, 4) &&

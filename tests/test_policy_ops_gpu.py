@@ -367,6 +367,8 @@ def check_recurrence(gates, x, resets, state, seed=0, use=(True, True)):
                                    # rows of a multiple of 16 bytes: tiles at every edge of steps, channels and rounds
                                    (3, 1, 64), (2, 5, 32), (5, 16, 40), (3, 48, 72), (2, 130, 200), (1, 777, 1024),
                                    (1, 4097, 64), (3, 2100, 96), (700, 33, 64), (70000, 2, 32),
+                                   # a few steps: four channels a thread, or one
+                                   (5, 7, 33), (4, 8, 36), (9, 8, 130), (2, 9, 36), (3000, 4, 515), (40, 3, 256),
                                    # few lanes over many steps: clusters of two and four, and ranges
                                    (3, 1500, 1024), (6, 1100, 1000), (2, 2100, 640), (1, 2500, 1600)])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -376,7 +378,8 @@ def test_recurrence_shapes(shape, dtype):
         check_recurrence(*rec_inputs(*shape, dtype, seed=sum(shape), resets=0.0, state=False), use=(True, False))
 
 
-@pytest.mark.parametrize("shape", [(3, 40, 64), (2, 300, 33), (64, 16, 128), (1, 3000, 512), (40, 200, 300)])
+@pytest.mark.parametrize("shape", [(3, 40, 64), (2, 300, 33), (64, 16, 128), (1, 3000, 512), (40, 200, 300),
+                                   (300, 6, 36), (50, 8, 31), (2, 1, 1000)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_recurrence_strides(shape, dtype):
     """Halves of one projection, time-major tensors, odd offsets: read in place."""
