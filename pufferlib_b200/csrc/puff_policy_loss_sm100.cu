@@ -230,9 +230,9 @@ puff_policy_loss_kernel(LossArgs p, double* __restrict__ partial)
     write_partial(total, partial);
 }
 
-// Rows that matter: one advantage each, or SEQ, a mean each (131072 x 256 196 us, 16777216 x 1 202, 100 x 100001 144).  TEAM threads a row, rows side by side in a warp where they
-// are short, one a CTA (TEAM 256) where they are long and few.  SEQ: a thread's share of the row's policy, kl and entropy
-// sums is divided by the row's length.
+// Rows that matter: one advantage each, or SEQ, a mean each (131072 x 256 196 us, 16777216 x 1 202, 100 x 100001 144).
+// TEAM threads a row, rows side by side in a warp where they are short, one a CTA (TEAM 256) where they are long and few.
+// SEQ: a thread's share of the row's policy, kl and entropy sums is divided by the row's length.
 template <int VEC, int TEAM, bool SEQ, bool ONE_ADVANTAGE>
 __global__ void __launch_bounds__(TEAM > kLossThreads ? TEAM : kLossThreads, TEAM > kLossThreads ? 1 : 4)
 puff_policy_loss_rows_kernel(LossArgs p, double* __restrict__ partial)
