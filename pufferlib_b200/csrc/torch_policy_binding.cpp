@@ -9,8 +9,10 @@
 // Each differentiable operator has an autograd kernel whose node keeps what the backward operator needs and calls it (nodes
 // of their own rather than torch::autograd::Function, whose context costs several microseconds a pass at the host).
 // The *_forward and *_backward operators can be called without autograd (for a program that captures a whole update
-// into a CUDA graph); their results are not differentiable, and a second derivative raises.
+// into a CUDA graph); their results are not differentiable, and a second derivative raises.  So does a forward-mode
+// derivative: a node like these has none, and its tangent would be lost.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/all.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -77,6 +79,13 @@ template <typename N> std::shared_ptr<N> new_node(torch::autograd::edge_list&& e
     std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
     node->set_next_edges(std::move(edges));
     return node;
+}
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool dual(const OptTensor& t) { return t.has_value() && dual(*t); }
+template <typename... Tensors> void refuse_forward_mode(const char* what, const Tensors&... tensors)
+{
+    TORCH_CHECK(!((dual(tensors) || ...) && c10::AutogradState::get_tls_state().get_fw_grad_mode()), what,
+                " has no forward-mode derivative");
 }
 SavedVariable saved(const OptTensor& t) { return present(t) ? SavedVariable(*t, false) : SavedVariable(); }
 
@@ -256,6 +265,7 @@ struct LogprobsNode : public Node {
     {
         std::lock_guard<std::mutex> lock(mutex_);
         if ((!grads[0].defined() && !grads[1].defined()) || !task_should_compute_output(0)) return {Tensor()};
+        refuse_forward_mode("the backward pass of puff_action_logprobs", grads[0], grads[1]);
         const BelowUnlessGraph below;
         const Tensor dlp = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(grads[1], at::MemoryFormat::Contiguous);
         const OptTensor dh = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
@@ -266,6 +276,7 @@ struct LogprobsNode : public Node {
 std::tuple<Tensor, Tensor> action_logprobs_autograd(const Tensor& logits, const Tensor& actions, double temperature,
                                                     bool want_entropy)
 {
+    refuse_forward_mode("puff_action_logprobs", logits);
     if (!(at::GradMode::is_enabled() && logits.requires_grad())) {
         at::AutoDispatchBelowADInplaceOrView below;
         return action_logprobs(logits, actions, temperature, want_entropy);
@@ -455,6 +466,7 @@ struct PolicyLossNode : public Node {
     {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return {Tensor(), Tensor()};
+        refuse_forward_mode("the backward pass of puff_policy_loss", grads[0]);
         const BelowUnlessGraph below;
         const bool want_dentropy = task_should_compute_output(1);
         auto [dlogprobs, dentropy] = loss_backward(slope.unpack(), row_scale.unpack(), weight.unpack(), grads[0],
@@ -469,6 +481,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor& logprobs, 
                                                         const OptTensor& entropy, double ent_coef, const OptTensor& mask,
                                                         c10::string_view reduction, double denominator)
 {
+    refuse_forward_mode("puff_policy_loss", logprobs, old_logprobs, advantages, ref_logprobs, entropy);
     if (at::GradMode::is_enabled())
         TORCH_CHECK(!old_logprobs.requires_grad() && !advantages.requires_grad() && !wants_grad(ref_logprobs),
                     "old_logprobs, advantages and ref_logprobs are constants of the loss; detach them");
@@ -617,6 +630,7 @@ struct RecurrenceNode : public Node {
     {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
+        refuse_forward_mode("the backward pass of puff_gated_recurrence", grads[0], grads[1]);
         const BelowUnlessGraph below;
         const OptTensor dout = grads[0].defined() ? OptTensor(grads[0].contiguous()) : std::nullopt;
         const OptTensor dfinal = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
@@ -628,6 +642,7 @@ struct RecurrenceNode : public Node {
 std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor& gates, const Tensor& inputs, const OptTensor& resets,
                                                      const OptTensor& state)
 {
+    refuse_forward_mode("puff_gated_recurrence", gates, inputs, state);
     if (!(at::GradMode::is_enabled() && (gates.requires_grad() || inputs.requires_grad() || wants_grad(state)))) {
         at::AutoDispatchBelowADInplaceOrView below;
         return gated_recurrence(gates, inputs, resets, state);
@@ -673,6 +688,7 @@ Tensor recurrence_step_cuda(const Tensor& gates, const Tensor& inputs, const Ten
 // the single step is for acting, not for training
 Tensor recurrence_step_autograd(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, Tensor new_state)
 {
+    refuse_forward_mode("puff_gated_recurrence_step", gates, inputs, state, new_state);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (gates.requires_grad() || inputs.requires_grad() || state.requires_grad() ||
                                                  new_state.requires_grad())),
                 "the single step has no gradient; call it under torch.no_grad() or use puff_gated_recurrence");

@@ -1,0 +1,69 @@
+"""CPU: the gradients of the policy-update operators as autograd's other modes take them, on tensors without data."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+M = "meta"
+
+
+def meta(*shape, dtype=torch.float32, grad=False):
+    return torch.empty(*shape, device=M, dtype=dtype, requires_grad=grad)
+
+
+def actions(*shape):
+    return meta(*shape, dtype=torch.int64)
+
+
+# an operator as a function of one tensor at a time, and that tensor's shape
+ONE_INPUT = {
+    "logits": ((4, 8), lambda pb, t: pb.action_logprobs(t, actions(4))[0]),
+    "logits without entropy": ((4, 8), lambda pb, t: pb.action_logprobs(t, actions(4), entropy=False)[0]),
+    "logprobs": ((4, 6), lambda pb, t: pb.policy_loss(t, meta(4, 6), meta(4, 6))[0]),
+    "old_logprobs": ((4, 6), lambda pb, t: pb.policy_loss(meta(4, 6), t, meta(4, 6))[0]),
+    "advantages": ((4, 6), lambda pb, t: pb.policy_loss(meta(4, 6), meta(4, 6), t)[0]),
+    "ref_logprobs": ((4, 6), lambda pb, t: pb.policy_loss(meta(4, 6), meta(4, 6), meta(4, 6), ref_logprobs=t, kl_coef=0.1)[0]),
+    "entropy": ((4, 6), lambda pb, t: pb.policy_loss(meta(4, 6), meta(4, 6), meta(4, 6), entropy=t, ent_coef=0.1)[0]),
+    "gates": ((2, 7, 8), lambda pb, t: pb.gated_recurrence(t, meta(2, 7, 8))[0]),
+    "inputs": ((2, 7, 8), lambda pb, t: pb.gated_recurrence(meta(2, 7, 8), t)[0]),
+    "state": ((2, 8), lambda pb, t: pb.gated_recurrence(meta(2, 7, 8), meta(2, 7, 8), state=t)[0]),
+    "step gates": ((2, 8), lambda pb, t: pb.gated_recurrence_step(t, meta(2, 8), meta(2, 8))[0]),
+    "step inputs": ((2, 8), lambda pb, t: pb.gated_recurrence_step(meta(2, 8), t, meta(2, 8))[0]),
+    "step state": ((2, 8), lambda pb, t: pb.gated_recurrence_step(meta(2, 8), meta(2, 8), t, new_state=meta(2, 8))[0]),
+    "step new_state": ((2, 8), lambda pb, t: pb.gated_recurrence_step(meta(2, 8), meta(2, 8), meta(2, 8), new_state=t)[0]),
+}
+
+
+@pytest.mark.parametrize("which", ONE_INPUT)
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(which, grad):
+    """A tangent would be lost on the way: there is no forward-mode derivative."""
+    import pufferlib_b200 as pb
+    shape, call = ONE_INPUT[which]
+    if grad and which in ("old_logprobs", "advantages", "ref_logprobs") or grad and which.startswith("step"):
+        pytest.skip("requires_grad is refused for itself")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(meta(*shape, grad=grad), meta(*shape))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(pb, dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(pb, dual)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda t: call(pb, t), (meta(*shape),), (meta(*shape),))
+    call(pb, meta(*shape))                       # outside of it nothing is refused
+
+
+def test_forward_mode_over_reverse_is_refused():
+    """A tangent on the incoming gradient of a backward pass."""
+    import pufferlib_b200 as pb
+    z, gates = meta(4, 8, grad=True), meta(2, 7, 8, grad=True)
+    x = meta(4, 6, grad=True)
+    for make in (lambda: (pb.action_logprobs(z, actions(4))[0], z), lambda: (pb.action_logprobs(z, actions(4))[1], z),
+                 lambda: (pb.policy_loss(x, meta(4, 6), meta(4, 6))[0], x),
+                 lambda: (pb.gated_recurrence(gates, meta(2, 7, 8))[0], gates),
+                 lambda: (pb.gated_recurrence(gates, meta(2, 7, 8))[1], gates)):
+        out, leaf = make()
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(torch.empty_like(out), torch.empty_like(out))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, dual, retain_graph=True)
+        torch.autograd.grad(out, leaf, torch.empty_like(out))
