@@ -63,15 +63,6 @@ template <typename T> T* ptr(const Tensor& t) { return t.defined() ? static_cast
 template <typename T> const T* ptr(const OptTensor& t) { return t.has_value() && t->defined() ? static_cast<const T*>(t->data_ptr()) : nullptr; }
 bool present(const OptTensor& t) { return t.has_value() && t->defined(); }
 OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
-// In a backward pass that builds no graph the backward operators are called below autograd: above it they would pass
-// through the boxed kernel that refuses second derivatives.
-struct BelowUnlessGraph {
-    std::optional<at::AutoDispatchBelowADInplaceOrView> below;
-    BelowUnlessGraph()
-    {
-        if (!at::GradMode::is_enabled()) below.emplace();
-    }
-};
 cudaStream_t current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 template <typename N> std::shared_ptr<N> new_node(torch::autograd::edge_list&& edges)
@@ -79,6 +70,25 @@ template <typename N> std::shared_ptr<N> new_node(torch::autograd::edge_list&& e
     std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
     node->set_next_edges(std::move(edges));
     return node;
+}
+// Where a backward pass builds a graph, its results hang on this node, with every input of the operator and every incoming
+// gradient behind it: whichever of them a second derivative is asked for, it raises.
+struct NoSecondDerivative : public Node {
+    const char* what = "";
+    std::string name() const override { return "PuffNoSecondDerivative"; }
+    variable_list apply(variable_list&&) override { TORCH_CHECK(false, what, " has no second derivative"); }
+};
+variable_list refuse_second_derivatives(const char* what, const Node& node, const variable_list& grads, variable_list&& results)
+{
+    if (!at::GradMode::is_enabled()) return std::move(results);
+    torch::autograd::edge_list edges = node.next_edges();
+    for (const Tensor& g : grads)
+        if (g.defined() && g.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(g));
+    auto refuse = new_node<NoSecondDerivative>(std::move(edges));
+    refuse->what = what;
+    for (const Tensor& r : results)
+        if (r.defined()) torch::autograd::set_history(r, refuse);
+    return std::move(results);
 }
 bool dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 bool dual(const OptTensor& t) { return t.has_value() && dual(*t); }
@@ -266,11 +276,12 @@ struct LogprobsNode : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if ((!grads[0].defined() && !grads[1].defined()) || !task_should_compute_output(0)) return {Tensor()};
         refuse_forward_mode("the backward pass of puff_action_logprobs", grads[0], grads[1]);
-        const BelowUnlessGraph below;
+        const at::AutoDispatchBelowADInplaceOrView below;
         const Tensor dlp = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(grads[1], at::MemoryFormat::Contiguous);
         const OptTensor dh = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
-        return {logprobs_backward(logits.unpack(), actions.unpack(), temperature, row_stats.unpack(),
-                                  optional(entropy.unpack(shared_from_this())), dlp, dh)};
+        return refuse_second_derivatives("puff_action_logprobs", *this, grads,
+                                         {logprobs_backward(logits.unpack(), actions.unpack(), temperature, row_stats.unpack(),
+                                                            optional(entropy.unpack(shared_from_this())), dlp, dh)});
     }
 };
 std::tuple<Tensor, Tensor> action_logprobs_autograd(const Tensor& logits, const Tensor& actions, double temperature,
@@ -467,11 +478,11 @@ struct PolicyLossNode : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return {Tensor(), Tensor()};
         refuse_forward_mode("the backward pass of puff_policy_loss", grads[0]);
-        const BelowUnlessGraph below;
+        const at::AutoDispatchBelowADInplaceOrView below;
         const bool want_dentropy = task_should_compute_output(1);
         auto [dlogprobs, dentropy] = loss_backward(slope.unpack(), row_scale.unpack(), weight.unpack(), grads[0],
                                                    optional(mask.unpack()), ent_coef, want_dentropy);
-        return {dlogprobs, want_dentropy ? dentropy : Tensor()};
+        return refuse_second_derivatives("puff_policy_loss", *this, grads, {dlogprobs, want_dentropy ? dentropy : Tensor()});
     }
 };
 bool wants_grad(const OptTensor& t) { return present(t) && t->requires_grad(); }
@@ -631,12 +642,12 @@ struct RecurrenceNode : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
         refuse_forward_mode("the backward pass of puff_gated_recurrence", grads[0], grads[1]);
-        const BelowUnlessGraph below;
+        const at::AutoDispatchBelowADInplaceOrView below;
         const OptTensor dout = grads[0].defined() ? OptTensor(grads[0].contiguous()) : std::nullopt;
         const OptTensor dfinal = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
         auto [dgates, dinputs, dstate] = recurrence_backward(gates.unpack(), inputs.unpack(), optional(resets.unpack()),
                                                              states.unpack(), dout, dfinal);
-        return {dgates, dinputs, dstate};
+        return refuse_second_derivatives("puff_gated_recurrence", *this, grads, {dgates, dinputs, dstate});
     }
 };
 std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor& gates, const Tensor& inputs, const OptTensor& resets,

@@ -67,3 +67,49 @@ def test_forward_mode_over_reverse_is_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, leaf, dual, retain_graph=True)
         torch.autograd.grad(out, leaf, torch.empty_like(out))
+
+
+def second_cases(pb):
+    """(output, its differentiable leaves) per operator and output."""
+    z, lp, ent = meta(4, 8, grad=True), meta(4, 6, grad=True), meta(4, 6, grad=True)
+    gates, x, s = meta(2, 7, 8, grad=True), meta(2, 7, 8, grad=True), meta(2, 8, grad=True)
+    yield pb.action_logprobs(z, actions(4))[0], [z]
+    yield pb.action_logprobs(z, actions(4))[1], [z]
+    for reduction in ("token", "sequence"):
+        yield pb.policy_loss(lp, meta(4, 6), meta(4, 6), reduction=reduction)[0], [lp]
+        yield pb.policy_loss(lp, meta(4, 6), meta(4, 6), entropy=ent, ent_coef=0.1, reduction=reduction)[0], [lp, ent]
+    yield pb.gated_recurrence(gates, x, state=s)[0], [gates, x, s]
+    yield pb.gated_recurrence(gates, x, state=s)[1], [gates, x, s]
+
+
+def test_second_derivatives_are_refused_for_every_leaf():
+    """A gradient taken with create_graph depends on all leaves: going back through it raises, whichever is asked for
+    and whatever else the result depends on."""
+    import pufferlib_b200 as pb
+    for out, leaves in second_cases(pb):
+        grads = torch.autograd.grad(out.sum(), leaves, create_graph=True)
+        assert all(g.requires_grad for g in grads)
+        for g in grads:
+            for leaf in leaves:
+                with pytest.raises(RuntimeError, match="derivative"):
+                    torch.autograd.grad((g * g).sum() + (leaf * leaf).sum(), leaf, retain_graph=True, allow_unused=True)
+        # also where the second derivative goes through the incoming gradient alone
+        weight = torch.ones_like(out).requires_grad_(True)
+        for out, leaves in second_cases(pb):
+            if out.shape != weight.shape:
+                continue
+            g = torch.autograd.grad(out, leaves[0], weight, create_graph=True)[0]
+            with pytest.raises(RuntimeError, match="derivative"):
+                torch.autograd.grad(g.sum(), weight)
+
+
+def test_first_derivatives_with_create_graph():
+    """create_graph itself is not refused: a trainer may ask for it for the sake of another term."""
+    import pufferlib_b200 as pb
+    for out, leaves in second_cases(pb):
+        (out.sum() + sum((v * v).sum() for v in leaves)).backward(create_graph=True)
+        for v in leaves:
+            assert v.grad.shape == v.shape
+            v.grad = None
+    for out, leaves in second_cases(pb):
+        assert not any(g.requires_grad for g in torch.autograd.grad(out.sum(), leaves))
