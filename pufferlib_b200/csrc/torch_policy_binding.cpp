@@ -7,7 +7,9 @@
 // tensors' device.
 //
 // Each differentiable operator has an autograd kernel whose node keeps what the backward operator needs and calls it (nodes
-// of their own rather than torch::autograd::Function, whose context costs several microseconds a pass at the host).
+// of their own rather than torch::autograd::Function, whose context costs several microseconds a pass at the host).  A
+// node unpacks what it kept before it goes below autograd: saved-tensor hooks run then, and those of activation
+// checkpointing compute a whole region again.
 // The *_forward and *_backward operators can be called without autograd (for a program that captures a whole update
 // into a CUDA graph); their results are not differentiable, and a second derivative raises.  So does a forward-mode
 // derivative: a node like these has none, and its tangent would be lost.
@@ -276,12 +278,16 @@ struct LogprobsNode : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if ((!grads[0].defined() && !grads[1].defined()) || !task_should_compute_output(0)) return {Tensor()};
         refuse_forward_mode("the backward pass of puff_action_logprobs", grads[0], grads[1]);
-        const at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor dlp = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(grads[1], at::MemoryFormat::Contiguous);
-        const OptTensor dh = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
-        return refuse_second_derivatives("puff_action_logprobs", *this, grads,
-                                         {logprobs_backward(logits.unpack(), actions.unpack(), temperature, row_stats.unpack(),
-                                                            optional(entropy.unpack(shared_from_this())), dlp, dh)});
+        const Tensor z = logits.unpack(), a = actions.unpack(), stats = row_stats.unpack();
+        const OptTensor h = optional(entropy.unpack(shared_from_this()));
+        Tensor dlogits;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const Tensor dlp = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(grads[1], at::MemoryFormat::Contiguous);
+            const OptTensor dh = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
+            dlogits = logprobs_backward(z, a, temperature, stats, h, dlp, dh);
+        }
+        return refuse_second_derivatives("puff_action_logprobs", *this, grads, {dlogits});
     }
 };
 std::tuple<Tensor, Tensor> action_logprobs_autograd(const Tensor& logits, const Tensor& actions, double temperature,
@@ -478,10 +484,14 @@ struct PolicyLossNode : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return {Tensor(), Tensor()};
         refuse_forward_mode("the backward pass of puff_policy_loss", grads[0]);
-        const at::AutoDispatchBelowADInplaceOrView below;
         const bool want_dentropy = task_should_compute_output(1);
-        auto [dlogprobs, dentropy] = loss_backward(slope.unpack(), row_scale.unpack(), weight.unpack(), grads[0],
-                                                   optional(mask.unpack()), ent_coef, want_dentropy);
+        const Tensor s = slope.unpack(), scale = row_scale.unpack(), w = weight.unpack();
+        const OptTensor kept = optional(mask.unpack());
+        Tensor dlogprobs, dentropy;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            std::tie(dlogprobs, dentropy) = loss_backward(s, scale, w, grads[0], kept, ent_coef, want_dentropy);
+        }
         return refuse_second_derivatives("puff_policy_loss", *this, grads, {dlogprobs, want_dentropy ? dentropy : Tensor()});
     }
 };
@@ -642,11 +652,15 @@ struct RecurrenceNode : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
         refuse_forward_mode("the backward pass of puff_gated_recurrence", grads[0], grads[1]);
-        const at::AutoDispatchBelowADInplaceOrView below;
-        const OptTensor dout = grads[0].defined() ? OptTensor(grads[0].contiguous()) : std::nullopt;
-        const OptTensor dfinal = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
-        auto [dgates, dinputs, dstate] = recurrence_backward(gates.unpack(), inputs.unpack(), optional(resets.unpack()),
-                                                             states.unpack(), dout, dfinal);
+        const Tensor g = gates.unpack(), x = inputs.unpack(), kept = states.unpack();
+        const OptTensor cut = optional(resets.unpack());
+        Tensor dgates, dinputs, dstate;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const OptTensor dout = grads[0].defined() ? OptTensor(grads[0].contiguous()) : std::nullopt;
+            const OptTensor dfinal = grads[1].defined() ? OptTensor(grads[1].contiguous()) : std::nullopt;
+            std::tie(dgates, dinputs, dstate) = recurrence_backward(g, x, cut, kept, dout, dfinal);
+        }
         return refuse_second_derivatives("puff_gated_recurrence", *this, grads, {dgates, dinputs, dstate});
     }
 };

@@ -113,3 +113,49 @@ def test_first_derivatives_with_create_graph():
             v.grad = None
     for out, leaves in second_cases(pb):
         assert not any(g.requires_grad for g in torch.autograd.grad(out.sum(), leaves))
+
+
+REGIONS = {
+    "head and log-probabilities": ((4, 5), lambda pb, t, w: pb.action_logprobs(t @ w, actions(4))[0]),
+    "log-probabilities without entropy": ((4, 5), lambda pb, t, w: pb.action_logprobs(t @ w, actions(4), entropy=False)[0]),
+    "loss": ((4, 5), lambda pb, t, w: pb.policy_loss(t @ w, meta(4, 8), meta(4), entropy=t @ w, ent_coef=0.1, reduction="sequence",
+                                                     mask=meta(4, 8, dtype=torch.bool))[0]),
+    "recurrence": ((2, 7, 5), lambda pb, t, w: pb.gated_recurrence(t @ w, t @ w, resets=meta(2, 7), state=(t @ w)[:, 0].contiguous())[0]),
+    "recurrence, final state": ((2, 7, 5), lambda pb, t, w: pb.gated_recurrence(t @ w, t @ w)[1]),
+}
+
+
+@pytest.mark.parametrize("which", REGIONS)
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_activation_checkpointing(which, reentrant):
+    """The operator at the end of a region whose activations are computed again in the backward pass."""
+    import pufferlib_b200 as pb
+    from torch.utils.checkpoint import checkpoint
+    shape, region = REGIONS[which]
+    t, w = meta(*shape, grad=True), meta(5, 8, grad=True)
+    out = checkpoint(lambda a, b: region(pb, a, b), t, w, use_reentrant=reentrant)
+    out.sum().backward()
+    assert t.grad.shape == t.shape and w.grad.shape == w.shape
+    # two regions in a row, and twice through the same graph
+    t.grad = w.grad = None
+    twice = sum(checkpoint(lambda a, b: region(pb, a, b), t, w, use_reentrant=reentrant).sum() for _ in range(2))
+    if not reentrant:
+        twice.backward(retain_graph=True)
+    twice.backward()
+    assert t.grad.shape == t.shape
+
+
+def test_unpack_hooks_run_under_autograd():
+    """Whatever a saved-tensor hook computes is recorded as under torch's own nodes."""
+    import pufferlib_b200 as pb
+    for which, (shape, region) in REGIONS.items():
+        t, w, seen = meta(*shape, grad=True), meta(5, 8, grad=True), []
+
+        def unpack(v):
+            with torch.enable_grad():
+                seen.append((torch.ones(2, requires_grad=True) * 2).requires_grad)
+            return v
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v, unpack):
+            out = region(pb, t, w)
+        out.sum().backward()
+        assert len(seen) >= 3 and all(seen), which
