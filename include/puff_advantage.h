@@ -427,6 +427,7 @@ int puff_policy_sm100_loss_backward(const float* slope, const float* row_scale, 
  * _step: one step of every row ([batch, channels], a row stride for gates and
  * inputs; resets [batch]) from state to new_state, which may be state itself.
  */
+#define PUFF_RECURRENCE_SAVED_STEPS 16   /* _saved_floats: batch * ceil(steps / this) * channels */
 long long puff_policy_sm100_recurrence_saved_floats(long long batch, long long steps, long long channels);
 size_t puff_policy_sm100_recurrence_scratch_bytes(long long batch, long long steps, long long channels);
 int puff_policy_sm100_recurrence(const void* gates, const void* inputs, int dtype, const void* resets,

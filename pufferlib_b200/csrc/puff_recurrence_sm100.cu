@@ -22,7 +22,7 @@
 
 namespace puff {
 
-constexpr int kRecTile = 16;       // steps whose inputs a warp holds in registers; also the distance of the saved states
+constexpr int kRecTile = PUFF_RECURRENCE_SAVED_STEPS;       // 16: steps whose inputs a warp holds in registers; also the distance of the saved states
 constexpr int kRecWarps = 8;       // warps of a CTA
 constexpr int kRecThreads = 32 * kRecWarps;
 

@@ -53,13 +53,33 @@ int dtype_code(const Tensor& t, const char* name)
     }
 }
 
-void check_f32(const Tensor& t, const Tensor& like, at::IntArrayRef sizes, const char* name)
+// A tensor's sizes as numbers, for the CUDA kernels, or as what may be symbols, for the Meta kernels, which also run while a
+// program is traced for sizes that change.
+template <typename I> struct Dims;
+template <> struct Dims<int64_t> {
+    using Ref = at::IntArrayRef;
+    static Ref sizes(const Tensor& t) { return t.sizes(); }
+    static Ref strides(const Tensor& t) { return t.strides(); }
+    static int64_t numel(const Tensor& t) { return t.numel(); }
+    static Tensor empty(Ref sizes, const at::TensorOptions& o) { return torch::empty(sizes, o); }
+};
+template <> struct Dims<c10::SymInt> {
+    using Ref = c10::SymIntArrayRef;
+    static Ref sizes(const Tensor& t) { return t.sym_sizes(); }
+    static Ref strides(const Tensor& t) { return t.sym_strides(); }
+    static c10::SymInt numel(const Tensor& t) { return t.sym_numel(); }
+    static Tensor empty(Ref sizes, const at::TensorOptions& o) { return at::empty_symint(sizes, o); }
+};
+
+template <typename I>
+void check_f32(const Tensor& t, const Tensor& like, typename Dims<I>::Ref sizes, const char* name)
 {
     TORCH_CHECK(t.device() == like.device(), "All tensors must be on same device");
     TORCH_CHECK(t.scalar_type() == torch::kFloat32, name, " must be float32");
-    TORCH_CHECK(t.sizes() == sizes, name, " must have shape ", sizes, ", got ", t.sizes());
+    TORCH_CHECK(Dims<I>::sizes(t) == sizes, name, " must have shape ", sizes, ", got ", Dims<I>::sizes(t));
     TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
 }
+void check_f32(const Tensor& t, const Tensor& like, at::IntArrayRef sizes, const char* name) { check_f32<int64_t>(t, like, sizes, name); }
 
 template <typename T> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 template <typename T> const T* ptr(const OptTensor& t) { return t.has_value() && t->defined() ? static_cast<const T*>(t->data_ptr()) : nullptr; }
@@ -104,16 +124,17 @@ SavedVariable saved(const OptTensor& t) { return present(t) ? SavedVariable(*t, 
 // ---- log-probabilities ------------------------------------------------------------------------------------------
 
 // The leading sizes of a tensor as rows [outer, inner] with one stride each
-struct Rows {
-    int64_t outer = 1, inner = 1, outer_stride = 0, inner_stride = 0;
+template <typename I> struct Rows {
+    I outer = 1, inner = 1, outer_stride = 0, inner_stride = 0;
 };
-Rows rows_of(const Tensor& t, int64_t lead, const char* name)
+template <typename I> Rows<I> rows_of(const Tensor& t, int64_t lead, const char* name)
 {
-    Rows r;
+    Rows<I> r;
+    const auto sizes = Dims<I>::sizes(t), strides = Dims<I>::strides(t);
     bool second = false;
     // from the innermost leading dimension outwards: one that continues the run so far is folded into it
     for (int64_t d = lead - 1; d >= 0; --d) {
-        const int64_t n = t.size(d), s = t.stride(d);
+        const I &n = sizes[d], &s = strides[d];
         if (n == 1) continue;
         if (!second && (r.inner == 1 || s == r.inner * r.inner_stride)) {
             if (r.inner == 1) r.inner_stride = s;
@@ -129,11 +150,11 @@ Rows rows_of(const Tensor& t, int64_t lead, const char* name)
     return r;
 }
 // logits and actions must be cut into [outer, inner] alike
-void rows_alike(Rows& a, Rows& b, const char* what)
+template <typename I> void rows_alike(Rows<I>& a, Rows<I>& b, const char* what)
 {
     if (a.inner == b.inner) return;
-    Rows& coarse = a.inner > b.inner ? a : b;
-    const Rows& fine = a.inner > b.inner ? b : a;
+    Rows<I>& coarse = a.inner > b.inner ? a : b;
+    const Rows<I>& fine = a.inner > b.inner ? b : a;
     TORCH_CHECK(coarse.outer == 1 && fine.inner > 0 && coarse.inner % fine.inner == 0, what,
                 " must be cut into rows alike; make one of them contiguous");
     coarse.outer = coarse.inner / fine.inner;
@@ -141,54 +162,56 @@ void rows_alike(Rows& a, Rows& b, const char* what)
     coarse.inner = fine.inner;
 }
 
-struct LogprobArgs {
+template <typename I> struct LogprobArgs {
     int dtype;
-    int64_t vocab, rows;
-    Rows l, a;
+    I vocab, rows;
+    Rows<I> l, a;
 };
-LogprobArgs logprob_args(const Tensor& logits, const Tensor& actions)
+template <typename I> LogprobArgs<I> logprob_args(const Tensor& logits, const Tensor& actions)
 {
-    LogprobArgs g;
+    LogprobArgs<I> g;
     g.dtype = dtype_code(logits, "logits");
     TORCH_CHECK(logits.dim() >= 1, "logits must have at least one dimension");
     TORCH_CHECK(actions.scalar_type() == torch::kInt64, "actions must be int64");
     TORCH_CHECK(actions.device() == logits.device(), "All tensors must be on same device");
     const int64_t lead = logits.dim() - 1;
-    TORCH_CHECK(actions.sizes() == logits.sizes().slice(0, lead), "actions must have the shape of logits without its last dimension");
-    g.vocab = logits.size(-1);
-    g.rows = actions.numel();
+    const auto sizes = Dims<I>::sizes(logits);
+    TORCH_CHECK(Dims<I>::sizes(actions) == sizes.slice(0, lead), "actions must have the shape of logits without its last dimension");
+    g.vocab = sizes[lead];
+    g.rows = Dims<I>::numel(actions);
     TORCH_CHECK(g.vocab > 0 || g.rows == 0, "logits must have at least one entry per row");
-    TORCH_CHECK(g.vocab <= 1 || logits.stride(-1) == 1, "the last dimension of logits must be contiguous");
+    TORCH_CHECK(g.vocab <= 1 || Dims<I>::strides(logits)[lead] == 1, "the last dimension of logits must be contiguous");
     if (g.rows > 0) {
-        g.l = rows_of(logits, lead, "logits");
-        g.a = rows_of(actions, lead, "actions");
-        rows_alike(g.l, g.a, "logits and actions");
+        g.l = rows_of<I>(logits, lead, "logits");
+        g.a = rows_of<I>(actions, lead, "actions");
+        rows_alike<I>(g.l, g.a, "logits and actions");
     }
     return g;
 }
 
 // (logprobs, entropy or an empty tensor, row_stats or an empty tensor; undefined tensors for those with `bare`)
+template <typename I>
 std::tuple<Tensor, Tensor, Tensor> logprobs_buffers(const Tensor& logits, const Tensor& actions, double temperature,
                                                     bool want_entropy, bool save, bool bare)
 {
     TORCH_CHECK(temperature > 0, "temperature must be positive");
     const auto opts = logits.options().dtype(torch::kFloat32);
-    return {torch::empty(actions.sizes(), opts),
-            want_entropy ? torch::empty(actions.sizes(), opts) : bare ? Tensor() : torch::empty({0}, opts),
-            save ? torch::empty({actions.numel(), 2}, opts) : bare ? Tensor() : torch::empty({0, 2}, opts)};
+    const auto sizes = Dims<I>::sizes(actions);
+    return {Dims<I>::empty(sizes, opts), want_entropy ? Dims<I>::empty(sizes, opts) : bare ? Tensor() : torch::empty({0}, opts),
+            save ? Dims<I>::empty({Dims<I>::numel(actions), 2}, opts) : bare ? Tensor() : torch::empty({0, 2}, opts)};
 }
 std::tuple<Tensor, Tensor, Tensor> logprobs_forward_meta(const Tensor& logits, const Tensor& actions, double temperature,
                                                          bool want_entropy, bool save)
 {
-    logprob_args(logits, actions);
-    return logprobs_buffers(logits, actions, temperature, want_entropy, save, false);
+    logprob_args<c10::SymInt>(logits, actions);
+    return logprobs_buffers<c10::SymInt>(logits, actions, temperature, want_entropy, save, false);
 }
 std::tuple<Tensor, Tensor, Tensor> logprobs_run(const Tensor& logits, const Tensor& actions, double temperature,
                                                 bool want_entropy, bool save, bool bare)
 {
-    const LogprobArgs g = logprob_args(logits, actions);
+    const auto g = logprob_args<int64_t>(logits, actions);
     const c10::cuda::CUDAGuard guard(logits.device());
-    auto out = logprobs_buffers(logits, actions, temperature, want_entropy, save, bare);
+    auto out = logprobs_buffers<int64_t>(logits, actions, temperature, want_entropy, save, bare);
     if (g.rows == 0) return out;
     check_rc(puff_policy_sm100_logprobs(logits.data_ptr(), g.dtype, ptr<const long long>(actions), g.l.outer, g.l.inner,
                                         g.vocab, g.l.outer_stride, g.l.inner_stride, g.a.outer_stride, g.a.inner_stride,
@@ -212,14 +235,14 @@ std::tuple<Tensor, Tensor, Tensor> logprobs_forward(const Tensor& logits, const 
 }
 std::tuple<Tensor, Tensor> action_logprobs_cuda(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
 {
-    // without entropy an undefined tensor, None in Python: an empty one would cost a tenth of a small call
+    // without entropy an undefined tensor, None in Python, here and below: an empty one would cost a tenth of a small call
     auto [logprobs, entropy, stats] = logprobs_run(logits, actions, temperature, want_entropy, false, true);
     return {logprobs, entropy};
 }
 std::tuple<Tensor, Tensor> action_logprobs_meta(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
 {
     auto out = logprobs_forward_meta(logits, actions, temperature, want_entropy, false);
-    return {std::get<0>(out), std::get<1>(out)};
+    return {std::get<0>(out), want_entropy ? std::get<1>(out) : Tensor()};
 }
 std::tuple<Tensor, Tensor> action_logprobs(const Tensor& logits, const Tensor& actions, double temperature, bool want_entropy)
 {
@@ -231,13 +254,13 @@ std::tuple<Tensor, Tensor> action_logprobs(const Tensor& logits, const Tensor& a
 Tensor logprobs_backward_meta(const Tensor& logits, const Tensor& actions, double, const Tensor&, const OptTensor&,
                               const Tensor&, const OptTensor&)
 {
-    logprob_args(logits, actions);
-    return torch::empty(logits.sizes(), logits.options());
+    logprob_args<c10::SymInt>(logits, actions);
+    return at::empty_symint(logits.sym_sizes(), logits.options());
 }
 Tensor logprobs_backward_cuda(const Tensor& logits, const Tensor& actions, double temperature, const Tensor& row_stats,
                               const OptTensor& entropy, const Tensor& dlogprobs, const OptTensor& dentropy)
 {
-    const LogprobArgs g = logprob_args(logits, actions);
+    const auto g = logprob_args<int64_t>(logits, actions);
     check_f32(row_stats, logits, {g.rows, 2}, "row_stats");
     check_f32(dlogprobs, logits, actions.sizes(), "dlogprobs");
     if (present(dentropy)) {
@@ -312,7 +335,7 @@ std::tuple<Tensor, Tensor> action_logprobs_autograd(const Tensor& logits, const 
     node->row_stats = SavedVariable(stats, false);
     if (want_entropy) node->entropy = SavedVariable(entropy, true);
     node->temperature = temperature;
-    return {logprobs, entropy};
+    return {logprobs, want_entropy ? entropy : Tensor()};
 }
 
 // ---- policy loss -------------------------------------------------------------------------------------------------
@@ -323,23 +346,25 @@ int reduction_code(c10::string_view reduction)
     return reduction == "token" ? PUFF_MEAN_TOKENS : PUFF_MEAN_SEQUENCES;
 }
 // one advantage per row?
+template <typename I>
 bool loss_args(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, const OptTensor& ref_logprobs,
                const OptTensor& entropy, const OptTensor& mask, double clip_low, double clip_high, double denominator)
 {
     TORCH_CHECK(logprobs.dim() == 2, "logprobs must be 2D [rows, steps]");
-    check_f32(logprobs, logprobs, logprobs.sizes(), "logprobs");
-    check_f32(old_logprobs, logprobs, logprobs.sizes(), "old_logprobs");
-    const int64_t rows = logprobs.size(0), steps = logprobs.size(1);
-    const bool per_row = advantages.dim() == 1 || (advantages.dim() == 2 && advantages.size(1) == 1 && steps != 1);
-    if (per_row && advantages.dim() == 2) check_f32(advantages, logprobs, {rows, 1}, "advantages");
-    else if (per_row) check_f32(advantages, logprobs, {rows}, "advantages");
-    else check_f32(advantages, logprobs, logprobs.sizes(), "advantages");
-    if (present(ref_logprobs)) check_f32(*ref_logprobs, logprobs, logprobs.sizes(), "ref_logprobs");
-    if (present(entropy)) check_f32(*entropy, logprobs, logprobs.sizes(), "entropy");
+    const auto sizes = Dims<I>::sizes(logprobs);
+    check_f32<I>(logprobs, logprobs, sizes, "logprobs");
+    check_f32<I>(old_logprobs, logprobs, sizes, "old_logprobs");
+    const I &rows = sizes[0], &steps = sizes[1];
+    const bool per_row = advantages.dim() == 1 || (advantages.dim() == 2 && Dims<I>::sizes(advantages)[1] == 1 && steps != 1);
+    if (per_row && advantages.dim() == 2) check_f32<I>(advantages, logprobs, {rows, 1}, "advantages");
+    else if (per_row) check_f32<I>(advantages, logprobs, {rows}, "advantages");
+    else check_f32<I>(advantages, logprobs, sizes, "advantages");
+    if (present(ref_logprobs)) check_f32<I>(*ref_logprobs, logprobs, sizes, "ref_logprobs");
+    if (present(entropy)) check_f32<I>(*entropy, logprobs, sizes, "entropy");
     if (present(mask)) {
         TORCH_CHECK(mask->device() == logprobs.device(), "All tensors must be on same device");
         TORCH_CHECK(mask->scalar_type() == torch::kBool, "mask must be bool");
-        TORCH_CHECK(mask->sizes() == logprobs.sizes(), "mask must have the shape of logprobs");
+        TORCH_CHECK(Dims<I>::sizes(*mask) == sizes, "mask must have the shape of logprobs");
         TORCH_CHECK(mask->is_contiguous(), "mask must be contiguous");
     }
     TORCH_CHECK(clip_low >= 0 && clip_high >= 0, "clip_low and clip_high must not be negative");
@@ -349,30 +374,33 @@ bool loss_args(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor&
 
 using LossOut = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 // (loss, ratio, stats, slope, row_scale, weight); the last three hold nothing unless `save` (undefined with `bare`)
+template <typename I>
 LossOut loss_buffers(const Tensor& logprobs, bool sequence, bool save, bool bare)
 {
     const auto opts = logprobs.options();
-    auto kept = [&](bool there, at::IntArrayRef sizes) {
-        return there ? torch::empty(sizes, opts) : bare ? Tensor() : torch::empty({0}, opts);
+    const auto sizes = Dims<I>::sizes(logprobs);
+    auto kept = [&](bool there, typename Dims<I>::Ref of) {
+        return there ? Dims<I>::empty(of, opts) : bare ? Tensor() : torch::empty({0}, opts);
     };
-    return {torch::empty({}, opts), torch::empty(logprobs.sizes(), opts), torch::empty({6}, opts), kept(save, logprobs.sizes()),
-            kept(save && sequence, {logprobs.size(0)}), kept(save, {1})};
+    return {torch::empty({}, opts), Dims<I>::empty(sizes, opts), torch::empty({6}, opts), kept(save, sizes),
+            kept(save && sequence, sizes.slice(0, 1)), kept(save, {1})};
 }
 LossOut loss_forward_meta(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
                           double clip_high, const OptTensor& ref_logprobs, double, const OptTensor& entropy, double,
                           const OptTensor& mask, c10::string_view reduction, double denominator, bool save)
 {
-    loss_args(logprobs, old_logprobs, advantages, ref_logprobs, entropy, mask, clip_low, clip_high, denominator);
-    return loss_buffers(logprobs, reduction_code(reduction) == PUFF_MEAN_SEQUENCES, save, false);
+    loss_args<c10::SymInt>(logprobs, old_logprobs, advantages, ref_logprobs, entropy, mask, clip_low, clip_high, denominator);
+    return loss_buffers<c10::SymInt>(logprobs, reduction_code(reduction) == PUFF_MEAN_SEQUENCES, save, false);
 }
 LossOut loss_run(const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages, double clip_low,
                           double clip_high, const OptTensor& ref_logprobs, double kl_coef, const OptTensor& entropy,
                  double ent_coef, const OptTensor& mask, c10::string_view reduction, double denominator, bool save, bool bare)
 {
-    const bool per_row = loss_args(logprobs, old_logprobs, advantages, ref_logprobs, entropy, mask, clip_low, clip_high, denominator);
+    const bool per_row =
+        loss_args<int64_t>(logprobs, old_logprobs, advantages, ref_logprobs, entropy, mask, clip_low, clip_high, denominator);
     const c10::cuda::CUDAGuard guard(logprobs.device());
     const bool sequence = reduction_code(reduction) == PUFF_MEAN_SEQUENCES;
-    LossOut out = loss_buffers(logprobs, sequence, save, bare);
+    LossOut out = loss_buffers<int64_t>(logprobs, sequence, save, bare);
     auto& [loss, ratio, stats, slope, row_scale, weight] = out;
     const int64_t rows = logprobs.size(0), steps = logprobs.size(1);
     const size_t sbytes = puff_policy_sm100_loss_scratch_bytes(rows, steps);
@@ -436,7 +464,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logprobs, const Ten
 std::tuple<Tensor, Tensor> loss_backward_meta(const Tensor& slope, const Tensor&, const Tensor&, const Tensor&,
                                               const OptTensor&, double, bool want_dentropy)
 {
-    return {torch::empty_like(slope), torch::empty(want_dentropy ? slope.sizes() : at::IntArrayRef({0}), slope.options())};
+    return {torch::empty_like(slope), want_dentropy ? torch::empty_like(slope) : torch::empty({0}, slope.options())};
 }
 std::tuple<Tensor, Tensor> loss_backward_cuda(const Tensor& slope, const Tensor& row_scale, const Tensor& weight,
                                               const Tensor& dloss, const OptTensor& mask, double ent_coef,
@@ -530,26 +558,30 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor& logprobs, 
 
 // ---- gated recurrence --------------------------------------------------------------------------------------------
 
-int check_resets(const OptTensor& resets, const Tensor& like, at::IntArrayRef sizes)
+template <typename I>
+int check_resets(const OptTensor& resets, const Tensor& like, typename Dims<I>::Ref sizes)
 {
     if (!present(resets)) return 0;
     const auto t = resets->scalar_type();
     TORCH_CHECK(resets->device() == like.device(), "All tensors must be on same device");
     TORCH_CHECK(t == torch::kFloat32 || t == torch::kBool || t == torch::kUInt8, "resets must be float32 or bool");
-    TORCH_CHECK(resets->sizes() == sizes, "resets must have shape ", sizes, ", got ", resets->sizes());
+    TORCH_CHECK(Dims<I>::sizes(*resets) == sizes, "resets must have shape ", sizes, ", got ", Dims<I>::sizes(*resets));
     TORCH_CHECK(resets->is_contiguous(), "resets must be contiguous");
     return t == torch::kFloat32 ? 4 : 1;
 }
-void recurrence_args(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, int64_t dims)
+// the size of an element of `resets`, 0 without
+template <typename I>
+int recurrence_args(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, int64_t dims)
 {
     dtype_code(gates, "gates");
     TORCH_CHECK(gates.dim() == dims, "gates must be ", dims == 3 ? "3D [batch, steps, channels]" : "2D [batch, channels]");
-    TORCH_CHECK(inputs.sizes() == gates.sizes() && inputs.scalar_type() == gates.scalar_type(),
+    const auto sizes = Dims<I>::sizes(gates);
+    TORCH_CHECK(Dims<I>::sizes(inputs) == sizes && inputs.scalar_type() == gates.scalar_type(),
                 "gates and inputs must have one shape and one type");
     TORCH_CHECK(inputs.device() == gates.device(), "All tensors must be on same device");
-    if (gates.numel() > 0 && gates.size(-1) > 1)
-        TORCH_CHECK(gates.stride(-1) == 1 && inputs.stride(-1) == 1, "the last dimension of gates and inputs must be contiguous");
-    check_resets(resets, gates, gates.sizes().slice(0, dims - 1));
+    if (Dims<I>::numel(gates) > 0 && sizes[dims - 1] > 1)
+        TORCH_CHECK(Dims<I>::strides(gates)[dims - 1] == 1 && Dims<I>::strides(inputs)[dims - 1] == 1, "the last dimension of gates and inputs must be contiguous");
+    return check_resets<I>(resets, gates, sizes.slice(0, dims - 1));
 }
 
 // the workspace of one call, or an undefined tensor where it needs none
@@ -561,26 +593,35 @@ Tensor recurrence_scratch(const Tensor& gates, size_t* bytes)
 
 using RecOut = std::tuple<Tensor, Tensor, Tensor>;
 // (outputs, final state, saved states or an empty tensor)
+template <typename I>
+RecOut recurrence_buffers(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const OptTensor& state, bool save,
+                          int* reset_bytes)
+{
+    *reset_bytes = recurrence_args<I>(gates, inputs, resets, 3);
+    const auto sizes = Dims<I>::sizes(gates);
+    const I &B = sizes[0], &T = sizes[1], &C = sizes[2];
+    if (present(state)) check_f32<I>(*state, gates, {B, C}, "state");
+    const auto f32 = gates.options().dtype(torch::kFloat32);
+    const I states = (T + (PUFF_RECURRENCE_SAVED_STEPS - 1)) / PUFF_RECURRENCE_SAVED_STEPS;
+    return {Dims<I>::empty(sizes, gates.options()), Dims<I>::empty({B, C}, f32), Dims<I>::empty({save ? B * states * C : I(0)}, f32)};
+}
 RecOut recurrence_forward_meta(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const OptTensor& state,
                                bool save)
 {
-    recurrence_args(gates, inputs, resets, 3);
-    const int64_t B = gates.size(0), T = gates.size(1), C = gates.size(2);
-    if (present(state)) check_f32(*state, gates, {B, C}, "state");
-    const auto f32 = gates.options().dtype(torch::kFloat32);
-    return {torch::empty({B, T, C}, gates.options()), torch::empty({B, C}, f32),
-            torch::empty({save ? puff_policy_sm100_recurrence_saved_floats(B, T, C) : 0}, f32)};
+    int reset_bytes;
+    return recurrence_buffers<c10::SymInt>(gates, inputs, resets, state, save, &reset_bytes);
 }
 RecOut recurrence_forward_cuda(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const OptTensor& state,
                                bool save)
 {
     const c10::cuda::CUDAGuard guard(gates.device());
-    RecOut out = recurrence_forward_meta(gates, inputs, resets, state, save);
+    int reset_bytes;
+    RecOut out = recurrence_buffers<int64_t>(gates, inputs, resets, state, save, &reset_bytes);
     auto& [outputs, final_state, saved] = out;
     size_t sbytes;
     const Tensor scratch = recurrence_scratch(gates, &sbytes);
     check_rc(puff_policy_sm100_recurrence(gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets),
-                                          check_resets(resets, gates, gates.sizes().slice(0, 2)), ptr<float>(state),
+                                          reset_bytes, ptr<float>(state),
                                           gates.size(0), gates.size(1), gates.size(2), gates.stride(0), gates.stride(1),
                                           inputs.stride(0), inputs.stride(1), outputs.data_ptr(), ptr<float>(final_state),
                                           save && saved.numel() > 0 ? ptr<float>(saved) : nullptr, ptr<void>(scratch), sbytes,
@@ -601,18 +642,26 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, const Tensor& i
 }
 
 // (dgates, dinputs, dstate)
+template <typename I>
+RecOut recurrence_gradients(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, int* reset_bytes)
+{
+    *reset_bytes = recurrence_args<I>(gates, inputs, resets, 3);
+    const auto sizes = Dims<I>::sizes(gates);
+    return {Dims<I>::empty(sizes, gates.options()), Dims<I>::empty(sizes, gates.options()),
+            Dims<I>::empty({sizes[0], sizes[2]}, gates.options().dtype(torch::kFloat32))};
+}
 RecOut recurrence_backward_meta(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const Tensor&,
                                 const OptTensor&, const OptTensor&)
 {
-    recurrence_args(gates, inputs, resets, 3);
-    return {torch::empty(gates.sizes(), gates.options()), torch::empty(gates.sizes(), gates.options()),
-            torch::empty({gates.size(0), gates.size(2)}, gates.options().dtype(torch::kFloat32))};
+    int reset_bytes;
+    return recurrence_gradients<c10::SymInt>(gates, inputs, resets, &reset_bytes);
 }
 RecOut recurrence_backward_cuda(const Tensor& gates, const Tensor& inputs, const OptTensor& resets, const Tensor& saved,
                                 const OptTensor& doutputs, const OptTensor& dfinal)
 {
     const c10::cuda::CUDAGuard guard(gates.device());
-    RecOut out = recurrence_backward_meta(gates, inputs, resets, saved, doutputs, dfinal);
+    int reset_bytes;
+    RecOut out = recurrence_gradients<int64_t>(gates, inputs, resets, &reset_bytes);
     const int64_t B = gates.size(0), T = gates.size(1), C = gates.size(2);
     check_f32(saved, gates, {puff_policy_sm100_recurrence_saved_floats(B, T, C)}, "saved");
     if (present(doutputs))
@@ -624,8 +673,8 @@ RecOut recurrence_backward_cuda(const Tensor& gates, const Tensor& inputs, const
     size_t sbytes;
     const Tensor scratch = recurrence_scratch(gates, &sbytes);
     check_rc(puff_policy_sm100_recurrence_backward(
-                 gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets),
-                 check_resets(resets, gates, gates.sizes().slice(0, 2)), ptr<const float>(saved), B, T, C, gates.stride(0),
+                 gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets), reset_bytes,
+                 ptr<const float>(saved), B, T, C, gates.stride(0),
                  gates.stride(1), inputs.stride(0), inputs.stride(1), ptr<void>(doutputs), ptr<float>(dfinal),
                  dgates.data_ptr(), dinputs.data_ptr(), ptr<float>(dstate), ptr<void>(scratch), sbytes, current_stream()),
              "puff_gated_recurrence_backward");
@@ -687,24 +736,25 @@ std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor& gates, const 
     return {outputs, final_state};
 }
 
-void step_args(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, const Tensor& new_state)
+template <typename I>
+int step_args(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, const Tensor& new_state)
 {
-    recurrence_args(gates, inputs, resets, 2);
-    check_f32(state, gates, gates.sizes(), "state");
-    check_f32(new_state, gates, gates.sizes(), "new_state");
+    check_f32<I>(state, gates, Dims<I>::sizes(gates), "state");
+    check_f32<I>(new_state, gates, Dims<I>::sizes(gates), "new_state");
+    return recurrence_args<I>(gates, inputs, resets, 2);
 }
 Tensor recurrence_step_meta(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, Tensor new_state)
 {
-    step_args(gates, inputs, state, resets, new_state);
-    return torch::empty(gates.sizes(), gates.options());
+    step_args<c10::SymInt>(gates, inputs, state, resets, new_state);
+    return at::empty_symint(gates.sym_sizes(), gates.options());
 }
 Tensor recurrence_step_cuda(const Tensor& gates, const Tensor& inputs, const Tensor& state, const OptTensor& resets, Tensor new_state)
 {
-    step_args(gates, inputs, state, resets, new_state);
+    const int reset_bytes = step_args<int64_t>(gates, inputs, state, resets, new_state);
     const c10::cuda::CUDAGuard guard(gates.device());
     Tensor outputs = torch::empty(gates.sizes(), gates.options());
     check_rc(puff_policy_sm100_recurrence_step(gates.data_ptr(), inputs.data_ptr(), dtype_code(gates, "gates"), ptr<void>(resets),
-                                               check_resets(resets, gates, gates.sizes().slice(0, 1)), ptr<const float>(state),
+                                               reset_bytes, ptr<const float>(state),
                                                gates.size(0), gates.size(1), gates.stride(0), inputs.stride(0),
                                                outputs.data_ptr(), ptr<float>(new_state), current_stream()),
              "puff_gated_recurrence_step");

@@ -159,3 +159,96 @@ def test_unpack_hooks_run_under_autograd():
             out = region(pb, t, w)
         out.sum().backward()
         assert len(seen) >= 3 and all(seen), which
+
+
+def traced(pb):
+    """name -> (function of one tensor whose first sizes change, the shapes it is called with)"""
+    def logprobs(z):
+        lp, h = pb.action_logprobs(z, torch.zeros(z.shape[:-1], dtype=torch.int64, device=M))
+        return lp.sum() + h.sum()
+
+    def logprobs_of_a_slice(z):
+        lp, h = pb.action_logprobs(z[:, :-1], torch.zeros(z.shape[:-1], dtype=torch.int64, device=M)[:, 1:], entropy=False)
+        assert h is None
+        return lp.sum()
+
+    def loss(lp):
+        out, ratio, stats = pb.policy_loss(lp, torch.empty_like(lp), torch.empty_like(lp), entropy=lp * 2, ent_coef=0.1,
+                                           mask=torch.ones_like(lp, dtype=torch.bool), reduction="sequence")
+        return out + (ratio.sum() + stats.sum()).detach()
+
+    def recurrence(g):
+        out, final = pb.gated_recurrence(g, g * 2, resets=torch.zeros(g.shape[:2], device=M),
+                                         state=torch.zeros(g.shape[0], g.shape[2], device=M))
+        return out.sum() + final.sum()
+
+    def halves(g):
+        gates, x = g.chunk(2, -1)
+        return pb.gated_recurrence(gates, x)[0].sum()
+
+    def step(g):
+        with torch.no_grad():
+            out, new = pb.gated_recurrence_step(g, g, torch.zeros_like(g), resets=torch.zeros(g.shape[0], device=M))
+        return out.sum() + new.sum()
+    return {"logprobs": (logprobs, [(4, 8), (6, 8), (9, 500)]), "logprobs 3d": (logprobs, [(4, 5, 8), (6, 3, 8), (2, 7, 700)]),
+            "logprobs of a slice": (logprobs_of_a_slice, [(4, 5, 8), (6, 3, 8), (2, 7, 700)]),
+            "loss": (loss, [(4, 6), (5, 6), (9, 17)]), "recurrence": (recurrence, [(2, 7, 8), (3, 9, 8), (5, 33, 20)]),
+            "halves": (halves, [(2, 7, 8), (3, 9, 8), (5, 33, 20)]), "step": (step, [(4, 8), (6, 8), (9, 20)])}
+
+
+NAMES = ["logprobs", "logprobs 3d", "logprobs of a slice", "loss", "recurrence", "halves", "step"]
+
+
+@pytest.mark.parametrize("which", NAMES)
+@pytest.mark.parametrize("dynamic", [None, True, False])
+def test_compiled_with_changing_shapes(which, dynamic):
+    """Traced ahead of time, forward and backward, with sizes as symbols from the second size on or from the first."""
+    import pufferlib_b200 as pb
+    f, shapes = traced(pb)[which]
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend="aot_eager", dynamic=dynamic, fullgraph=True)
+    for shape in shapes:
+        leaf = meta(*shape, grad=True)
+        out = compiled(leaf)
+        assert out.shape == ()
+        if which != "step":
+            assert torch.autograd.grad(out, leaf)[0].shape == shape
+    torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("which", NAMES)
+def test_traced_with_symbols(which):
+    """One trace holds for other sizes: nothing in it is a number that was a size."""
+    import pufferlib_b200 as pb
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, shapes = traced(pb)[which]
+
+    def both(leaf):
+        if which == "step":
+            return f(leaf)
+        leaf = leaf.detach().requires_grad_(True)
+        return torch.autograd.grad(f(leaf), leaf)[0]
+    graph = make_fx(both, tracing_mode="symbolic")(meta(*shapes[0]))
+    other = tuple(n + 3 for n in shapes[0][:-1]) + shapes[0][-1:]
+    assert graph(meta(*other)).shape == both(meta(*other)).shape
+
+
+def test_without_entropy_every_path_returns_none():
+    """The operator itself, with and without a graph, on tensors without data: as on the GPU."""
+    import pufferlib_b200  # noqa: F401
+    import pufferlib_b200 as pb
+    pb.action_logprobs(meta(4, 8), actions(4))
+    op = torch.ops.pufferlib.puff_action_logprobs
+    assert op(meta(4, 8), actions(4), 1.0, False)[1] is None
+    assert op(meta(4, 8, grad=True), actions(4), 1.0, False)[1] is None
+
+
+def test_shapes_are_still_refused_while_tracing():
+    import pufferlib_b200 as pb
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for f, shape in ((lambda z: pb.action_logprobs(z, actions(5))[0], (4, 8)),
+                     (lambda z: pb.policy_loss(z, meta(4, 5), meta(4, 6))[0], (4, 6)),
+                     (lambda z: pb.gated_recurrence(z, meta(2, 7, 9))[0], (2, 7, 8)),
+                     (lambda z: pb.gated_recurrence_step(z, z, meta(2, 9))[0], (2, 8))):
+        with pytest.raises(RuntimeError, match="shape"):
+            make_fx(f, tracing_mode="symbolic")(meta(*shape))
