@@ -38,6 +38,7 @@ extern "C" {
 #define PUFF_ERR_DEVICE_BOUNDS -11  /* debug builds (PUFF_DEBUG_BOUNDS): a kernel formed an out-of-range index (see _device_status) */
 #define PUFF_ERR_DTYPE        -12   /* unknown element type                       */
 #define PUFF_ERR_VALUE        -13   /* a scalar argument is outside its range     */
+#define PUFF_ERR_CUDA_BASE  -1000   /* this minus a CUDA error code, where a positive result says something else */
 
 /* ---- kernel variants ----------------------------------------------------- */
 #define PUFF_VARIANT_AUTO       0   /* pick from (num_segments, horizon, alignment): a bit-exact serial kernel,
@@ -338,8 +339,10 @@ int puff_priorities_sm100_weights_noalloc(const float* seg_abs_sum, float* weigh
  * A logit of -inf is an action that cannot be taken.  A row with nothing but
  * -inf has log-probability -inf, entropy 0 and no gradient.  actions[r] < 0
  * marks padding: log-probability and entropy 0, no gradient, whatever its logits
- * hold.  actions[r] >= vocab does the same and raises the flag that
- * puff_policy_sm100_bad_action() returns (and clears) after synchronising.
+ * hold.  actions[r] >= vocab does the same and raises a flag of the device:
+ * puff_policy_sm100_bad_action() synchronises the current device, clears its flag
+ * and returns 1 if it was raised, 0 if not, and PUFF_ERR_CUDA_BASE minus the CUDA
+ * error code if a CUDA call fails (an error of an earlier kernel included).
  *
  * _backward: dlogits (contiguous [outer * inner, vocab], every row written) =
  *     (dlogprobs (onehot - p) - dentropy p (log p + entropy)) / temperature

@@ -18,7 +18,7 @@ LIB_PATH = os.environ.get("PUFF_ADV_LIB") or os.path.join(_HERE, "libpuff_advant
 OK = 0
 ERR_NULL, ERR_SHAPE, ERR_VARIANT, ERR_ALIGN, ERR_ALIAS = -1, -2, -3, -4, -5
 ERR_ARCH, ERR_DRIVER, ERR_DEVICE_WAIT, ERR_WORKSPACE, ERR_SIZE, ERR_DEVICE_BOUNDS = -6, -7, -8, -9, -10, -11
-ERR_DTYPE, ERR_VALUE = -12, -13
+ERR_DTYPE, ERR_VALUE, ERR_CUDA_BASE = -12, -13, -1000
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 MEAN_TOKENS, MEAN_SEQUENCES = 0, 1
 NOALLOC_MAX_SEGMENTS = 524288

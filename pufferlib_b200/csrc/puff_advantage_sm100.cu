@@ -617,6 +617,7 @@ extern "C" const char* puff_advantage_sm100_strerror(int code)
         default: break;
     }
     if (code > 0) return cudaGetErrorString(static_cast<cudaError_t>(code));
+    if (code < PUFF_ERR_CUDA_BASE) return cudaGetErrorString(static_cast<cudaError_t>(PUFF_ERR_CUDA_BASE - code));
     return "unknown error code";
 }
 

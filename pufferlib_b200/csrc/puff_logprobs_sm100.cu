@@ -877,14 +877,12 @@ extern "C" int puff_policy_sm100_logprobs_backward(const void* logits, int dtype
 
 extern "C" int puff_policy_sm100_bad_action(void)
 {
+    int flag = 0;
     cudaError_t e = cudaDeviceSynchronize();
-    if (e != cudaSuccess) return static_cast<int>(e);
-    int h = 0;
-    e = cudaMemcpyFromSymbol(&h, g_bad_action, sizeof(int));
-    if (e != cudaSuccess) return static_cast<int>(e);
-    if (h != 0) {
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&flag, g_bad_action, sizeof(int));
+    if (e == cudaSuccess && flag != 0) {
         const int zero = 0;
-        cudaMemcpyToSymbol(g_bad_action, &zero, sizeof(int));
+        e = cudaMemcpyToSymbol(g_bad_action, &zero, sizeof(int));
     }
-    return h;
+    return e == cudaSuccess ? flag : PUFF_ERR_CUDA_BASE - static_cast<int>(e);
 }

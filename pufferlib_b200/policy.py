@@ -7,6 +7,8 @@ pufferlib/pytorch.py), as differentiable operators over the experience buffers'
 only, on the current stream of the tensors' device, and raise when the extension
 is missing.  No second derivatives.
 """
+import contextlib
+
 import torch
 
 from .advantage import _ops as _load_ops
@@ -35,10 +37,14 @@ def action_logprobs(logits, actions, temperature=1.0, entropy=True):
     return logprobs, ent if entropy else None
 
 
-def bad_action():
-    """Whether an action beyond the vocabulary was met since the last call (synchronises the device)."""
+def bad_action(device=None):
+    """Whether `action_logprobs` on `device` (default: the current one) has met an action beyond the vocabulary since
+    the last call for it.  Synchronises that device; an error of CUDA raises."""
     from . import cabi
-    code = cabi.load().puff_policy_sm100_bad_action()
+    with contextlib.nullcontext() if device is None else torch.cuda.device(device):
+        code = cabi.load().puff_policy_sm100_bad_action()
+    if code < 0:
+        cabi.check(code, "puff_policy_sm100_bad_action")
     return code != 0
 
 
