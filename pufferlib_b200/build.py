@@ -11,8 +11,10 @@ nvcc flags `-O3`), with the flags this implementation needs instead:
                                registration, linked against the library above
 
 Both land next to this file so that the package works from the source tree.
-Outputs are rebuilt only when a source is newer.
+Outputs are rebuilt only when a source is newer or when they were made under
+other settings (command, compiler, torch), which build/ keeps a record of.
 """
+import hashlib
 import os
 import shutil
 import subprocess
@@ -62,9 +64,36 @@ def _host_cxx():
     return "g++"
 
 
-def _stale(target, sources):
+def _settings(command, versions=()):
+    """What decides about a compiled file besides its sources: the command, the
+    compiler behind it and the versions of the libraries whose headers it reads.
+    None without that compiler: then only the age of what is there can be looked at."""
+    try:
+        compiler = subprocess.run([command[0], "--version"], capture_output=True, text=True).stdout
+    except OSError:
+        return None
+    return hashlib.sha256(repr([list(command), compiler, list(versions)]).encode()).hexdigest()
+
+
+def _record_of(target):
+    return os.path.join(OBJ_DIR, os.path.basename(target) + ".settings")
+
+
+def _record(target, settings):
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with open(_record_of(target) + f".{os.getpid()}", "w") as f:
+        f.write(settings)
+    os.replace(f.name, _record_of(target))
+
+
+def _stale(target, sources, settings=None):
+    """Older than a source, or recorded as made under other settings."""
     if not os.path.isfile(target):
         return True
+    if settings is not None and os.path.isfile(_record_of(target)):
+        with open(_record_of(target)) as f:
+            if f.read() != settings:
+                return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(s) > t for s in sources)
 
@@ -73,6 +102,18 @@ def _run(cmd, verbose):
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
+
+
+def _link(command, target, rest, settings, verbose):
+    """Under a name of its own first: a process that loads the library meanwhile, or another build, sees a whole one."""
+    part = f"{target}.{os.getpid()}.part"
+    try:
+        _run(command + ["-o", part] + rest, verbose)
+        os.replace(part, target)
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+    _record(target, settings)
 
 
 def build_debug_cabi(out_path, verbose=False):
@@ -85,25 +126,36 @@ def build_debug_cabi(out_path, verbose=False):
     return out_path
 
 
-def _objects(sources, deps_of_all, command, force, verbose):
-    """Compile each source to build/<name>.o unless the object is newer than the
-    source and every file of `deps_of_all`; stale ones are compiled side by side."""
+def _objects(sources, deps_of_all, command, force, verbose, versions=(), also=()):
+    """Compile each source to build/<name>.<settings>.o unless that object is newer
+    than the source and every file of `deps_of_all`; stale ones are compiled side by
+    side.  `also`: flags that leave the object as it is (what the compiler prints)."""
     os.makedirs(OBJ_DIR, exist_ok=True)
+    settings = (_settings(command, versions) or "unknown")[:12]
     objects, running = [], []
     for name in sources:
-        src, obj = os.path.join(CSRC, name), os.path.join(OBJ_DIR, name + ".o")
+        src, obj = os.path.join(CSRC, name), os.path.join(OBJ_DIR, f"{name}.{settings}.o")
         objects.append(obj)
         if force or _stale(obj, [src] + deps_of_all):
-            cmd = command + ["-c", "-o", obj, src]
+            part = f"{obj}.{os.getpid()}.part"
+            cmd = command + list(also) + ["-c", "-o", part, src]
             if verbose:
                 print(" ".join(cmd), flush=True)
-            running.append((cmd, obj, subprocess.Popen(cmd)))
-    failed = [(cmd, obj) for cmd, obj, proc in running if proc.wait() != 0]
-    for _, obj in failed:
-        if os.path.exists(obj):
-            os.remove(obj)
+            running.append((cmd, part, obj, subprocess.Popen(cmd)))
+    failed = None
+    for cmd, part, obj, proc in running:
+        if proc.wait() == 0:
+            os.replace(part, obj)
+        else:
+            failed = failed or cmd
+            if os.path.exists(part):
+                os.remove(part)
     if failed:
-        raise subprocess.CalledProcessError(1, failed[0][0])
+        raise subprocess.CalledProcessError(1, failed)
+    for name in sources:        # objects of settings that are gone
+        for old in os.listdir(OBJ_DIR):
+            if old.startswith(name + ".") and old.endswith(".o") and os.path.join(OBJ_DIR, old) not in objects:
+                os.remove(os.path.join(OBJ_DIR, old))
     return objects
 
 
@@ -111,12 +163,12 @@ def build_cabi(force=False, verbose=False, ptxas_info=False):
     headers = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cuh")]
     headers.append(os.path.join(INCLUDE, "puff_advantage.h"))
     sources = [os.path.join(CSRC, s) for s in CU_SOURCES]
-    if force or _stale(CABI_LIB, sources + headers):
+    settings = _settings([NVCC] + NVCC_FLAGS)
+    if force or ptxas_info or _stale(CABI_LIB, sources + headers, settings):
         flags = [f for f in NVCC_FLAGS if f != "-shared"]
-        if ptxas_info:
-            flags += ["-Xptxas", "-v"]
-        objects = _objects(CU_SOURCES, headers, [NVCC] + flags, force, verbose)
-        _run([NVCC] + NVCC_FLAGS + ["-o", CABI_LIB] + objects, verbose)
+        objects = _objects(CU_SOURCES, headers, [NVCC] + flags, force or ptxas_info, verbose,
+                           also=["-Xptxas", "-v"] if ptxas_info else [])
+        _link([NVCC] + NVCC_FLAGS, CABI_LIB, objects, settings, verbose)
     return CABI_LIB
 
 
@@ -125,19 +177,21 @@ def build_torch_ext(force=False, verbose=False):
     from torch.utils.cpp_extension import include_paths, library_paths
     header = os.path.join(INCLUDE, "puff_advantage.h")
     deps = [os.path.join(CSRC, s) for s in TORCH_SOURCES] + [header, CABI_LIB]
-    if force or _stale(TORCH_EXT, deps):
-        cxx = _host_cxx()
-        inc = [f"-I{p}" for p in include_paths()]
-        inc += [f"-I{os.path.join(CUDA_HOME, 'include')}", f"-I{sysconfig.get_paths()['include']}"]
-        libdir = library_paths()[0]
-        flags = [cxx, "-O2", "-std=c++17", "-fPIC",
-                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-                 "-DTORCH_EXTENSION_NAME=_C"] + inc
-        objects = _objects(TORCH_SOURCES, [header], flags, force, verbose)
-        _run([cxx, "-shared", "-o", TORCH_EXT] + objects + [
+    cxx = _host_cxx()
+    inc = [f"-I{p}" for p in include_paths()]
+    inc += [f"-I{os.path.join(CUDA_HOME, 'include')}", f"-I{sysconfig.get_paths()['include']}"]
+    libdir = library_paths()[0]
+    flags = [cxx, "-O2", "-std=c++17", "-fPIC",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             "-DTORCH_EXTENSION_NAME=_C"] + inc
+    versions = [torch.__version__, torch.version.cuda]
+    settings = _settings(flags, versions)
+    if force or _stale(TORCH_EXT, deps, settings):
+        objects = _objects(TORCH_SOURCES, [header], flags, force, verbose, versions)
+        _link([cxx, "-shared"], TORCH_EXT, objects + [
               f"-L{HERE}", "-lpuff_advantage_sm100", "-Wl,-rpath,$ORIGIN",
               f"-L{libdir}", f"-Wl,-rpath,{libdir}",
-              "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"], verbose)
+              "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"], settings, verbose)
     return TORCH_EXT
 
 
