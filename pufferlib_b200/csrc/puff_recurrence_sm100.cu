@@ -11,7 +11,7 @@
 //
 // Memory-bound: three elements moved a step forward, five backward; the arithmetic behind them, two special functions and
 // some twenty instructions a step for two channels, is close to the bound, so what surrounds it (addresses, joins, waits)
-// decides.  8192 x 64 x 128 bf16: 76 us forward (5.3 TB/s of 6.55) and 117 backward (5.7); fp32 125 and 211 (6.4);
+// decides.  8192 x 64 x 128 bf16: 79 us forward (5.1 TB/s of 6.55) and 117 backward (5.7); fp32 125 and 211 (6.4);
 // 256 x 4096 x 128 fp32 281 and 453.  One thread a channel, step after step, took 1904 us for the first pair.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -54,9 +54,11 @@ __device__ __forceinline__ bool is_reset(const RecArgs& p, long long i)
     return p.reset_bytes == 1 && static_cast<const unsigned char*>(p.resets)[i] != 0;
 }
 
-// keep = sigmoid(g) and take = 1 - keep = sigmoid(-g).  The smaller of the two is 1 / (1 + e^|g|), good to a few
-// ulp however small; the larger is 1 minus it, so that the two add up to 1 and the state stays a weighted mean.
-// One register, the code, holds both: the smaller one with the sign of g.
+// keep = sigmoid(g) and take = 1 - keep = sigmoid(-g).  The smaller of the two is 1 / (1 + e^|g|), good to 8 half steps
+// of fp32 (4 of ex2.approx, 2 of rcp.approx, 1 each of what surrounds them) down to 2^-126, below which it is 0; the
+// larger is 1 minus it, so that the two add up to 1 and the state stays a weighted mean.  e^h = 2^t (1 + r) with
+// t = h log2(e) rounded and r = h - t ln 2 what the rounding left out, which grows with h: without it the gate is 8 half
+// steps further off at 10, 63 at 85 (it costs 8192 x 64 x 128 bf16 3 us of 79 forward, none backward).  One register, the code, holds both gates: the smaller one with the sign of g.
 __device__ __forceinline__ float rcp_approx(float x)
 {
     float y;
@@ -96,15 +98,25 @@ __device__ __forceinline__ void v_add(float (&d)[VEC], const float (&a)[VEC], co
         d[0] = a[0] + b[0];
     }
 }
+constexpr float kLn2High = 0.693147182464599609375f, kLn2Low = -1.904654299957768e-09f;    // ln 2 in 48 bits
 template <int VEC>
 __device__ __forceinline__ void gate_codes(const float (&g)[VEC], float (&code)[VEC])
 {
-    float e[VEC], one[VEC], d[VEC];
+    float h[VEC], t[VEC], e[VEC], r[VEC], one[VEC], d[VEC], log2e[VEC], high[VEC], low[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        e[v] = exp2_approx(fabsf(g[v]) * kLog2e);
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(h[v]) : "f"(fabsf(g[v])), "f"(88.0f));     // e^88 is finite, its reciprocal 0
+        log2e[v] = kLog2e;
+        high[v] = -kLn2High;
+        low[v] = -kLn2Low;
         one[v] = 1.0f;
     }
+    v_mul(t, h, log2e);
+    v_fma(r, t, high, h);
+    v_fma(r, t, low, r);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) e[v] = exp2_approx(t[v]);
+    v_fma(e, e, r, e);
     v_add(d, e, one);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) code[v] = copysignf(rcp_approx(d[v]), g[v]);
