@@ -225,7 +225,7 @@ static void tune_init()
                                                            "PUFF_ADV_CTAS_PER_SM", "PUFF_ADV_GROUP",
                                                            "PUFF_ADV_SCAN_THREADS", "PUFF_ADV_RESERVE_SMS",
                                                            "PUFF_ADV_TILE_ROWS", "PUFF_ADV_PDL", "PUFF_ADV_SCAN_WIDE",
-                                                           "PUFF_ADV_B1_WARP_TEAMS"};
+                                                           "PUFF_ADV_B1_WARP_TEAMS", "PUFF_ADV_TILE_WAIT_US"};
         for (int i = 0; i < PUFF_TUNE_COUNT; ++i) {
             const char* v = getenv(names[i]);
             g_tune[i].store((v != nullptr && *v != '\0') ? atoi(v) : -1, std::memory_order_relaxed);

@@ -34,6 +34,7 @@ struct RecArgs {
     long long batch, steps, channels;
     long long gates_batch_stride, gates_step_stride, inputs_batch_stride, inputs_step_stride;
     int reset_bytes;
+    unsigned wait_ns;        // how long to wait for a tile
 };
 
 // How the work is cut.  A warp owns 32 lanes of VEC channels and walks 16 steps at a time, all of them in registers.
@@ -1017,7 +1018,7 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
                                             float* saved, void* scratch, size_t scratch_bytes, void* cuda_stream)
 {
     RecArgs p = {gates, inputs, resets, state, batch, steps, channels, gates_batch_stride, gates_step_stride,
-                 inputs_batch_stride, inputs_step_stride, resets != nullptr ? reset_bytes : 0};
+                 inputs_batch_stride, inputs_step_stride, resets != nullptr ? reset_bytes : 0, 0u};
     int rc = check_recurrence(p, dtype);
     if (rc != PUFF_OK) return rc;
     const long long lanes = batch * channels, n = lanes * steps;
@@ -1062,6 +1063,7 @@ extern "C" int puff_policy_sm100_recurrence(const void* gates, const void* input
     if (tma) {
         int* status = device_status_ptr();
         if (status == nullptr) return PUFF_ERR_DRIVER;
+        p.wait_ns = tile_wait_ns();
         const size_t smem = tma_smem(2, kTmaForwardStages);
 #define PUFF_RUN2(T, VEC)                                                                                                \
     (plan.shares > 1                                                                                                     \
@@ -1094,7 +1096,7 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
                                                      void* scratch, size_t scratch_bytes, void* cuda_stream)
 {
     RecArgs p = {gates, inputs, resets, nullptr, batch, steps, channels, gates_batch_stride, gates_step_stride,
-                 inputs_batch_stride, inputs_step_stride, resets != nullptr ? reset_bytes : 0};
+                 inputs_batch_stride, inputs_step_stride, resets != nullptr ? reset_bytes : 0, 0u};
     int rc = check_recurrence(p, dtype);
     if (rc != PUFF_OK) return rc;
     const long long lanes = batch * channels, n = lanes * steps;
@@ -1146,6 +1148,7 @@ extern "C" int puff_policy_sm100_recurrence_backward(const void* gates, const vo
     if (tma) {
         int* status = device_status_ptr();
         if (status == nullptr) return PUFF_ERR_DRIVER;
+        p.wait_ns = tile_wait_ns();
         const size_t smem = tma_smem(3, kTmaBackwardStages);
 #define PUFF_RUN2(T, VEC)                                                                                                \
     (plan.shares > 1                                                                                                     \
@@ -1178,7 +1181,7 @@ extern "C" int puff_policy_sm100_recurrence_step(const void* gates, const void* 
                                                  void* outputs, float* new_state, void* cuda_stream)
 {
     RecArgs p = {gates, inputs, resets, nullptr, batch, 1, channels, gates_stride, channels, inputs_stride, channels,
-                 resets != nullptr ? reset_bytes : 0};
+                 resets != nullptr ? reset_bytes : 0, 0u};
     int rc = check_recurrence(p, dtype);
     if (rc != PUFF_OK) return rc;
     const long long n = batch * channels;

@@ -10,7 +10,8 @@ namespace puff {
 constexpr int kTmaTileBytes = kRecTile * 128;
 constexpr int kTmaForwardStages = 3, kTmaBackwardStages = 2;
 
-// bounded, as every wait of the library: 2^24 polls or 2 s, then the status word and no further waiting
+// every wait is bounded: 2^24 polls or kTileWaitNs
+constexpr unsigned kTileWaitNs = 2000000000u;
 struct TileBarrier {
     uint32_t at;
     __device__ __forceinline__ void init() const { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at) : "memory"); }
@@ -18,25 +19,27 @@ struct TileBarrier {
     {
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at), "r"(bytes) : "memory");
     }
-    __device__ __forceinline__ bool passed(uint32_t parity) const
+    __device__ __forceinline__ bool passed(uint32_t parity, unsigned hint_ns) const
     {
         uint32_t ok;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
-                     : "=r"(ok) : "r"(at), "r"(parity), "r"(200000u) : "memory");
+                     : "=r"(ok) : "r"(at), "r"(parity), "r"(hint_ns) : "memory");
         return ok != 0;
     }
-    __device__ __forceinline__ void wait(uint32_t parity, bool& given_up, int* status) const
+    // (with no time at all it does not even look, so that a test gives up whatever has arrived)
+    __device__ __forceinline__ bool wait(uint32_t parity, unsigned limit_ns) const
     {
-        if (given_up || passed(parity)) return;
+        const unsigned hint = limit_ns < 200000u ? limit_ns : 200000u;
+        if (limit_ns == 0) return false;
+        if (passed(parity, hint)) return true;
         unsigned long long start, now;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
         for (uint32_t polls = 0; polls < (1u << 24); ++polls) {
-            if (passed(parity)) return;
+            if (passed(parity, hint)) return true;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-            if (now - start > 2000000000ull) break;
+            if (now - start > limit_ns) break;
         }
-        given_up = true;
-        atomicExch(status, PUFF_ERR_DEVICE_WAIT);
+        return false;
     }
 };
 __device__ __forceinline__ void tile_load(uint32_t to, const CUtensorMap* map, int c, int t, int b, TileBarrier bar)
@@ -100,7 +103,27 @@ struct TileRing {
         }
         tile_fence();
     }
+    // The warp waits for its tile in `stage`.  If one of its lanes gives up, all do: the status word is set, nothing is
+    // requested or waited for any more (what the kernel computes from then on counts for nothing, but the other warps of
+    // its group meet it at their joins), and first what is in flight has to arrive, this tile and, if `next`, the one
+    // behind it: it writes to shared memory, which must not be left before.
+    __device__ __forceinline__ void wait(int stage, uint32_t phase, bool next, unsigned limit_ns, bool& given_up, int* status) const
+    {
+        if (given_up) return;
+        const bool ok = bar(stage).wait(phase, limit_ns);
+        if (__all_sync(0xffffffffu, ok)) return;
+        given_up = true;
+        if ((threadIdx.x & 31) == 0) atomicExch(status, PUFF_ERR_DEVICE_WAIT);
+        bar(stage).wait(phase, kTileWaitNs);
+        if (next) bar(stage == STAGES - 1 ? 0 : stage + 1).wait(stage == STAGES - 1 ? phase ^ 1u : phase, kTileWaitNs);
+        __syncwarp();
+    }
 };
+static unsigned tile_wait_ns()
+{
+    const int us = tune_value(PUFF_TUNE_TILE_WAIT_US, -1);
+    return us < 0 || us > 2000000 ? kTileWaitNs : 1000u * static_cast<unsigned>(us);
+}
 
 // Forward: three stages, so that two tiles are on their way while one is worked on; the states take the inputs' place.
 template <typename T, int VEC, RecMode MODE>
@@ -123,8 +146,9 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
     const long long tiles = (p.steps + kRecTile - 1) / kRecTile;
     const int step = kRecTile * plan.warps * plan.shares, c0 = static_cast<int>(q.c) - q.lane * VEC, b0 = static_cast<int>(q.b);
     const int t_end = static_cast<int>(q.t_end), t_begin = static_cast<int>(q.t_begin);
+    bool given_up = false;
     auto request = [&](int t, int stage) {      // the tile of this warp in the round that begins at t
-        if (q.lane == 0 && t < t_end) {
+        if (q.lane == 0 && t < t_end && !given_up) {
             const TileBarrier bar = ring.bar(stage);
             bar.expect(2 * kTmaTileBytes);
             tile_load(ring.at(stage, 0), &gates, c0, t + q.slot * kRecTile, b0, bar);
@@ -150,13 +174,12 @@ puff_recurrence_tma_kernel(const __grid_constant__ CUtensorMap gates, const __gr
     float* save = saved != nullptr ? saved + (q.b * tiles + t0 / kRecTile) * p.channels + q.c : nullptr;
     int stage = 0, parity = 0;
     uint32_t phase = 0;
-    bool given_up = false;
     for (int t = t_begin; t < t_end; t += step, t0 += step, parity ^= 1) {
         const int n = q.steps_at(t0);
         const unsigned cut = reset_mask<false>(p, resets);
         const bool plain = n == kRecTile && cut == 0;
         resets = resets_ahead<false>(p, q, t0 + step, q.steps_at(t0 + step));
-        ring.bar(stage).wait(phase, given_up, status);
+        ring.wait(stage, phase, t + step < t_end, p.wait_ns, given_up, status);
         uint32_t* const g_words = ring.words(stage, 0);
         uint32_t* const x_words = ring.words(stage, 1);
         const TmaTile<Raw> raw_g = {g_words}, raw_x = {x_words};
@@ -228,8 +251,9 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
     const int step = kRecTile * plan.warps * plan.shares, c0 = static_cast<int>(q.c) - q.lane * VEC, b0 = static_cast<int>(q.b);
     const int t_begin = static_cast<int>(q.t_begin);
     const int first = t_begin + (static_cast<int>(q.t_end) - t_begin - 1) / step * step;
+    bool given_up = false;
     auto request = [&](int t, int stage) {
-        if (q.lane == 0 && t >= t_begin) {
+        if (q.lane == 0 && t >= t_begin && !given_up) {
             const TileBarrier bar = ring.bar(stage);
             bar.expect(A * kTmaTileBytes);
             tile_load(ring.at(stage, 0), &gates, c0, t + q.slot * kRecTile, b0, bar);
@@ -260,7 +284,6 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
                 if (q.ok) carry[v] = apply_pair(pairs[r * lanes + q.index + v], carry[v]);
     int stage = 0;
     uint32_t phase = 0;
-    bool given_up = false;
     for (int t = first; t >= t_begin; t -= step) {
         const int t0 = t + q.slot * kRecTile, t1 = t0 - step;
         const int n = q.steps_at(t0);
@@ -271,7 +294,8 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
         const bool plain = n == kRecTile && cut == 0;
         saved_before(t1);
         resets = t1 >= t_begin ? resets_ahead<false>(p, q, t1, q.steps_at(t1)) : 0u;
-        ring.bar(stage).wait(phase, given_up, status);
+        // (the tile behind this one is requested below, but for the first round's and where nothing has to be stored first)
+        ring.wait(stage, phase, t - step >= t_begin && (MODE == kSummary || t == first), p.wait_ns, given_up, status);
         const TmaTile<Raw> raw_g = {ring.words(stage, 0)}, raw_d = {ring.words(stage, 1)}, raw_x = {ring.words(stage, A - 1)};
         float code[kRecTile][VEC], slope[kRecTile][VEC];
         if (MODE == kSummary) {
