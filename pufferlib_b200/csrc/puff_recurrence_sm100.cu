@@ -17,6 +17,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/puff_advantage.h"
 #include "puff_policy.cuh"
 
@@ -57,9 +59,7 @@ __device__ __forceinline__ bool is_reset(const RecArgs& p, long long i)
 
 // keep = sigmoid(g) and take = 1 - keep = sigmoid(-g).  The smaller of the two is 1 / (1 + e^|g|), good to 8 half steps
 // of fp32 (4 of ex2.approx, 2 of rcp.approx, 1 each of what surrounds them) down to 2^-126, below which it is 0; the
-// larger is 1 minus it, so that the two add up to 1 and the state stays a weighted mean.  e^h = 2^t (1 + r) with
-// t = h log2(e) rounded and r = h - t ln 2 what the rounding left out, which grows with h: without it the gate is 8 half
-// steps further off at 10, 63 at 85 (it costs 8192 x 64 x 128 bf16 3 us of 79 forward, none backward).  One register, the code, holds both gates: the smaller one with the sign of g.
+// larger is 1 minus it, so that the two add up to 1 and the state stays a weighted mean.  One register, the code, holds both gates: the smaller one with the sign of g.
 __device__ __forceinline__ float rcp_approx(float x)
 {
     float y;
@@ -99,22 +99,39 @@ __device__ __forceinline__ void v_add(float (&d)[VEC], const float (&a)[VEC], co
         d[0] = a[0] + b[0];
     }
 }
-constexpr float kLn2High = 0.693147182464599609375f, kLn2Low = -1.904654299957768e-09f;    // ln 2 in 48 bits
-template <int VEC>
+// e^h, h = |g|, as 2^t (1 + r): t is h log2(e), r what t leaves out of it.  Rounded once and without r the gate is 8 half steps
+// further off at 10, 63 at 85.  A bf16 value has 8 bits, so that its product with the upper 16 of log2(e) is exact, and r
+// is h times the rest of it, tilted so that 1 + r stays within 0.3 half steps of e^r up to 88.  Other types: t rounded, and
+// r = h - t ln 2 with ln 2 in 48 bits; there h ends at 88, where e^h is finite still and its reciprocal 0 already.
+// (bf16 forward, without r, with the first form, with the second: 8192 x 64 x 128 77, 79, 80 us; 6525 x 8 x 1888 172, 176,
+// 178; 4 x 8192 x 1024 70, 75, 76.)
+constexpr float kLog2eUpper = 1.44268798828125f, kLog2eRest = 4.889379397354787e-06f;
+constexpr float kLn2High = 0.693147182464599609375f, kLn2Low = -1.904654299957768e-09f;
+template <typename T, int VEC>
 __device__ __forceinline__ void gate_codes(const float (&g)[VEC], float (&code)[VEC])
 {
-    float h[VEC], t[VEC], e[VEC], r[VEC], one[VEC], d[VEC], log2e[VEC], high[VEC], low[VEC];
+    float t[VEC], e[VEC], r[VEC], one[VEC], d[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        asm("min.NaN.f32 %0, %1, %2;" : "=f"(h[v]) : "f"(fabsf(g[v])), "f"(88.0f));     // e^88 is finite, its reciprocal 0
-        log2e[v] = kLog2e;
-        high[v] = -kLn2High;
-        low[v] = -kLn2Low;
-        one[v] = 1.0f;
+    for (int v = 0; v < VEC; ++v) one[v] = 1.0f;
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            t[v] = fabsf(g[v]) * kLog2eUpper;
+            r[v] = fabsf(g[v]) * kLog2eRest;
+        }
+    } else {
+        float h[VEC], log2e[VEC], high[VEC], low[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            asm("min.NaN.f32 %0, %1, %2;" : "=f"(h[v]) : "f"(fabsf(g[v])), "f"(88.0f));
+            log2e[v] = kLog2e;
+            high[v] = -kLn2High;
+            low[v] = -kLn2Low;
+        }
+        v_mul(t, h, log2e);
+        v_fma(r, t, high, h);
+        v_fma(r, t, low, r);
     }
-    v_mul(t, h, log2e);
-    v_fma(r, t, high, h);
-    v_fma(r, t, low, r);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) e[v] = exp2_approx(t[v]);
     v_fma(e, e, r, e);
@@ -277,14 +294,15 @@ __device__ __forceinline__ void group_barrier(int group, int warps)
 }
 
 // ---- what a warp does with a tile in registers.  PLAIN: sixteen steps, none a reset (for any lane of the warp).
-template <typename L, int VEC, bool PLAIN>
-__device__ __forceinline__ void tile_gates(const typename L::Raw& raw_g, const typename L::Raw& raw_x, bool there, float (&keep)[VEC],
+template <typename T, int VEC, bool PLAIN>
+__device__ __forceinline__ void tile_gates(const typename Lane<T, VEC>::Raw& raw_g, const typename Lane<T, VEC>::Raw& raw_x, bool there, float (&keep)[VEC],
                                            float (&fresh)[VEC])
 {
+    using L = Lane<T, VEC>;
     float g[VEC], x[VEC], code[VEC], take[VEC];
     L::get(raw_g, g);
     L::get(raw_x, x);
-    gate_codes(g, code);
+    gate_codes<T>(g, code);
     if (!PLAIN && !there)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) code[v] = kHold;
@@ -307,7 +325,7 @@ __device__ __forceinline__ void forward_stream(const Tile& raw_g, const Tile& ra
 #pragma unroll
     for (int j = 0; j < kRecTile; ++j, out += stride) {
         float keep[VEC], fresh[VEC];
-        tile_gates<L, VEC, PLAIN>(raw_g[j], raw_x[j], j < n, keep, fresh);
+        tile_gates<T, VEC, PLAIN>(raw_g[j], raw_x[j], j < n, keep, fresh);
         advance<VEC, PLAIN>(h, keep, fresh, (cut >> j) & 1u);
         if (ok && (PLAIN || j < n)) *reinterpret_cast<typename L::Raw*>(out) = L::put(h);
     }
@@ -318,7 +336,7 @@ __device__ __forceinline__ void forward_pair(const Tile& raw_g, const Tile& raw_
 {
 #pragma unroll
     for (int j = 0; j < kRecTile; ++j) {
-        tile_gates<Lane<T, VEC>, VEC, PLAIN>(raw_g[j], raw_x[j], j < n, keep[j], fresh[j]);
+        tile_gates<T, VEC, PLAIN>(raw_g[j], raw_x[j], j < n, keep[j], fresh[j]);
         if (j == 0) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
@@ -512,7 +530,7 @@ __device__ __forceinline__ void backward_states(const Tile& raw_g, const Tile& r
         float g[VEC], x[VEC], keep[VEC], take[VEC], fresh[VEC], minus[VEC], diff[VEC], product[VEC];
         L::get(raw_g[j], g);
         L::get(raw_x[j], x);
-        gate_codes(g, code[j]);
+        gate_codes<T>(g, code[j]);
         const bool reset = !PLAIN && (cut >> j) & 1u;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -630,7 +648,7 @@ puff_recurrence_backward_kernel(RecArgs p, RecPlan plan, float2* pairs, const fl
             for (int j = 0; j < kRecTile; ++j) {
                 float g[VEC];
                 L::get(raw_g[j], g);
-                gate_codes(g, code[j]);
+                gate_codes<T>(g, code[j]);
                 if (j >= n)
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) code[j][v] = kHold;
@@ -695,7 +713,7 @@ puff_recurrence_step_kernel(const T* __restrict__ gates, const T* __restrict__ i
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             float g[1] = {to_f32(gate.v[v])}, code[1], keep[1], take[1];
-            gate_codes(g, code);
+            gate_codes<T>(g, code);
             gate_pairs(code, keep, take);
             const float fresh = take[0] * to_f32(input.v[v]);
             after.v[v] = reset ? fresh : fmaf(keep[0], before.v[v], fresh);
@@ -760,7 +778,7 @@ puff_recurrence_short_kernel(RecArgs p, T* __restrict__ outputs, float* __restri
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 float g[1] = {to_f32(gate[j].v[v])}, code[1], keep[1], take[1];
-                gate_codes(g, code);
+                gate_codes<T>(g, code);
                 gate_pairs(code, keep, take);
                 const float fresh = take[0] * to_f32(input[j].v[v]);
                 h.v[v] = cut >> j & 1u ? fresh : fmaf(keep[0], h.v[v], fresh);
@@ -796,7 +814,7 @@ puff_recurrence_backward_short_kernel(RecArgs p, const float* __restrict__ saved
             for (int v = 0; v < VEC; ++v) {
                 const float x = to_f32(input[j].v[v]);
                 float g[1] = {to_f32(gate[j].v[v])}, cd[1], keep[1], take[1];
-                gate_codes(g, cd);
+                gate_codes<T>(g, cd);
                 gate_pairs(cd, keep, take);
                 if (cut >> j & 1u) h[v] = 0.0f;
                 code[j][v] = cd[0];

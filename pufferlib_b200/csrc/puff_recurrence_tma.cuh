@@ -303,7 +303,7 @@ puff_recurrence_backward_tma_kernel(const __grid_constant__ CUtensorMap gates, c
             for (int j = 0; j < kRecTile; ++j) {
                 float g[VEC];
                 L::get(raw_g[j], g);
-                gate_codes(g, code[j]);
+                gate_codes<T>(g, code[j]);
                 if (j >= n)
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) code[j][v] = kHold;
