@@ -335,7 +335,9 @@ int puff_priorities_sm100_weights_noalloc(const float* seg_abs_sum, float* weigh
  * Rows are addressed as [outer, inner] with a stride each, in elements, so that
  * a slice of [sequences, steps, vocab] needs no copy; the elements of a row are
  * adjacent.  entropy (nullable), logprobs: fp32 [outer * inner], contiguous.
- * row_stats (nullable): 2 fp32 per row for the backward pass, 8-byte aligned.
+ * row_stats (nullable): 2 fp32 per row for the backward pass, 8-byte aligned; for
+ * vocab <= PUFF_LOGPROBS_STATS_ABOVE they are neither written here nor read there,
+ * though _backward wants an address all the same.
  * A logit of -inf is an action that cannot be taken.  A row with nothing but
  * -inf has log-probability -inf, entropy 0 and no gradient.  actions[r] < 0
  * marks padding: log-probability and entropy 0, no gradient, whatever its logits
@@ -348,6 +350,7 @@ int puff_priorities_sm100_weights_noalloc(const float* seg_abs_sum, float* weigh
  *     (dlogprobs (onehot - p) - dentropy p (log p + entropy)) / temperature
  * dentropy nullable (then entropy may be too).
  */
+#define PUFF_LOGPROBS_STATS_ABOVE 384
 int puff_policy_sm100_logprobs(const void* logits, int dtype, const long long* actions,
                                long long outer, long long inner, long long vocab,
                                long long logits_outer_stride, long long logits_inner_stride,

@@ -583,7 +583,7 @@ puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const l
 // row took 316 and 278; instruction issue (81 and 87 %) bounds it, DRAM stands at 40 %.
 // Up to which size a row is small, against a warp a row (us, small / warp): 500000 x 256 bf16 forward 131 / 283 and backward
 // 207 / 260; 200000 x 333 86 / 131 and 131 / 133; 200000 x 500 117 / 131 and 184 / 139.
-constexpr int kLpSmall = 512, kLpSmallBackward = 384;
+constexpr int kLpSmall = 512, kLpSmallBackward = PUFF_LOGPROBS_STATS_ABOVE;      // 384
 template <typename T, bool ENT, int G, bool BACKWARD>
 __global__ void __launch_bounds__(kLpThreads)
 puff_logprobs_small_kernel(const T* __restrict__ logits, RowMap lmap, const long long* __restrict__ actions, RowMap amap,

@@ -191,6 +191,8 @@ template <typename I> LogprobArgs<I> logprob_args(const Tensor& logits, const Te
 
 // (logprobs, entropy or an empty tensor, row_stats or an empty tensor; undefined tensors for those with `bare`)
 template <typename I>
+bool stats_saved(const I& vocab) { return vocab > PUFF_LOGPROBS_STATS_ABOVE; }
+template <typename I>
 std::tuple<Tensor, Tensor, Tensor> logprobs_buffers(const Tensor& logits, const Tensor& actions, double temperature,
                                                     bool want_entropy, bool save, bool bare)
 {
@@ -198,7 +200,9 @@ std::tuple<Tensor, Tensor, Tensor> logprobs_buffers(const Tensor& logits, const 
     const auto opts = logits.options().dtype(torch::kFloat32);
     const auto sizes = Dims<I>::sizes(actions);
     return {Dims<I>::empty(sizes, opts), want_entropy ? Dims<I>::empty(sizes, opts) : bare ? Tensor() : torch::empty({0}, opts),
-            save ? Dims<I>::empty({Dims<I>::numel(actions), 2}, opts) : bare ? Tensor() : torch::empty({0, 2}, opts)};
+            save && stats_saved<I>(Dims<I>::sizes(logits)[logits.dim() - 1]) ? Dims<I>::empty({Dims<I>::numel(actions), 2}, opts)
+            : bare                                                           ? Tensor()
+                                                                             : torch::empty({0, 2}, opts)};
 }
 std::tuple<Tensor, Tensor, Tensor> logprobs_forward_meta(const Tensor& logits, const Tensor& actions, double temperature,
                                                          bool want_entropy, bool save)
@@ -217,7 +221,7 @@ std::tuple<Tensor, Tensor, Tensor> logprobs_run(const Tensor& logits, const Tens
                                         g.vocab, g.l.outer_stride, g.l.inner_stride, g.a.outer_stride, g.a.inner_stride,
                                         static_cast<float>(temperature), ptr<float>(std::get<0>(out)),
                                         want_entropy ? ptr<float>(std::get<1>(out)) : nullptr,
-                                        save ? ptr<float>(std::get<2>(out)) : nullptr, current_stream()),
+                                        save && stats_saved(g.vocab) ? ptr<float>(std::get<2>(out)) : nullptr, current_stream()),
              "puff_action_logprobs");
     return out;
 }
@@ -261,7 +265,9 @@ Tensor logprobs_backward_cuda(const Tensor& logits, const Tensor& actions, doubl
                               const OptTensor& entropy, const Tensor& dlogprobs, const OptTensor& dentropy)
 {
     const auto g = logprob_args<int64_t>(logits, actions);
-    check_f32(row_stats, logits, {g.rows, 2}, "row_stats");
+    check_f32(row_stats, logits, {stats_saved(g.vocab) ? g.rows : 0, 2}, "row_stats");
+    // where they are not read, some address that is none of the output's
+    const float* stats = stats_saved(g.vocab) ? ptr<const float>(row_stats) : ptr<const float>(actions);
     check_f32(dlogprobs, logits, actions.sizes(), "dlogprobs");
     if (present(dentropy)) {
         TORCH_CHECK(present(entropy), "dentropy needs the entropy of the forward pass");
@@ -274,7 +280,7 @@ Tensor logprobs_backward_cuda(const Tensor& logits, const Tensor& actions, doubl
     check_rc(puff_policy_sm100_logprobs_backward(
                  logits.data_ptr(), g.dtype, ptr<const long long>(actions), g.l.outer, g.l.inner, g.vocab,
                  g.l.outer_stride, g.l.inner_stride, g.a.outer_stride, g.a.inner_stride, static_cast<float>(temperature),
-                 ptr<const float>(row_stats), present(dentropy) ? ptr<float>(entropy) : nullptr,
+                 stats, present(dentropy) ? ptr<float>(entropy) : nullptr,
                  ptr<const float>(dlogprobs), ptr<float>(dentropy), dlogits.data_ptr(), current_stream()),
              "puff_action_logprobs_backward");
     return dlogits;

@@ -252,3 +252,16 @@ def test_shapes_are_still_refused_while_tracing():
                      (lambda z: pb.gated_recurrence_step(z, z, meta(2, 9))[0], (2, 8))):
         with pytest.raises(RuntimeError, match="shape"):
             make_fx(f, tracing_mode="symbolic")(meta(*shape))
+
+
+@pytest.mark.parametrize("vocab", [1, 18, 384, 385, 5000])
+def test_row_statistics_are_kept_only_for_rows_that_need_them(vocab):
+    """The backward pass of small rows works the statistics out again: nothing is saved for it."""
+    import pufferlib_b200 as pb
+    pb.action_logprobs(meta(2, 3), actions(2))
+    _, _, stats = torch.ops.pufferlib.puff_action_logprobs_forward(meta(7, vocab), actions(7), 1.0, True, True)
+    assert stats.shape == ((0, 2) if vocab <= 384 else (7, 2))
+    saved = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t.numel()) or t, lambda t: t):
+        pb.action_logprobs(meta(7, vocab, grad=True), actions(7), entropy=False)
+    assert sum(saved) == 7 * vocab + 7 + (14 if vocab > 384 else 0)
