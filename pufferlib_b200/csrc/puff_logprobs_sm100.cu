@@ -8,7 +8,9 @@
 // pufferlib/pytorch.py sample_logits), for action heads of a few entries up to vocabularies of 10^5 and more.
 //
 // Memory-bound in principle, 2 to 4 bytes a logit read once forward, read and written once backward; in practice the
-// exponentials and the instructions around them are close behind: five or so a 16-bit logit fit under the copy rate.
+// exponentials and the instructions around them are close behind: five or so a 16-bit logit fit under the copy rate.  That
+// is why every exponential is one ex2.approx, good to 4 half steps of fp32 where expf is good to 2: 524288 x 18 fp32 is
+// 9.7e-8 off 64 bits (relative, all outputs together), fp32 arithmetic with expf 6.3e-8.
 // On a B200 that copies at 6.55 TB/s: 4096 x 131072 bf16 195 us forward with entropy (5.5 TB/s), 176 without, 328
 // backward (6.55); 524288 x 18 fp32 20 and 29 us; 8 x 131072 bf16 about 5 us, a cluster of eight CTAs a row.
 #include <cooperative_groups.h>
@@ -226,8 +228,9 @@ __device__ __forceinline__ void soft_warp_join(SoftSums& a, float c)
 
 // A thread's own ring of 16-byte slots in shared memory, filled by asynchronous copies and read by nobody else, so that
 // no thread waits for another: kRing - 1 groups of kGroup vectors are on their way while one is used, for no registers.
-// (4096 x 131072 bf16 with entropy, groups x depth at four CTAs an SM: 2 x 5 192 us, 2 x 3 195, 3 x 3 186, 4 x 2 188;
-// without entropy 176, 180, 178, 182; 2040 x 50001 fp16 53, 57, 55, 59.)
+// (4096 x 131072 bf16 with entropy, groups x depth at four CTAs an SM, measured while each thread had a reference of its
+// own from the start: 2 x 5 192 us, 2 x 3 195, 3 x 3 186, 4 x 2 188; without entropy 176, 180, 178, 182; 2040 x 50001 fp16
+// 53, 57, 55, 59.)
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kGroup = 2, kRing = 5;
@@ -464,7 +467,7 @@ struct GradientRow {
     unsigned shift;
     bool none;
 };
-// vectors first, first + 32, ... of the row, U of them; 4 x 131072 rows: eight at once 337 us, four 369; shifted ones need
+// vectors first, first + 32, ... of the row, U of them; 4096 x 131072 bf16: eight at once 328 us, four 369; shifted ones need
 // twice the registers, and eight of those spill (143 us against 94 for 2040 x 50001)
 template <typename T, bool ENT, int U, bool SHIFTED>
 __device__ __forceinline__ void gradient_vectors(const GradientRow& row, const RowGradient& grad, long long first)
@@ -578,7 +581,8 @@ puff_logprobs_backward_kernel(const T* __restrict__ logits, RowMap lmap, const l
 // Small rows, both directions.  A CTA brings 256 / G rows into shared memory by 16-byte copies of their common span,
 // wherever rows begin; G threads then work on a row from there (fewer than 33 elements each), and the backward pass
 // writes gradients over the logits and copies the span out.  The maximum and the sums are computed
-// again in the backward pass: reading them back would cost more than the arithmetic.  Rows start at different banks:
+// again in the backward pass, so that the forward pass keeps nothing of a row (reading 8 bytes of each back instead has not
+// been measured).  Rows start at different banks:
 // row i of the tile begins its walk i * skew elements in.  524288 x 18 fp32: 20 us forward and 29 backward, where a warp a
 // row took 316 and 278; instruction issue (81 and 87 %) bounds it, DRAM stands at 40 %.
 // Up to which size a row is small, against a warp a row (us, small / warp): 500000 x 256 bf16 forward 131 / 283 and backward

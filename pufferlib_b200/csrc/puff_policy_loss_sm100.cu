@@ -135,7 +135,9 @@ template <> struct Pack<4> {
     }
 };
 
-// Sums over a few tokens in fp32, joined in fp64; numbers of tokens are whole
+// Sums over a thread's one or four tokens in fp32, joined in fp64: three roundings of four tokens' sum at most, where fp64
+// from the tokens on was among what took 415 us.  The policy terms, which nearly cancel, carry their roundings along.
+// Numbers of tokens are whole.
 struct LossSums {
     float policy, policy_rest, kl, entropy, neg_d, excess;
 };
@@ -321,6 +323,7 @@ puff_policy_loss_final_kernel(const double* __restrict__ partial, int n_partial,
     }
 }
 
+// slope times weight, dloss and, for sequences, the row's scale: two or three fp32 products of factors rounded once each.
 // VEC 4 with row_scale: four adjacent tokens are of one row (steps divisible by four)
 template <int VEC>
 __global__ void __launch_bounds__(kLossThreads)

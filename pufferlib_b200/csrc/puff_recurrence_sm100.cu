@@ -11,8 +11,8 @@
 //
 // Memory-bound: three elements moved a step forward, five backward; the arithmetic behind them, two special functions and
 // some twenty instructions a step for two channels, is close to the bound, so what surrounds it (addresses, joins, waits)
-// decides.  8192 x 64 x 128 bf16: 79 us forward (5.1 TB/s of 6.55) and 117 backward (5.7); fp32 125 and 211 (6.4);
-// 256 x 4096 x 128 fp32 281 and 453.  One thread a channel, step after step, took 1904 us for the first pair.
+// decides.  8192 x 64 x 128 bf16: 79 us forward (5.1 TB/s of 6.55) and 118 backward (5.7); fp32 128 and 209 (6.4);
+// 256 x 4096 x 128 fp32 276 and 450.  One thread a channel, step after step, took 1904 us for the first pair.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -5,7 +5,9 @@ and `loss.backward()` (pufferl.py:385-422; sample_logits of
 pufferlib/pytorch.py), as differentiable operators over the experience buffers'
 `[segments, horizon]` layout.  Like the advantage ops they run on an sm_100 GPU
 only, on the current stream of the tensors' device, and raise when the extension
-is missing.  No second derivatives.
+is missing.  Reverse-mode gradients only: second derivatives and forward mode
+raise.  Activation checkpointing and ahead-of-time tracing (torch.compile, sizes
+that change included) take them as any other operator.
 """
 import contextlib
 
