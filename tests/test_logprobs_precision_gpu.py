@@ -6,7 +6,10 @@ s = 1 + e, e = exp(-d), and nothing else is added, so that few roundings are lef
   1          4 U from ex2.approx of the remainder of max * log2(e) twice: in the term and in the factor that takes it out
   s          2 U: one sum, one product
 so s is off by 10 U + e (4 + 3 d) U at most, log s by as much and 2 U log s, and the log-probability by one more rounding
-of each.  The entropy log s - u / s has e d (ex2's 4, the argument's 3 d, and 8 more) U on top."""
+of each.  The entropy log s - u / s has e d (ex2's 4, the argument's 3 d, and 8 more) U on top.
+
+That is with the sums taken relative to the row's maximum.  The kernel's reference may lie 4.4 bits below it, which on
+paper is 3 U more for the argument of the largest term; what is met here is 3 U in all."""
 import math
 
 import pytest
