@@ -176,7 +176,8 @@ __device__ __forceinline__ float2 soft_terms(const SoftScale& z, const uint4 (&q
 // The reference m need not be the maximum: it is kept while the new terms add up to no more than 5/4 of as many ones, so
 // that it lies at most 4.4 bits below the maximum (16-bit types; fp32 3.4), which write_row takes out again.  That spares
 // looking for the maximum everywhere (half an instruction an element, and everything waiting for it: an exact one shared by
-// the warp took 5 to 19 % longer).  Otherwise: the vectors' maximum, one rescaling, and their terms again.
+// the warp took 5 to 19 % longer).  Otherwise: the vectors' maximum, one rescaling, and their terms again, which rows pay
+// for that climb all along: 4096 x 131072 bf16 334 us from -20 to 20, 195 without a trend.
 template <typename T, bool ENT, int K>
 __device__ __forceinline__ void soft_add_vectors(SoftSums& a, SoftScale& z, const uint4 (&q)[K], unsigned valid, float c)
 {
